@@ -1,0 +1,627 @@
+// Mixture-of-experts routing and row exchange.
+//
+// Router.  For a token with logits z[0..E) the k experts with the largest
+// logits are chosen (ties: the lowest index) and weighted by
+//   normalised:  w_j = exp(z_j - m) / sum_{i chosen} exp(z_i - m)
+//   otherwise:   w_j = exp(z_j - m) / sum_{all e}    exp(z_e - m),   m = max z
+// A row whose logits are all -inf gets weights 0 (not 0/0).  The gradient is
+//   normalised:  dz_j = w_j (dw_j - sum_i w_i dw_i) on the chosen, 0 elsewhere
+//   otherwise:   dz_e = p_e (dw_e [chosen] - sum_i w_i dw_i)
+// The choices c = t*k + j are grouped by expert, stably: slots[c] is the row of
+// choice c in the grouped order, order[slot] the choice of that row, and
+// offsets[e] the first row of expert e.  Only integer atomics are used, so the
+// result does not depend on the order of execution.
+//
+// Exchange.  dispatch copies token rows to their k grouped rows, combine forms
+// the weighted sum of a token's k rows; each is the other's gradient.  All four
+// are bound by memory: one thread owns 8 columns of one token, so the token's
+// row is read (or written) once whatever k is, and sums are in fp32 with one
+// rounding to bf16 at the end.
+#include "common.cuh"
+
+namespace tdb {
+namespace moe {
+
+constexpr int kMaxExperts = 512;
+constexpr int kMaxTopK = 16;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kTokensPerBlock = 64;  // routing: 8 tokens per warp; up to 64 tokens are routed by one launch
+
+// Monotone map float -> uint32 (larger float, larger key); both zeros map to
+// the same key, NaN to the largest.  Every key of a float is > 0.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return 0xffffffffu;
+  const uint32_t u = v == 0.f ? 0u : __float_as_uint(v);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float load_logit(const T* p);
+template <>
+__device__ __forceinline__ float load_logit<float>(const float* p) { return __ldg(p); }
+template <>
+__device__ __forceinline__ float load_logit<uint16_t>(const uint16_t* p) { return bf16_bits_to_float(__ldg(p)); }
+
+// One warp: the top k of one token.  Lane j < k returns the j-th choice's id
+// and weight.  NP = experts per lane (expert i*32 + lane).
+template <int NP, typename T>
+__device__ __forceinline__ void choose(const T* row, int E, int k, int normalize, int& my_id, float& my_w) {
+  const int lane = threadIdx.x & 31;
+  float v[NP];
+  uint32_t key[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int e = i * 32 + lane;
+    v[i] = e < E ? load_logit<T>(row + e) : -INFINITY;
+    key[i] = e < E ? order_key(v[i]) : 0u;
+  }
+  float my_z = -INFINITY, top = -INFINITY;
+  my_id = 0;
+  for (int j = 0; j < k; ++j) {
+    uint32_t best = key[0];
+    int at = 0;
+#pragma unroll
+    for (int i = 1; i < NP; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        at = i;
+      }
+    const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+    const uint32_t id = __reduce_min_sync(0xffffffffu, best == m ? uint32_t(at * 32 + lane) : 0x7fffffffu);
+    if ((id & 31u) == uint32_t(lane)) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        if (uint32_t(i) == id >> 5) key[i] = 0u;
+    }
+    const float z = key_value(m);
+    if (j == 0) top = z;
+    if (lane == j) {
+      my_id = int(id);
+      my_z = z;
+    }
+  }
+  if (top == -INFINITY) {  // no expert is open to this token
+    my_w = 0.f;
+    return;
+  }
+  const float e = lane < k ? expf(my_z - top) : 0.f;
+  float s;
+  if (normalize) {
+    s = warp_sum(e);
+  } else {
+    float part = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) part += i * 32 + lane < E ? expf(v[i] - top) : 0.f;
+    s = warp_sum(part);
+  }
+  my_w = e / s;
+}
+
+// Exclusive scan of total[0..E) into start[0..E], by one warp.
+__device__ __forceinline__ void scan_experts(const int* total, int* start, int E) {
+  const int lane = threadIdx.x & 31;
+  const int per = (E + 31) / 32;
+  int sum = 0;
+  for (int i = 0; i < per; ++i) {
+    const int e = lane * per + i;
+    if (e < E) sum += total[e];
+  }
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += up;
+  }
+  int run = inc - sum;
+  for (int i = 0; i < per; ++i) {
+    const int e = lane * per + i;
+    if (e < E) {
+      start[e] = run;
+      run += total[e];
+    }
+  }
+  if (lane == 31) start[E] = inc;
+}
+
+// Stable ranks of the block's choices [c0, c1): base[e] is the first slot of
+// the block's choices of expert e.  Warp w owns a contiguous share, so ranks
+// follow the choice index.  wh: [kWarps][E] shared ints.
+__device__ __forceinline__ void rank_choices(const int* ids, int c0, int c1, int E, const int* base, int* wh,
+                                             int* __restrict__ order, int* __restrict__ slots) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int share = ((c1 - c0 + kWarps - 1) / kWarps + 31) / 32 * 32;
+  const int lo = min(c0 + warp * share, c1), hi = min(lo + share, c1);
+  for (int i = threadIdx.x; i < kWarps * E; i += kThreads) wh[i] = 0;
+  __syncthreads();
+  for (int c = lo + lane; c < hi; c += 32) atomicAdd(&wh[warp * E + ids[c]], 1);
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kThreads) {
+    int run = base[e];
+    for (int w = 0; w < kWarps; ++w) {
+      const int n = wh[w * E + e];
+      wh[w * E + e] = run;
+      run += n;
+    }
+  }
+  __syncthreads();
+  for (int c = lo; c < hi; c += 32) {
+    const int mine = c + lane;
+    const bool on = mine < hi;
+    const int id = on ? ids[mine] : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, id);
+    int first = 0;
+    if (on) first = wh[warp * E + id];
+    __syncwarp();
+    if (on) {
+      const int slot = first + __popc(same & ((1u << lane) - 1u));
+      slots[mine] = slot;
+      order[slot] = mine;
+      if ((same >> lane) == 1u) wh[warp * E + id] = slot + 1;  // the last of its group
+    }
+    __syncwarp();
+  }
+}
+
+// Top k, weights and the block's expert counts; with one block also the
+// grouping (hist unused).
+template <int NP, typename T>
+__global__ void __launch_bounds__(kThreads) choose_kernel(const T* __restrict__ logits, int64_t ld, int tokens, int E,
+                                                          int k, int normalize, int* ids, float* __restrict__ weights,
+                                                          int* __restrict__ hist, int* __restrict__ offsets,
+                                                          int* __restrict__ order, int* __restrict__ slots) {
+  extern __shared__ int sh[];
+  int* count = sh;  // [E]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < E; e += kThreads) count[e] = 0;
+  __syncthreads();
+  const int t0 = blockIdx.x * kTokensPerBlock, t1 = min(t0 + kTokensPerBlock, tokens);
+  for (int t = t0 + warp; t < t1; t += kWarps) {
+    int id;
+    float w;
+    choose<NP, T>(logits + int64_t(t) * ld, E, k, normalize, id, w);
+    if (lane < k) {
+      ids[int64_t(t) * k + lane] = id;
+      weights[int64_t(t) * k + lane] = w;
+      atomicAdd(&count[id], 1);
+    }
+  }
+  __syncthreads();
+  if (gridDim.x > 1) {
+    for (int e = threadIdx.x; e < E; e += kThreads) hist[int64_t(blockIdx.x) * E + e] = count[e];
+    return;
+  }
+  int* start = sh + E;           // [E + 1]
+  int* wh = start + E + 1;       // [kWarps][E]
+  if (warp == 0) scan_experts(count, start, E);
+  __syncthreads();
+  for (int e = threadIdx.x; e <= E; e += kThreads) offsets[e] = start[e];
+  rank_choices(ids, 0, tokens * k, E, start, wh, order, slots);
+}
+
+// Slots of one block's choices from every block's counts.
+__global__ void __launch_bounds__(kThreads) group_kernel(const int* __restrict__ ids, const int* __restrict__ hist,
+                                                         int blocks, int tokens, int E, int k, int* __restrict__ offsets,
+                                                         int* __restrict__ order, int* __restrict__ slots) {
+  extern __shared__ int sh[];
+  int* total = sh;          // [E]
+  int* before = sh + E;     // [E]
+  int* start = before + E;  // [E + 1]
+  int* wh = start + E + 1;  // [kWarps][E]
+  for (int e = threadIdx.x; e < E; e += kThreads) total[e] = before[e] = 0;
+  __syncthreads();
+  // thread (lane over experts, group over blocks): coalesced rows of hist
+  const int wide = E < kThreads ? (E + 31) / 32 * 32 : kThreads;
+  const int groups = kThreads / wide;
+  const int part = threadIdx.x / wide;
+  if (part < groups) {
+    for (int e = threadIdx.x % wide; e < E; e += wide) {
+      int all = 0, mine = 0;
+#pragma unroll 8
+      for (int b = part; b < blocks; b += groups) {
+        const int n = __ldg(hist + int64_t(b) * E + e);
+        all += n;
+        mine += b < int(blockIdx.x) ? n : 0;
+      }
+      atomicAdd(&total[e], all);
+      atomicAdd(&before[e], mine);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) scan_experts(total, start, E);
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= E; e += kThreads) offsets[e] = start[e];
+  for (int e = threadIdx.x; e < E; e += kThreads) before[e] += start[e];
+  __syncthreads();
+  const int t0 = blockIdx.x * kTokensPerBlock, t1 = min(t0 + kTokensPerBlock, tokens);
+  rank_choices(ids, t0 * k, t1 * k, E, before, wh, order, slots);
+}
+
+__device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_logit(uint16_t* p, float v) { *p = float_to_bf16_bits(v); }
+
+// One warp per token.
+template <int NP, typename T, typename O>
+__global__ void __launch_bounds__(kThreads) route_bwd_kernel(const T* __restrict__ logits, int64_t ld, int tokens, int E,
+                                                             int k, int normalize, const int* __restrict__ ids,
+                                                             const float* __restrict__ weights,
+                                                             const float* __restrict__ dweights, O* __restrict__ out,
+                                                             int64_t ld_out) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  int id = -1;
+  float w = 0.f, dw = 0.f;
+  if (lane < k) {
+    id = ids[t * k + lane];
+    w = weights[t * k + lane];
+    dw = dweights[t * k + lane];
+  }
+  const float dot = warp_sum(w * dw);
+  O* o = out + t * ld_out;
+  if (normalize) {
+    const float g = w * (dw - dot);
+    float r[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) r[i] = 0.f;
+    for (int j = 0; j < k; ++j) {
+      const int at = __shfl_sync(0xffffffffu, id, j);
+      const float gj = __shfl_sync(0xffffffffu, g, j);
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        if (at == i * 32 + lane) r[i] = gj;
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      if (i * 32 + lane < E) store_logit(o + i * 32 + lane, r[i]);
+    return;
+  }
+  float z[NP], d[NP], top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    z[i] = i * 32 + lane < E ? load_logit<T>(logits + t * ld + i * 32 + lane) : -INFINITY;
+    top = fmaxf(top, z[i]);
+    d[i] = -dot;
+  }
+#pragma unroll
+  for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+  for (int j = 0; j < k; ++j) {
+    const int at = __shfl_sync(0xffffffffu, id, j);
+    const float gj = __shfl_sync(0xffffffffu, dw, j);
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      if (at == i * 32 + lane) d[i] += gj;
+  }
+  float part = 0.f;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    z[i] = top == -INFINITY ? 0.f : expf(z[i] - top);  // padding lanes: exp(-inf) = 0
+    part += z[i];
+  }
+  const float s = warp_sum(part);
+  const float inv = s > 0.f ? 1.f / s : (s == 0.f ? 0.f : s);  // all -inf: zero gradient; NaN stays NaN
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+    if (i * 32 + lane < E) store_logit(o + i * 32 + lane, z[i] * inv * d[i]);
+}
+
+// ---------------------------------------------------------------------------
+// Exchange.  Block (x: threads of a token, y: tokens); 8 bf16 columns per
+// thread and step.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
+  const uint32_t a[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(a[i] << 16);
+    v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+// The token's k slots (and weights) into shared memory; a slot outside the
+// grouped rows is recorded and becomes -1.
+__device__ __forceinline__ void load_choices(const int* __restrict__ slots, const float* __restrict__ weights, int64_t t,
+                                             int tokens, int k, int* s_slot, float* s_w, int* status) {
+  for (int j = threadIdx.x; j < k; j += blockDim.x) {
+    int s = -1;
+    if (t < tokens) {
+      s = slots[t * k + j];
+      if (uint32_t(s) >= uint32_t(tokens) * uint32_t(k)) {
+        record_status(status, kBadArgument, 200, int(t), s);
+        s = -1;
+      }
+    }
+    s_slot[j] = s;
+    if (weights) s_w[j] = t < tokens ? weights[t * k + j] : 0.f;
+  }
+  __syncthreads();
+}
+
+__global__ void __launch_bounds__(kThreads) dispatch_kernel(const uint16_t* __restrict__ x, int64_t ldx, int tokens, int k,
+                                                            int vecs, const int* __restrict__ slots,
+                                                            uint16_t* __restrict__ out, int64_t ldo, int* status) {
+  __shared__ int s_slot[8][kMaxTopK];
+  const int64_t t = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+  load_choices(slots, nullptr, t, tokens, k, s_slot[threadIdx.y], nullptr, status);
+  if (t >= tokens) return;
+  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(x + t * ldx) + v);
+    for (int j = 0; j < k; ++j) {
+      const int s = s_slot[threadIdx.y][j];
+      if (s >= 0) reinterpret_cast<uint4*>(out + int64_t(s) * ldo)[v] = q;
+    }
+  }
+}
+
+// out[t] = residual[t] + sum_j w_j y[slot_j] (weights null: all 1).
+__global__ void __launch_bounds__(kThreads) combine_kernel(const uint16_t* __restrict__ y, int64_t ldy, int tokens, int k,
+                                                           int vecs, const int* __restrict__ slots,
+                                                           const float* __restrict__ weights,
+                                                           const uint16_t* __restrict__ residual, int64_t ldr,
+                                                           uint16_t* __restrict__ out, int64_t ldo, int* status) {
+  __shared__ int s_slot[8][kMaxTopK];
+  __shared__ float s_w[8][kMaxTopK];
+  const int64_t t = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+  load_choices(slots, weights, t, tokens, k, s_slot[threadIdx.y], s_w[threadIdx.y], status);
+  if (t >= tokens) return;
+  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+    float acc[8] = {};
+    for (int j0 = 0; j0 < k; j0 += 4) {
+      uint4 q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = j0 + i < k ? s_slot[threadIdx.y][j0 + i] : -1;
+        q[i] = s >= 0 ? __ldg(reinterpret_cast<const uint4*>(y + int64_t(s) * ldy) + v) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (j0 + i >= k) break;
+        float f[8];
+        unpack8(q[i], f);
+        const float w = weights ? s_w[threadIdx.y][j0 + i] : 1.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[c] += w * f[c];
+      }
+    }
+    if (residual) {
+      float f[8];
+      unpack8(__ldg(reinterpret_cast<const uint4*>(residual + t * ldr) + v), f);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) acc[c] += f[c];
+    }
+    reinterpret_cast<uint4*>(out + t * ldo)[v] = pack8(acc);
+  }
+}
+
+// dy[slot_j] = w_j dout[t];  dw_j = <dout[t], y[slot_j]> (fp32).
+__global__ void __launch_bounds__(kThreads) combine_bwd_kernel(const uint16_t* __restrict__ dout, int64_t ldd,
+                                                               const uint16_t* __restrict__ y, int64_t ldy, int tokens,
+                                                               int k, int vecs, const int* __restrict__ slots,
+                                                               const float* __restrict__ weights,
+                                                               uint16_t* __restrict__ dy, int64_t lddy,
+                                                               float* __restrict__ dweights, int* status) {
+  __shared__ int s_slot[8][kMaxTopK];
+  __shared__ float s_w[8][kMaxTopK];
+  __shared__ float s_dot[kWarps][kMaxTopK];
+  const int64_t t = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+  load_choices(slots, weights, t, tokens, k, s_slot[threadIdx.y], s_w[threadIdx.y], status);
+  const int lane = threadIdx.x & 31;
+  const int warps = blockDim.x >> 5, warp = threadIdx.y * warps + (threadIdx.x >> 5);
+  for (int j0 = 0; j0 < k; j0 += 4) {  // four choices at a time: dout is read again from L1/L2 for k > 4
+    float dot[4] = {};
+    if (t < tokens) {
+      for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+        uint4 q[4];
+        int s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[i] = j0 + i < k ? s_slot[threadIdx.y][j0 + i] : -1;
+          q[i] = s[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(y + int64_t(s[i]) * ldy) + v) : make_uint4(0, 0, 0, 0);
+        }
+        float d[8];
+        unpack8(__ldg(reinterpret_cast<const uint4*>(dout + t * ldd) + v), d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (s[i] < 0) continue;
+          float f[8], g[8];
+          unpack8(q[i], f);
+          const float w = s_w[threadIdx.y][j0 + i];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            dot[i] += d[c] * f[c];
+            g[c] = w * d[c];
+          }
+          reinterpret_cast<uint4*>(dy + int64_t(s[i]) * lddy)[v] = pack8(g);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float sum = warp_sum(dot[i]);
+      if (lane == 0 && j0 + i < k) s_dot[warp][j0 + i] = sum;
+    }
+  }
+  __syncthreads();
+  if (t < tokens)
+    for (int j = threadIdx.x; j < k; j += blockDim.x) {
+      float sum = 0.f;
+      for (int w = 0; w < warps; ++w) sum += s_dot[threadIdx.y * warps + w][j];
+      dweights[t * k + j] = sum;
+    }
+}
+
+static dim3 exchange_block(int vecs) {
+  int x = (vecs + 31) / 32 * 32;
+  if (x > kThreads) x = kThreads;
+  int y = kThreads / x;
+  return dim3(x, y > 8 ? 8 : y);
+}
+
+static bool bad_rows(const void* p, int64_t ld, int H) {
+  return !p || reinterpret_cast<uintptr_t>(p) % 16 || ld % 8 || ld < H;
+}
+
+template <typename T>
+static int route(const T* logits, int64_t ld, int tokens, int E, int k, int normalize, int* ids, float* weights,
+                 int* offsets, int* order, int* slots, int* hist, cudaStream_t s) {
+  const int blocks = tokens > 0 ? (tokens + kTokensPerBlock - 1) / kTokensPerBlock : 1;
+  const size_t one = size_t(2 * E + 1 + kWarps * E) * 4, many = size_t(E) * 4;
+  const size_t smem = blocks == 1 ? one : many;
+#define TDB_CHOOSE(NP) \
+  choose_kernel<NP, T><<<blocks, kThreads, smem, s>>>(logits, ld, tokens, E, k, normalize, ids, weights, hist, offsets, order, slots)
+  if (E <= 32) TDB_CHOOSE(1);
+  else if (E <= 64) TDB_CHOOSE(2);
+  else if (E <= 128) TDB_CHOOSE(4);
+  else if (E <= 256) TDB_CHOOSE(8);
+  else TDB_CHOOSE(16);
+#undef TDB_CHOOSE
+  tdb_host::launched(1);
+  if (blocks > 1) {
+    group_kernel<<<blocks, kThreads, size_t(3 * E + 1 + kWarps * E) * 4, s>>>(ids, hist, blocks, tokens, E, k, offsets,
+                                                                             order, slots);
+    tdb_host::launched(1);
+  }
+  return int(cudaGetLastError());
+}
+
+template <typename T, typename O>
+static int route_bwd(const T* logits, int64_t ld, int tokens, int E, int k, int normalize, const int* ids,
+                     const float* weights, const float* dweights, O* out, int64_t ld_out, cudaStream_t s) {
+  const int blocks = (tokens + kWarps - 1) / kWarps;
+#define TDB_BWD(NP) \
+  route_bwd_kernel<NP, T, O><<<blocks, kThreads, 0, s>>>(logits, ld, tokens, E, k, normalize, ids, weights, dweights, out, ld_out)
+  if (E <= 32) TDB_BWD(1);
+  else if (E <= 64) TDB_BWD(2);
+  else if (E <= 128) TDB_BWD(4);
+  else if (E <= 256) TDB_BWD(8);
+  else TDB_BWD(16);
+#undef TDB_BWD
+  tdb_host::launched(1);
+  return int(cudaGetLastError());
+}
+
+static int check_route(const char* what, int64_t ld, int tokens, int E, int k) {
+  if (tokens < 0 || E < 1 || E > kMaxExperts || k < 1 || k > kMaxTopK || k > E || ld < E ||
+      int64_t(tokens) * k >= (int64_t(1) << 31))
+    return tdb_host::fail(int(cudaErrorInvalidValue),
+                          "%s: 1..%d experts, 1..%d choices per token (at most the experts), tokens * choices < 2^31", what,
+                          kMaxExperts, kMaxTopK);
+  return 0;
+}
+
+static int check_exchange(const char* what, int tokens, int k, int H) {
+  if (tokens < 0 || k < 1 || k > kMaxTopK || H < 8 || H % 8 || int64_t(tokens) * k >= (int64_t(1) << 31))
+    return tdb_host::fail(int(cudaErrorInvalidValue), "%s: 1..%d choices per token, columns a multiple of 8", what,
+                          kMaxTopK);
+  return 0;
+}
+
+static int bad_alignment(const char* what) {
+  return tdb_host::fail(int(cudaErrorInvalidValue), "%s: rows must be 16-byte aligned and at least as wide as the columns", what);
+}
+
+}  // namespace moe
+}  // namespace tdb
+
+using namespace tdb;
+using namespace tdb::moe;
+
+// Ints of scratch that tdb_moe_route needs (0: none).
+TDB_API long long tdb_moe_route_scratch_ints(int tokens, int E) {
+  const int64_t blocks = (int64_t(tokens) + kTokensPerBlock - 1) / kTokensPerBlock;
+  return blocks > 1 ? blocks * E : 0;
+}
+
+// logits fp32 (logits_bf16 = 0) or bf16 [tokens, E] (row stride ld) -> ids,
+// weights, slots, order [tokens * k], offsets [E + 1].
+TDB_API int tdb_moe_route(const void* logits, int logits_bf16, int64_t ld, int tokens, int E, int k, int normalize,
+                          int* ids, float* weights, int* offsets, int* order, int* slots, int* scratch, void* stream) {
+  if (int rc = check_route("moe route", ld, tokens, E, k)) return rc;
+  if (!offsets || (tokens > 0 && (!logits || !ids || !weights || !order || !slots)) ||
+      (tokens > kTokensPerBlock && !scratch))
+    return tdb_host::fail(int(cudaErrorInvalidValue), "moe route: null pointer");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (logits_bf16)
+    return route(static_cast<const uint16_t*>(logits), ld, tokens, E, k, normalize, ids, weights, offsets, order, slots,
+                 scratch, s);
+  return route(static_cast<const float*>(logits), ld, tokens, E, k, normalize, ids, weights, offsets, order, slots,
+               scratch, s);
+}
+
+// dlogits (fp32 or bf16, [tokens, E], row stride ld_out) from dweights; the
+// logits are read only when the weights were not normalised.
+TDB_API int tdb_moe_route_bwd(const void* logits, int logits_bf16, int64_t ld, int tokens, int E, int k, int normalize,
+                              const int* ids, const float* weights, const float* dweights, void* dlogits, int out_bf16,
+                              int64_t ld_out, void* stream) {
+  if (int rc = check_route("moe route backward", ld < ld_out ? ld : ld_out, tokens, E, k)) return rc;
+  if (tokens == 0) return 0;
+  if (!logits || !ids || !weights || !dweights || !dlogits)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "moe route backward: null pointer");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (logits_bf16) {
+    const uint16_t* z = static_cast<const uint16_t*>(logits);
+    return out_bf16 ? route_bwd(z, ld, tokens, E, k, normalize, ids, weights, dweights, static_cast<uint16_t*>(dlogits), ld_out, s)
+                    : route_bwd(z, ld, tokens, E, k, normalize, ids, weights, dweights, static_cast<float*>(dlogits), ld_out, s);
+  }
+  const float* z = static_cast<const float*>(logits);
+  return out_bf16 ? route_bwd(z, ld, tokens, E, k, normalize, ids, weights, dweights, static_cast<uint16_t*>(dlogits), ld_out, s)
+                  : route_bwd(z, ld, tokens, E, k, normalize, ids, weights, dweights, static_cast<float*>(dlogits), ld_out, s);
+}
+
+// out[slots[t*k + j]] = x[t] (bf16 rows of H columns).
+TDB_API int tdb_moe_dispatch(const void* x, int64_t ldx, int tokens, int k, int H, const int* slots, void* out,
+                             int64_t ldo, void* stream) {
+  if (int rc = check_exchange("moe dispatch", tokens, k, H)) return rc;
+  if (tokens == 0) return 0;
+  if (!slots || bad_rows(x, ldx, H) || bad_rows(out, ldo, H)) return bad_alignment("moe dispatch");
+  const dim3 block = exchange_block(H / 8);
+  dispatch_kernel<<<(tokens + block.y - 1) / block.y, block, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint16_t*>(x), ldx, tokens, k, H / 8, slots, static_cast<uint16_t*>(out), ldo,
+      tdb_host::status_ptr());
+  tdb_host::launched(1);
+  return int(cudaGetLastError());
+}
+
+// out[t] = (residual[t]) + sum_j (weights[t*k + j] or 1) * y[slots[t*k + j]].
+TDB_API int tdb_moe_combine(const void* y, int64_t ldy, int tokens, int k, int H, const int* slots, const float* weights,
+                            const void* residual, int64_t ldr, void* out, int64_t ldo, void* stream) {
+  if (int rc = check_exchange("moe combine", tokens, k, H)) return rc;
+  if (tokens == 0) return 0;
+  if (!slots || bad_rows(y, ldy, H) || bad_rows(out, ldo, H) || (residual && bad_rows(residual, ldr, H)))
+    return bad_alignment("moe combine");
+  const dim3 block = exchange_block(H / 8);
+  combine_kernel<<<(tokens + block.y - 1) / block.y, block, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint16_t*>(y), ldy, tokens, k, H / 8, slots, weights, static_cast<const uint16_t*>(residual), ldr,
+      static_cast<uint16_t*>(out), ldo, tdb_host::status_ptr());
+  tdb_host::launched(1);
+  return int(cudaGetLastError());
+}
+
+// Gradients of tdb_moe_combine: dy (grouped rows) and dweights [tokens * k].
+TDB_API int tdb_moe_combine_bwd(const void* dout, int64_t ldd, const void* y, int64_t ldy, int tokens, int k, int H,
+                                const int* slots, const float* weights, void* dy, int64_t lddy, float* dweights,
+                                void* stream) {
+  if (int rc = check_exchange("moe combine backward", tokens, k, H)) return rc;
+  if (tokens == 0) return 0;
+  if (!slots || !weights || !dweights || bad_rows(dout, ldd, H) || bad_rows(y, ldy, H) || bad_rows(dy, lddy, H))
+    return bad_alignment("moe combine backward");
+  const dim3 block = exchange_block(H / 8);
+  combine_bwd_kernel<<<(tokens + block.y - 1) / block.y, block, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint16_t*>(dout), ldd, static_cast<const uint16_t*>(y), ldy, tokens, k, H / 8, slots, weights,
+      static_cast<uint16_t*>(dy), lddy, dweights, tdb_host::status_ptr());
+  tdb_host::launched(1);
+  return int(cudaGetLastError());
+}

@@ -162,6 +162,20 @@ int tdb_xent_combine(const float* all_stats, int world, int rows, float* gstats,
 int tdb_xent_grad(void* logits, int64_t ld, const int64_t* targets, int64_t vocab_start, int valid_cols, int cols,
                   int rows, const float* gstats, float scale, void* stream);
 
+/* ---- mixture-of-experts routing and row exchange (moe.cu) ---------------- */
+long long tdb_moe_route_scratch_ints(int tokens, int E);
+int tdb_moe_route(const void* logits, int logits_bf16, int64_t ld, int tokens, int E, int k, int normalize, int* ids,
+                  float* weights, int* offsets, int* order, int* slots, int* scratch, void* stream);
+int tdb_moe_route_bwd(const void* logits, int logits_bf16, int64_t ld, int tokens, int E, int k, int normalize,
+                      const int* ids, const float* weights, const float* dweights, void* dlogits, int out_bf16,
+                      int64_t ld_out, void* stream);
+int tdb_moe_dispatch(const void* x, int64_t ldx, int tokens, int k, int H, const int* slots, void* out, int64_t ldo,
+                     void* stream);
+int tdb_moe_combine(const void* y, int64_t ldy, int tokens, int k, int H, const int* slots, const float* weights,
+                    const void* residual, int64_t ldr, void* out, int64_t ldo, void* stream);
+int tdb_moe_combine_bwd(const void* dout, int64_t ldd, const void* y, int64_t ldy, int tokens, int k, int H,
+                        const int* slots, const float* weights, void* dy, int64_t lddy, float* dweights, void* stream);
+
 /* ---- optimizer (optim.cu) ----------------------------------------------- */
 int tdb_sumsq_partials_count(void);
 int tdb_sumsq(const float* g, int64_t n, double* partial, double* out, int accumulate, void* stream);

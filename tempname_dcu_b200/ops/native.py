@@ -102,6 +102,28 @@ def stream_ptr(stream=None) -> int:
     return int(stream.cuda_stream)
 
 
+class on_device:
+    """``with on_device(t.device):`` -- the calls inside launch on ``t``'s device
+    and its current stream.  Free of CUDA calls when that is the current device."""
+
+    def __init__(self, device):
+        self.device = device
+        self.guard = None
+
+    def __enter__(self):
+        import torch
+        if self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+            self.guard = None
+        return False
+
+
 def read_status() -> list[int]:
     """Synchronously read the device status word [code, where, d0, d1]."""
     buf = (ctypes.c_int * 4)()
