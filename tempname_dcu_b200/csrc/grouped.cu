@@ -1,0 +1,253 @@
+// Entry points of the products grouped by expert (grouped.cuh) and the
+// grouped bias gradient.
+#include "grouped.cuh"
+#include "tensor_map.h"
+
+namespace tdb {
+namespace grouped {
+
+template <int CG, int BN, int OP, int MODE>
+__global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Params p) {
+  mainloop<CG, BN, OP, MODE>(p);
+}
+
+// Most m tiles that `rows` rows in `groups` groups can need: each group adds
+// at most one partial tile.
+static int64_t most_tiles(int64_t rows, int64_t groups, int tile_m) {
+  return rows / tile_m + (rows < groups ? rows : groups);
+}
+
+template <int CG, int BN, int OP, int MODE>
+static int launch(const Params& p, cudaStream_t stream) {
+  using Cfg = Config<CG, BN>;
+  auto kern = kernel<CG, BN, OP, MODE>;
+  const int smem = Cfg::smem_bytes(p.groups);
+  static_assert(Cfg::smem_bytes(kMaxGroups) <= 227 * 1024, "shared memory budget");
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr_set[dev & 63]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(kMaxGroups));
+    if (e != cudaSuccess) return tdb_host::fail(int(e), "cudaFuncSetAttribute(grouped) failed");
+    attr_set[dev & 63] = true;
+  }
+  const int64_t nt = (p.N + BN - 1) / BN;
+  const int64_t tiles = OP == kWeightGrad ? int64_t(p.groups) * ((p.M + Cfg::kTileM - 1) / Cfg::kTileM) * nt
+                                          : most_tiles(p.rows, p.groups, Cfg::kTileM) * nt;
+  if (tiles >= (int64_t(1) << 31)) return tdb_host::fail(int(cudaErrorInvalidValue), "grouped: more than 2^31 output tiles");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  int64_t units = tdb_host::grid_sms() / CG;
+  if (CG == 2) {  // SM pairs that can be resident at once
+    static int pairs[64] = {0};
+    if (!pairs[dev & 63]) {
+      cfg.gridDim = dim3(unsigned(tdb_host::sm_count() / 2 * 2));
+      int n = 0;
+      cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+      if (e != cudaSuccess || n <= 0) return tdb_host::fail(int(e), "grouped: no active SM pairs possible");
+      pairs[dev & 63] = n;
+    }
+    if (units > pairs[dev & 63]) units = pairs[dev & 63];
+  }
+  if (units < 1) units = 1;
+  if (tiles < units) units = tiles;
+  cfg.gridDim = dim3(unsigned(units * CG));
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  tdb_host::launched(1);
+  if (e != cudaSuccess) return tdb_host::fail(int(e), "grouped: launch failed");
+  return 0;
+}
+
+template <int OP, int MODE>
+static int launch_tile(int tile, const Params& p, cudaStream_t s) {
+  return tile == 512 ? launch<2, 256, OP, MODE>(p, s) : launch<1, 128, OP, MODE>(p, s);
+}
+
+// Tile of a call: SM pairs (256 x 256) when the groups have rows enough to
+// fill their tiles on average, else 128 x 128.
+static int pick_tile(int op, int64_t rows, int groups, int M, int N) {
+  if (op == kWeightGrad) return M >= 256 && N >= 256 ? 512 : 128;
+  return rows >= int64_t(groups) * 192 && N >= 256 ? 512 : 128;
+}
+
+// Sums of dy's rows per group and column.  One block per group and 64
+// columns: 8 threads x 8 columns by 32 row lanes, joined in a fixed order.
+__global__ void __launch_bounds__(256) bias_grad_kernel(const uint16_t* __restrict__ dy, int64_t ld, int rows, int N,
+                                                        const int* __restrict__ offsets, float* __restrict__ out,
+                                                        int accumulate, int* status) {
+  __shared__ float sh[32][65];
+  const int g = blockIdx.y, cx = threadIdx.x & 7, lane_row = threadIdx.x >> 3;
+  const int col = blockIdx.x * 64 + cx * 8;
+  const int lo = offsets[g], hi = offsets[g + 1];
+  if (lo < 0 || hi < lo || hi > rows) {
+    if (threadIdx.x == 0) record_status(status, kBadArgument, 301, g, hi);
+    return;
+  }
+  float acc[8] = {};
+  if (col < N) {
+#pragma unroll 4
+    for (int r = lo + lane_row; r < hi; r += 32) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(dy + int64_t(r) * ld + col));
+      const uint32_t a[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[2 * j] += __uint_as_float(a[j] << 16);
+        acc[2 * j + 1] += __uint_as_float(a[j] & 0xffff0000u);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sh[lane_row][cx * 8 + j] = acc[j];
+  __syncthreads();
+  const int c = blockIdx.x * 64 + int(threadIdx.x);
+  if (threadIdx.x < 64 && c < N) {
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) s += sh[r][threadIdx.x];
+    float* o = out + int64_t(g) * N + c;
+    *o = accumulate ? *o + s : s;
+  }
+}
+
+static bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
+
+static int bad(const char* what) { return tdb_host::fail(int(cudaErrorInvalidValue), "%s", what); }
+
+}  // namespace grouped
+}  // namespace tdb
+
+using namespace tdb;
+using namespace tdb::grouped;
+
+// Tile code that a grouped call takes (op 0 forward, 1 data gradient, 2 weight
+// gradient): 512 = 256 x 256 on SM pairs, 128 = 128 x 128.
+TDB_API int tdb_grouped_pick_tile(int op, long long rows, int groups, int M, int N) {
+  return tdb::grouped::pick_tile(op, rows, groups, M, N);
+}
+
+// C[r, :] = epilogue(A[r, :] W_g) for the rows r of group g, g = 0..groups:
+//   data_grad 0: A [rows, K], W [groups, N, K], C [rows, N] = A W_g^T (+ bias)
+//   data_grad 1: A [rows, K], W [groups, K, N], C [rows, N] = A W_g
+// mode kStore, kBias, kBiasGelu (data_grad 0; aux_out gets the pre-activation)
+// or kGeluBwd (data_grad 1; aux holds it).  Rows outside every group keep
+// their contents.  tile 0 picks the tile.
+TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data_grad, const int* offsets, int groups,
+                             void* C, int64_t ldc, int rows, int N, int K, int mode, const void* bias, const void* aux,
+                             int64_t ld_aux, void* aux_out, int tile, void* stream) {
+  if (groups < 1 || groups > kMaxGroups || rows < 0 || N <= 0 || K <= 0 || N % 8 || K % 8)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "grouped: 1..%d groups, N and K multiples of 8", kMaxGroups);
+  if (rows == 0) return 0;
+  if (!A || !W || !C || !offsets || lda % 8 || lda < K || ldc % 8 || ldc < N || misaligned(A) || misaligned(W) ||
+      misaligned(C) || (bias && misaligned(bias)))
+    return bad("grouped: operands must be 16-byte aligned with 16-byte row strides");
+  const bool modes_ok = data_grad ? (mode == gemm::kStore || mode == gemm::kGeluBwd)
+                                  : (mode == gemm::kStore || mode == gemm::kBias || mode == gemm::kBiasGelu);
+  if (!modes_ok || (mode == gemm::kBias && !bias)) return bad("grouped: epilogue mode not available");
+  if ((mode == gemm::kBiasGelu && (!aux_out || misaligned(aux_out) || ld_aux % 8 || ld_aux < N)) ||
+      (mode == gemm::kGeluBwd && (!aux || misaligned(aux) || ld_aux % 8 || ld_aux < N)))
+    return bad("grouped: the pre-activation must be 16-byte aligned with 16-byte row strides");
+  if (tile == 0) tile = tdb::grouped::pick_tile(data_grad ? kDataGrad : kForward, rows, groups, 0, N);
+  if (tile != 128 && tile != 512) return bad("grouped: tile must be 0, 128 or 512");
+  Params p = {};
+  int rc = tdb_host::make_tmap_2d(&p.tmA, A, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(K), uint64_t(rows),
+                                  uint64_t(lda), gemm::BK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  if (data_grad)
+    rc = tdb_host::make_tmap_3d(&p.tmB, W, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(N), uint64_t(K),
+                                uint64_t(groups), uint64_t(N), uint64_t(N) * uint64_t(K), 64, gemm::BK,
+                                CU_TENSOR_MAP_SWIZZLE_128B);
+  else
+    rc = tdb_host::make_tmap_3d(&p.tmB, W, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(K), uint64_t(N),
+                                uint64_t(groups), uint64_t(K), uint64_t(N) * uint64_t(K), gemm::BK, 128,
+                                CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  rc = tdb_host::make_tmap_2d(&p.tmC, C, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(N), uint64_t(rows),
+                              uint64_t(ldc), 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  if (mode == gemm::kBiasGelu) {
+    rc = tdb_host::make_tmap_2d(&p.tmAux, aux_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(N), uint64_t(rows),
+                                uint64_t(ld_aux), 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  p.offsets = offsets;
+  p.groups = groups;
+  p.rows = rows;
+  p.N = N;
+  p.K = K;
+  p.band = tile == 512 ? 8 : 16;
+  p.C = static_cast<uint16_t*>(C);
+  p.ldc = ldc;
+  p.aux_out = static_cast<uint16_t*>(aux_out);
+  p.aux = static_cast<const uint16_t*>(aux);
+  p.ld_aux = ld_aux;
+  p.bias = static_cast<const uint16_t*>(bias);
+  p.status = tdb_host::status_ptr();
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (data_grad)
+    return mode == gemm::kGeluBwd ? launch_tile<kDataGrad, gemm::kGeluBwd>(tile, p, s)
+                                  : launch_tile<kDataGrad, gemm::kStore>(tile, p, s);
+  if (mode == gemm::kBiasGelu) return launch_tile<kForward, gemm::kBiasGelu>(tile, p, s);
+  if (mode == gemm::kBias) return launch_tile<kForward, gemm::kBias>(tile, p, s);
+  return launch_tile<kForward, gemm::kStore>(tile, p, s);
+}
+
+// C[g] (fp32 [groups, N, K]) (+)= dY_g^T X_g over the rows of group g:
+// dY [rows, N], X [rows, K].
+TDB_API int tdb_grouped_weight_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, const int* offsets,
+                                    int groups, float* C, int rows, int N, int K, int accumulate, int tile,
+                                    void* stream) {
+  if (groups < 1 || groups > kMaxGroups || rows < 0 || N <= 0 || K <= 0 || N % 8 || K % 8)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "grouped weight gradient: 1..%d groups, N and K multiples of 8",
+                          kMaxGroups);
+  if (!C || misaligned(C)) return bad("grouped weight gradient: the output must be 16-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {
+    if (accumulate) return 0;
+    return int(cudaMemsetAsync(C, 0, size_t(groups) * N * K * sizeof(float), s));
+  }
+  if (!dY || !X || !offsets || ldy % 8 || ldy < N || ldx % 8 || ldx < K || misaligned(dY) || misaligned(X))
+    return bad("grouped weight gradient: operands must be 16-byte aligned with 16-byte row strides");
+  if (tile == 0) tile = tdb::grouped::pick_tile(kWeightGrad, rows, groups, N, K);
+  if (tile != 128 && tile != 512) return bad("grouped weight gradient: tile must be 0, 128 or 512");
+  Params p = {};
+  int rc = tdb_host::make_tmap_2d(&p.tmA, dY, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(N), uint64_t(rows),
+                                  uint64_t(ldy), 64, gemm::BK, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  rc = tdb_host::make_tmap_2d(&p.tmB, X, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(K), uint64_t(rows),
+                              uint64_t(ldx), 64, gemm::BK, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  rc = tdb_host::make_tmap_3d(&p.tmC, C, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, uint64_t(K), uint64_t(N), uint64_t(groups),
+                              uint64_t(K), uint64_t(N) * uint64_t(K), 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  p.offsets = offsets;
+  p.groups = groups;
+  p.rows = rows;
+  p.M = N;
+  p.N = K;
+  p.band = 8;
+  p.accumulate = accumulate;
+  p.status = tdb_host::status_ptr();
+  return launch_tile<kWeightGrad, gemm::kAccF32>(tile, p, s);
+}
+
+// out[g] (fp32 [groups, N]) (+)= the sum of dY's rows of group g.
+TDB_API int tdb_grouped_bias_grad(const void* dY, int64_t ldy, const int* offsets, int groups, float* out, int rows,
+                                  int N, int accumulate, void* stream) {
+  if (groups < 1 || groups > kMaxGroups || rows < 0 || N <= 0 || N % 8)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "grouped bias gradient: 1..%d groups, N a multiple of 8", kMaxGroups);
+  if (!out || !offsets || (rows > 0 && (!dY || ldy % 8 || ldy < N || misaligned(dY))))
+    return bad("grouped bias gradient: rows must be 16-byte aligned");
+  bias_grad_kernel<<<dim3((N + 63) / 64, groups), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint16_t*>(dY), ldy, rows, N, offsets, out, accumulate, tdb_host::status_ptr());
+  tdb_host::launched(1);
+  return int(cudaGetLastError());
+}

@@ -110,6 +110,27 @@ int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, 
                 int(r), (unsigned long long)inner, (unsigned long long)outer, box_inner, box_outer);
   return 0;
 }
+
+int make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int elem_bytes, uint64_t inner,
+                 uint64_t outer, uint64_t depth, uint64_t row_stride_elems, uint64_t depth_stride_elems,
+                 uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(int(cudaErrorNotSupported), "cuTensorMapEncodeTiled unavailable");
+  if (reinterpret_cast<uintptr_t>(base) % 16)
+    return fail(int(cudaErrorInvalidValue), "TMA base address must be 16-byte aligned");
+  if ((row_stride_elems * elem_bytes) % 16 || (depth_stride_elems * elem_bytes) % 16)
+    return fail(int(cudaErrorInvalidValue), "TMA strides must be multiples of 16 bytes");
+  cuuint64_t dims[3] = {inner, outer, depth};
+  cuuint64_t strides[2] = {row_stride_elems * uint64_t(elem_bytes), depth_stride_elems * uint64_t(elem_bytes)};
+  cuuint32_t box[3] = {box_inner, box_outer, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, dtype, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(int(cudaErrorInvalidValue), "cuTensorMapEncodeTiled failed (%d): %llu x %llu x %llu, box %u, %u", int(r),
+                (unsigned long long)inner, (unsigned long long)outer, (unsigned long long)depth, box_inner, box_outer);
+  return 0;
+}
 }  // namespace tdb_host
 
 // ---------------------------------------------------------------------------

@@ -176,6 +176,16 @@ int tdb_moe_combine(const void* y, int64_t ldy, int tokens, int k, int H, const 
 int tdb_moe_combine_bwd(const void* dout, int64_t ldd, const void* y, int64_t ldy, int tokens, int k, int H,
                         const int* slots, const float* weights, void* dy, int64_t lddy, float* dweights, void* stream);
 
+/* ---- products grouped by expert (grouped.cu) ----------------------------- */
+int tdb_grouped_pick_tile(int op, long long rows, int groups, int M, int N);
+int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data_grad, const int* offsets, int groups, void* C,
+                     int64_t ldc, int rows, int N, int K, int mode, const void* bias, const void* aux, int64_t ld_aux,
+                     void* aux_out, int tile, void* stream);
+int tdb_grouped_weight_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, const int* offsets, int groups,
+                            float* C, int rows, int N, int K, int accumulate, int tile, void* stream);
+int tdb_grouped_bias_grad(const void* dY, int64_t ldy, const int* offsets, int groups, float* out, int rows, int N,
+                          int accumulate, void* stream);
+
 /* ---- optimizer (optim.cu) ----------------------------------------------- */
 int tdb_sumsq_partials_count(void);
 int tdb_sumsq(const float* g, int64_t n, double* partial, double* out, int accumulate, void* stream);

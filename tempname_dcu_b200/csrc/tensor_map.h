@@ -1,4 +1,4 @@
-// Host helper that builds 2-D TMA descriptors (cuTensorMapEncodeTiled).
+// Host helpers that build 2-D and 3-D TMA descriptors (cuTensorMapEncodeTiled).
 #pragma once
 #include <cuda.h>
 #include <stdint.h>
@@ -10,4 +10,9 @@ namespace tdb_host {
 int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int elem_bytes, uint64_t inner,
                  uint64_t outer, uint64_t row_stride_elems, uint32_t box_inner, uint32_t box_outer,
                  CUtensorMapSwizzle swizzle);
+// The same for `depth` such matrices, `depth_stride_elems` apart; the copied
+// tile is box_inner x box_outer x 1.
+int make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int elem_bytes, uint64_t inner,
+                 uint64_t outer, uint64_t depth, uint64_t row_stride_elems, uint64_t depth_stride_elems,
+                 uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle);
 }  // namespace tdb_host
