@@ -1,81 +1,40 @@
 // Entry points of the products grouped by expert (grouped.cuh) and the
 // grouped bias gradient.
 #include "grouped.cuh"
+#include "grouped_launch.cuh"
 #include "tensor_map.h"
 
 namespace tdb {
 namespace grouped {
 
-template <int CG, int BN, int OP, int MODE>
-__global__ void __launch_bounds__(kThreads, 1) kernel(const __grid_constant__ Params p) {
-  mainloop<CG, BN, OP, MODE>(p);
+template <int CG, int BN>
+__global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_constant__ Params p) {
+  mainloop<CG, BN>(p);
 }
 
-// Most m tiles that `rows` rows in `groups` groups can need: each group adds
-// at most one partial tile.
-static int64_t most_tiles(int64_t rows, int64_t groups, int tile_m) {
-  return rows / tile_m + (rows < groups ? rows : groups);
-}
-
-template <int CG, int BN, int OP, int MODE>
-static int launch(const Params& p, cudaStream_t stream) {
+template <int CG, int BN>
+static int launch_weight_grad(const Params& p, cudaStream_t stream) {
   using Cfg = Config<CG, BN>;
-  auto kern = kernel<CG, BN, OP, MODE>;
-  const int smem = Cfg::smem_bytes(p.groups);
   static_assert(Cfg::smem_bytes(kMaxGroups) <= 227 * 1024, "shared memory budget");
-  static bool attr_set[64] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (!attr_set[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(kMaxGroups));
-    if (e != cudaSuccess) return tdb_host::fail(int(e), "cudaFuncSetAttribute(grouped) failed");
-    attr_set[dev & 63] = true;
-  }
-  const int64_t nt = (p.N + BN - 1) / BN;
-  const int64_t tiles = OP == kWeightGrad ? int64_t(p.groups) * ((p.M + Cfg::kTileM - 1) / Cfg::kTileM) * nt
-                                          : most_tiles(p.rows, p.groups, Cfg::kTileM) * nt;
-  if (tiles >= (int64_t(1) << 31)) return tdb_host::fail(int(cudaErrorInvalidValue), "grouped: more than 2^31 output tiles");
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = size_t(smem);
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
-  int64_t units = tdb_host::grid_sms() / CG;
-  if (CG == 2) {  // SM pairs that can be resident at once
-    static int pairs[64] = {0};
-    if (!pairs[dev & 63]) {
-      cfg.gridDim = dim3(unsigned(tdb_host::sm_count() / 2 * 2));
-      int n = 0;
-      cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
-      if (e != cudaSuccess || n <= 0) return tdb_host::fail(int(e), "grouped: no active SM pairs possible");
-      pairs[dev & 63] = n;
-    }
-    if (units > pairs[dev & 63]) units = pairs[dev & 63];
-  }
-  if (units < 1) units = 1;
-  if (tiles < units) units = tiles;
-  cfg.gridDim = dim3(unsigned(units * CG));
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-  tdb_host::launched(1);
-  if (e != cudaSuccess) return tdb_host::fail(int(e), "grouped: launch failed");
-  return 0;
+  const int64_t tiles = int64_t(p.groups) * ((p.M + Cfg::kTileM - 1) / Cfg::kTileM) * ((p.N + BN - 1) / BN);
+  static LaunchState state[64];
+  return launch_units<CG>(weight_grad_kernel<CG, BN>, p, tiles, Cfg::smem_bytes(p.groups), Cfg::smem_bytes(kMaxGroups),
+                          state, stream);
 }
 
 template <int OP, int MODE>
-static int launch_tile(int tile, const Params& p, cudaStream_t s) {
-  return tile == 512 ? launch<2, 256, OP, MODE>(p, s) : launch<1, 128, OP, MODE>(p, s);
+static int launch_rows_tile(int tile, const RowsParams& p, cudaStream_t s) {
+  if (tile == 512) return launch_rows<2, 256, OP, MODE, false>(p, s);
+  if (tile == 128) return launch_rows<1, 128, OP, MODE, false>(p, s);
+  return launch_rows<1, 32, OP, MODE, false>(p, s);
 }
 
-// Tile of a call: SM pairs (256 x 256) when the groups have rows enough to
-// fill their tiles on average, else 128 x 128.
+// Tile of a call.  Forward and data gradient: up to 256 rows x 256 columns on
+// SM pairs (512), 128 x 128 (128) or 32 x 128 (32), the smallest whose rows
+// hold an average group.
 static int pick_tile(int op, int64_t rows, int groups, int M, int N) {
   if (op == kWeightGrad) return M >= 256 && N >= 256 ? 512 : 128;
+  if (rows <= int64_t(groups) * 32) return 32;
   return rows >= int64_t(groups) * 192 && N >= 256 ? 512 : 128;
 }
 
@@ -129,7 +88,7 @@ using namespace tdb;
 using namespace tdb::grouped;
 
 // Tile code that a grouped call takes (op 0 forward, 1 data gradient, 2 weight
-// gradient): 512 = 256 x 256 on SM pairs, 128 = 128 x 128.
+// gradient); see pick_tile.
 TDB_API int tdb_grouped_pick_tile(int op, long long rows, int groups, int M, int N) {
   return tdb::grouped::pick_tile(op, rows, groups, M, N);
 }
@@ -156,26 +115,25 @@ TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data
       (mode == gemm::kGeluBwd && (!aux || misaligned(aux) || ld_aux % 8 || ld_aux < N)))
     return bad("grouped: the pre-activation must be 16-byte aligned with 16-byte row strides");
   if (tile == 0) tile = tdb::grouped::pick_tile(data_grad ? kDataGrad : kForward, rows, groups, 0, N);
-  if (tile != 128 && tile != 512) return bad("grouped: tile must be 0, 128 or 512");
-  Params p = {};
-  int rc = tdb_host::make_tmap_2d(&p.tmA, A, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(K), uint64_t(rows),
-                                  uint64_t(lda), gemm::BK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (tile != 32 && tile != 128 && tile != 512) return bad("grouped: tile must be 0, 32, 128 or 512");
+  RowsParams p = {};
+  const uint32_t box_rows = tile == 32 ? 32 : 64;
+  int rc = tdb_host::make_tmap_2d(&p.tmB, A, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(K), uint64_t(rows),
+                                  uint64_t(lda), gemm::BK, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   if (data_grad)
-    rc = tdb_host::make_tmap_3d(&p.tmB, W, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(N), uint64_t(K),
+    rc = tdb_host::make_tmap_3d(&p.tmA, W, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(N), uint64_t(K),
                                 uint64_t(groups), uint64_t(N), uint64_t(N) * uint64_t(K), 64, gemm::BK,
                                 CU_TENSOR_MAP_SWIZZLE_128B);
   else
-    rc = tdb_host::make_tmap_3d(&p.tmB, W, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(K), uint64_t(N),
+    rc = tdb_host::make_tmap_3d(&p.tmA, W, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(K), uint64_t(N),
                                 uint64_t(groups), uint64_t(K), uint64_t(N) * uint64_t(K), gemm::BK, 128,
                                 CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  rc = tdb_host::make_tmap_2d(&p.tmC, C, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(N), uint64_t(rows),
-                              uint64_t(ldc), 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+  rc = make_output_map(&p.tmC, C, rows, N, ldc);
   if (rc) return rc;
   if (mode == gemm::kBiasGelu) {
-    rc = tdb_host::make_tmap_2d(&p.tmAux, aux_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(N), uint64_t(rows),
-                                uint64_t(ld_aux), 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = make_output_map(&p.tmAux, aux_out, rows, N, ld_aux);
     if (rc) return rc;
   }
   p.offsets = offsets;
@@ -183,7 +141,7 @@ TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data
   p.rows = rows;
   p.N = N;
   p.K = K;
-  p.band = tile == 512 ? 8 : 16;
+  p.band = kBand;
   p.C = static_cast<uint16_t*>(C);
   p.ldc = ldc;
   p.aux_out = static_cast<uint16_t*>(aux_out);
@@ -193,11 +151,11 @@ TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data
   p.status = tdb_host::status_ptr();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (data_grad)
-    return mode == gemm::kGeluBwd ? launch_tile<kDataGrad, gemm::kGeluBwd>(tile, p, s)
-                                  : launch_tile<kDataGrad, gemm::kStore>(tile, p, s);
-  if (mode == gemm::kBiasGelu) return launch_tile<kForward, gemm::kBiasGelu>(tile, p, s);
-  if (mode == gemm::kBias) return launch_tile<kForward, gemm::kBias>(tile, p, s);
-  return launch_tile<kForward, gemm::kStore>(tile, p, s);
+    return mode == gemm::kGeluBwd ? launch_rows_tile<kDataGrad, gemm::kGeluBwd>(tile, p, s)
+                                  : launch_rows_tile<kDataGrad, gemm::kStore>(tile, p, s);
+  if (mode == gemm::kBiasGelu) return launch_rows_tile<kForward, gemm::kBiasGelu>(tile, p, s);
+  if (mode == gemm::kBias) return launch_rows_tile<kForward, gemm::kBias>(tile, p, s);
+  return launch_rows_tile<kForward, gemm::kStore>(tile, p, s);
 }
 
 // C[g] (fp32 [groups, N, K]) (+)= dY_g^T X_g over the rows of group g:
@@ -236,7 +194,7 @@ TDB_API int tdb_grouped_weight_grad(const void* dY, int64_t ldy, const void* X, 
   p.band = 8;
   p.accumulate = accumulate;
   p.status = tdb_host::status_ptr();
-  return launch_tile<kWeightGrad, gemm::kAccF32>(tile, p, s);
+  return tile == 512 ? launch_weight_grad<2, 256>(p, s) : launch_weight_grad<1, 128>(p, s);
 }
 
 // out[g] (fp32 [groups, N]) (+)= the sum of dY's rows of group g.

@@ -1,0 +1,83 @@
+// Host side of the persistent grouped kernels: grid size and launch.
+#pragma once
+#include "grouped_rows.cuh"
+#include "tensor_map.h"
+
+namespace tdb {
+namespace grouped {
+
+constexpr int kBand = 8;  // token tiles per raster band
+
+struct LaunchState {
+  bool ready = false;
+  int pairs = 0;  // SM pairs that can be resident at once (CG = 2)
+};
+
+// Launches `kern` on as many CTAs (CG = 1) or SM pairs (CG = 2) as there are
+// tiles, at most one per SM of the caller's share.
+template <int CG, class P>
+static int launch_units(void (*kern)(P), const P& p, int64_t tiles, int smem, int max_smem, LaunchState* states,
+                        cudaStream_t stream) {
+  if (tiles >= (int64_t(1) << 31)) return tdb_host::fail(int(cudaErrorInvalidValue), "grouped: more than 2^31 output tiles");
+  int dev = 0;
+  cudaGetDevice(&dev);
+  LaunchState& state = states[dev & 63];
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  if (!state.ready) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, max_smem);
+    if (e != cudaSuccess) return tdb_host::fail(int(e), "cudaFuncSetAttribute(grouped) failed");
+    if (CG == 2) {
+      cfg.gridDim = dim3(unsigned(tdb_host::sm_count() / 2 * 2));
+      int n = 0;
+      e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+      if (e != cudaSuccess || n <= 0) return tdb_host::fail(int(e), "grouped: no active SM pairs possible");
+      state.pairs = n;
+    }
+    state.ready = true;
+  }
+  int64_t units = tdb_host::grid_sms() / CG;
+  if (CG == 2 && units > state.pairs) units = state.pairs;
+  if (units < 1) units = 1;
+  if (tiles < units) units = tiles;
+  cfg.gridDim = dim3(unsigned(units * CG));
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  tdb_host::launched(1);
+  if (e != cudaSuccess) return tdb_host::fail(int(e), "grouped: launch failed");
+  return 0;
+}
+
+template <int CG, int BT, int OP, int MODE, bool MX4>
+__global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant__ RowsParams p) {
+  rows_mainloop<CG, BT, OP, MODE, MX4>(p);
+}
+
+template <int CG, int BT, int OP, int MODE, bool MX4>
+static int launch_rows(const RowsParams& p, cudaStream_t stream) {
+  using Cfg = RowsConfig<CG, BT, MX4>;
+  static_assert(Cfg::smem_bytes(kMaxGroups) <= 227 * 1024, "shared memory budget");
+  // most tiles that the rows can need: each group adds at most one partial tile
+  const int64_t row_tiles = p.rows / BT + (p.rows < p.groups ? p.rows : p.groups);
+  const int64_t tiles = row_tiles * ((p.N + Cfg::kTileN - 1) / Cfg::kTileN);
+  static LaunchState state[64];
+  return launch_units<CG>(rows_kernel<CG, BT, OP, MODE, MX4>, p, tiles, Cfg::smem_bytes(p.groups),
+                          Cfg::smem_bytes(kMaxGroups), state, stream);
+}
+
+// bf16 output rows in blocks of 32 rows x 32 columns.
+static int make_output_map(CUtensorMap* map, const void* C, int rows, int N, int64_t ldc) {
+  return tdb_host::make_tmap_2d(map, C, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(N), uint64_t(rows), uint64_t(ldc),
+                                32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+}  // namespace grouped
+}  // namespace tdb

@@ -1,0 +1,344 @@
+// Microscaled 4-bit floating point ("MXFP4"): quantiser, its inverse and the
+// product of two quantised operands on tcgen05 kind::mxf4.
+//
+// Values are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two per
+// byte with the even K index in the low half; each 32 consecutive K values of a
+// row share a ue8m0 scale 2^(byte - 127).  For a block of absolute maximum a
+// the exponent is the smallest e with a * 2^-e <= 6, so nothing saturates, and
+// the scaled values round to nearest even.  A block that holds an infinity or
+// NaN gets byte 255, which decodes as NaN; an all-zero block byte 0.
+//
+// Scales are stored in 512-byte atoms of 128 rows x 128 K values, byte
+// (r % 32) * 16 + (r % 128) / 32 * 4 + j of row r and 32-value block j -- the
+// order in which tcgen05.cp 32x128b.warpx4 brings them to TMEM.  Atoms of one
+// 128-row block are consecutive along K, rounded up to an even number (a K
+// step of the product is 256 values); blocks past K hold byte 0.  With
+// offsets the rows of each group start a new 128-row block, so that a tile of
+// the grouped product starts at a block wherever its group starts.
+#include "grouped_launch.cuh"
+
+namespace tdb {
+namespace mx4 {
+
+using grouped::kMaxGroups;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBatch = 4;  // 256-value pieces in flight per warp
+
+// Block exponent from the bits of the largest |bf16|: the smallest e with
+// a <= 6 * 2^e = 1.5 * 2^(e + 2), at least -127 (also for 0 and subnormals).
+__host__ __device__ __forceinline__ int block_exponent(uint32_t abs_bits) {
+  const int field = int(abs_bits >> 7);
+  if (field == 0) return -127;
+  const int e = field - 127 - 2 + ((abs_bits & 0x7f) > 0x40 ? 1 : 0);
+  return e < -127 ? -127 : e;  // at most 126
+}
+
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// Magnitude code m (3 bits) as a float: m * 0.5 below 2, else (1 + m % 2 / 2) * 2^(m / 2 - 1).
+__device__ __forceinline__ float e2m1_value(uint32_t code) {
+  const uint32_t m = code & 7u;
+  const float a = m < 2u ? 0.5f * float(m) : __uint_as_float(((126u + (m >> 1)) << 23) | ((m & 1u) << 22));
+  return __uint_as_float(__float_as_uint(a) | ((code & 8u) << 28));
+}
+
+struct Layout {
+  const int* off;    // shared: group offsets, or null
+  const int* block;  // shared: first 128-row block of each group
+  int groups;
+  int rows, mat_blocks;  // without offsets: rows and blocks of one matrix
+  // Scale block and row in it of row `r`; false for a row outside every group.
+  __device__ __forceinline__ bool find(int64_t r, int64_t& blk, int& in) const {
+    if (!off) {
+      const int64_t m = r / rows;
+      const int local = int(r - m * rows);
+      blk = m * mat_blocks + local / 128;
+      in = local % 128;
+      return true;
+    }
+    if (r < off[0] || r >= off[groups]) return false;
+    int lo = 0, hi = groups - 1;  // the last group that starts at or before r holds it
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (off[mid] <= int(r)) lo = mid; else hi = mid - 1;
+    }
+    const int local = int(r) - off[lo];
+    blk = block[lo] + local / 128;
+    in = local % 128;
+    return true;
+  }
+};
+
+// Builds the layout's tables; returns false (status recorded) for bad offsets.
+__device__ __forceinline__ bool make_layout(Layout& l, const int* offsets, int groups, int rows, int mat_blocks, int* sh,
+                                            int* status) {
+  l.off = nullptr;
+  l.block = nullptr;
+  l.groups = groups;
+  l.rows = rows;
+  l.mat_blocks = mat_blocks;
+  if (!offsets) return true;
+  int* off = sh;
+  int* first = off + groups + 1;
+  int* block = first + groups + 1;
+  __shared__ int bad_offsets;
+  if (threadIdx.x < 32) {
+    const bool bad = grouped::load_offsets(offsets, groups, rows, off, status);
+    __syncwarp();
+    if (!bad) grouped::scan_tiles<128, true>(off, groups, first, block);
+    if (threadIdx.x == 0) bad_offsets = bad;
+  }
+  __syncthreads();
+  l.off = off;
+  l.block = block;
+  return !bad_offsets;
+}
+
+// A warp takes 256 consecutive values of a row (two scale words), a lane 8.
+__global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t total_rows,
+                                                            int K, uint8_t* __restrict__ q, uint8_t* __restrict__ sf,
+                                                            const int* offsets, int groups, int rows, int mat_blocks,
+                                                            int* status) {
+  extern __shared__ int sh[];
+  Layout l;
+  if (!make_layout(l, offsets, groups, rows, mat_blocks, sh, status)) return;
+  const int lane = threadIdx.x & 31;
+  const int pieces = (K + 255) / 256;
+  const int64_t total = total_rows * pieces;
+  const int64_t step = int64_t(gridDim.x) * kWarps;
+  for (int64_t i0 = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); i0 < total; i0 += step * kBatch) {
+    uint4 in[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int64_t i = i0 + b * step;
+      in[b] = make_uint4(0, 0, 0, 0);
+      if (i < total) {
+        const int64_t r = i / pieces;
+        const int k = int(i - r * pieces) * 256 + lane * 8;
+        if (k < K) in[b] = __ldg(reinterpret_cast<const uint4*>(x + r * ldx + k));
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int64_t i = i0 + b * step;
+      if (i >= total) break;
+      const int64_t r = i / pieces;
+      const int piece = int(i - r * pieces);
+      const int k = piece * 256 + lane * 8;
+      const uint32_t w[4] = {in[b].x, in[b].y, in[b].z, in[b].w};
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool finite = top < 0x7f80u;
+      const int e = finite ? block_exponent(top) : 128;
+      uint32_t byte = uint32_t(e + 127);
+      const float inv = finite ? __uint_as_float(uint32_t(127 - e) << 23) : 0.f;  // 2^-e, normal for e in [-127, 126]
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = finite ? __uint_as_float(w[j] << 16) * inv : 0.f;
+        v[2 * j + 1] = finite ? __uint_as_float(w[j] & 0xffff0000u) * inv : 0.f;
+      }
+      int64_t blk;
+      int row;
+      if (!l.find(r, blk, row)) continue;
+      if (k < K) *reinterpret_cast<uint32_t*>(q + r * (K / 2) + k / 2) = e2m1x8(v);
+      // four blocks' bytes -> one word of the atom
+      byte |= __shfl_down_sync(0xffffffffu, byte, 4) << 8;
+      byte |= __shfl_down_sync(0xffffffffu, byte, 8) << 16;
+      if ((lane & 15) == 0)
+        *reinterpret_cast<uint32_t*>(sf + ((blk * pieces + piece) * 2 + (lane >> 4)) * 512 + (row & 31) * 16 +
+                                     (row >> 5) * 4) = byte;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf,
+                                                              int64_t total_rows, int K, uint16_t* __restrict__ out,
+                                                              int64_t ldo, const int* offsets, int groups, int rows,
+                                                              int mat_blocks, int* status) {
+  extern __shared__ int sh[];
+  Layout l;
+  if (!make_layout(l, offsets, groups, rows, mat_blocks, sh, status)) return;
+  const int lane = threadIdx.x & 31;
+  const int pieces = (K + 255) / 256;
+  const int64_t total = total_rows * pieces;
+  const int64_t step = int64_t(gridDim.x) * kWarps;
+  for (int64_t i0 = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); i0 < total; i0 += step * kBatch) {
+    uint32_t in[kBatch], byte[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int64_t i = i0 + b * step;
+      in[b] = 0;
+      byte[b] = 0;
+      if (i < total) {
+        const int64_t r = i / pieces;
+        const int piece = int(i - r * pieces);
+        const int k = piece * 256 + lane * 8;
+        int64_t blk;
+        int row;
+        if (k < K && l.find(r, blk, row)) {
+          in[b] = __ldg(reinterpret_cast<const uint32_t*>(q + r * (K / 2) + k / 2));
+          byte[b] = __ldg(sf + ((blk * pieces + piece) * 2 + (lane >> 4)) * 512 + (row & 31) * 16 + (row >> 5) * 4 +
+                          ((lane >> 2) & 3));
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int64_t i = i0 + b * step;
+      if (i >= total) break;
+      const int64_t r = i / pieces;
+      const int k = int(i - r * pieces) * 256 + lane * 8;
+      if (k >= K || (l.off && (r < l.off[0] || r >= l.off[groups]))) continue;
+      const float scale = __uint_as_float(byte[b] == 255u ? 0x7fffffffu : byte[b] == 0u ? 0x00400000u : byte[b] << 23);
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o[j] = pack_bf16x2(e2m1_value(in[b] >> (8 * j)) * scale, e2m1_value(in[b] >> (8 * j + 4)) * scale);
+      *reinterpret_cast<uint4*>(out + r * ldo + k) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+}
+
+static int64_t pairs_of(int64_t K) { return (K + 255) / 256; }
+
+// 128-row scale blocks of an operand: matrices x ceil(rows / 128), or with
+// groups the most that any offsets can need.
+static int64_t blocks_of(int64_t matrices, int64_t rows, int64_t groups) {
+  if (groups > 0) return rows / 128 + (rows < groups ? rows : groups);
+  return matrices * ((rows + 127) / 128);
+}
+
+static unsigned grid_for(int64_t rows, int64_t K) {
+  const int64_t blocks = (rows * pairs_of(K) + kWarps * kBatch - 1) / (kWarps * kBatch);
+  const int64_t most = int64_t(tdb_host::sm_count()) * 8;
+  return unsigned(blocks < most ? (blocks > 0 ? blocks : 1) : most);
+}
+
+static int check(const char* what, int64_t matrices, int64_t rows, int64_t K, int groups, const void* offsets) {
+  if (matrices < 1 || rows < 0 || K < 32 || K % 32 || K >= (int64_t(1) << 31) || rows >= (int64_t(1) << 31) ||
+      (offsets && (groups < 1 || groups > kMaxGroups || matrices != 1)))
+    return tdb_host::fail(int(cudaErrorInvalidValue), "%s: K must be a multiple of 32; 1..%d groups of one matrix's rows",
+                          what, kMaxGroups);
+  return 0;
+}
+
+}  // namespace mx4
+}  // namespace tdb
+
+using namespace tdb;
+
+// Bytes of the scales of `matrices` [rows, K] operands, or (groups > 0) of one
+// whose rows lie in that many groups.
+TDB_API long long tdb_mx4_scale_bytes(long long matrices, long long rows, long long K, int groups) {
+  return mx4::blocks_of(matrices, rows, groups) * mx4::pairs_of(K) * 1024;
+}
+
+// x bf16 [matrices * rows, K] (row stride ldx) -> q [matrices * rows, K / 2]
+// (dense) and scales.
+TDB_API int tdb_mx4_quantize(const void* x, int64_t ldx, int64_t matrices, int64_t rows, int64_t K, const int* offsets,
+                             int groups, void* q, void* sf, void* stream) {
+  if (int rc = mx4::check("mx4 quantize", matrices, rows, K, groups, offsets)) return rc;
+  if (rows == 0) return 0;
+  if (!x || !q || !sf || ldx % 8 || ldx < K || reinterpret_cast<uintptr_t>(x) % 16 ||
+      (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(sf)) % 16)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 quantize: rows must be 16-byte aligned");
+  mx4::quantize_kernel<<<mx4::grid_for(matrices * rows, K), mx4::kThreads,
+                         offsets ? size_t(3 * (groups + 1)) * 4 : 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint16_t*>(x), ldx, matrices * rows, int(K), static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf),
+      offsets, groups, int(rows), int((rows + 127) / 128), tdb_host::status_ptr());
+  tdb_host::launched(1);
+  return int(cudaGetLastError());
+}
+
+// The bf16 values of a quantised operand (exact: three significant bits and a
+// power of two), [matrices * rows, K] with row stride ldo.
+TDB_API int tdb_mx4_dequantize(const void* q, const void* sf, int64_t matrices, int64_t rows, int64_t K,
+                               const int* offsets, int groups, void* out, int64_t ldo, void* stream) {
+  if (int rc = mx4::check("mx4 dequantize", matrices, rows, K, groups, offsets)) return rc;
+  if (rows == 0) return 0;
+  if (!out || !q || !sf || ldo % 8 || ldo < K || reinterpret_cast<uintptr_t>(out) % 16 ||
+      (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(sf)) % 16)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 dequantize: rows must be 16-byte aligned");
+  mx4::dequantize_kernel<<<mx4::grid_for(matrices * rows, K), mx4::kThreads,
+                           offsets ? size_t(3 * (groups + 1)) * 4 : 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(sf), matrices * rows, int(K), static_cast<uint16_t*>(out),
+      ldo, offsets, groups, int(rows), int((rows + 127) / 128), tdb_host::status_ptr());
+  tdb_host::launched(1);
+  return int(cudaGetLastError());
+}
+
+// Tile code that a 4-bit product takes: 512 = up to 256 rows x 256 columns on
+// SM pairs, 128 = 128 x 128.
+TDB_API int tdb_mx4_pick_tile(long long rows, int groups, int N) {
+  return rows >= int64_t(groups) * 192 && N >= 256 ? 512 : 128;
+}
+
+// C[r, :] = x[r] w_g^T (+ bias[g]) for the rows r of group g, x and w as
+// tdb_mx4_quantize wrote them (x [rows, K] with the same offsets, w [groups, N,
+// K] as `groups` matrices).  offsets null: one group of all rows (groups = 1).
+TDB_API int tdb_mx4_gemm(const void* qx, const void* sfx, const void* qw, const void* sfw, const int* offsets, int groups,
+                         void* C, int64_t ldc, int rows, int N, int K, const void* bias, int tile, void* stream) {
+  using namespace tdb::grouped;
+  if (groups < 1 || groups > kMaxGroups || (!offsets && groups != 1) || rows < 0 || N <= 0 || N % 8 || K < 32 || K % 32)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 product: 1..%d groups, N a multiple of 8, K of 32", kMaxGroups);
+  if (rows == 0) return 0;
+  if (!qx || !sfx || !qw || !sfw || !C || ldc % 8 || ldc < N ||
+      (reinterpret_cast<uintptr_t>(qx) | reinterpret_cast<uintptr_t>(sfx) | reinterpret_cast<uintptr_t>(qw) |
+       reinterpret_cast<uintptr_t>(sfw) | reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(bias)) % 16)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 product: operands must be 16-byte aligned, output rows too");
+  if (tile == 0) tile = tdb_mx4_pick_tile(rows, groups, N);
+  if (tile != 128 && tile != 512)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 product: tile must be 0, 128 or 512");
+  const int64_t pairs = mx4::pairs_of(K);
+  const int64_t x_blocks = offsets ? mx4::blocks_of(1, rows, groups) : mx4::blocks_of(1, rows, 0);
+  const int64_t w_blocks = (N + 127) / 128;
+  if (x_blocks * pairs >= (int64_t(1) << 31) || int64_t(groups) * w_blocks * pairs >= (int64_t(1) << 31))
+    return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 product: too many scale blocks");
+  RowsParams p = {};
+  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
+  int rc = tdb_host::make_tmap_3d(&p.tmA, qw, u8, 1, uint64_t(K / 2), uint64_t(N), uint64_t(groups), uint64_t(K / 2),
+                                  uint64_t(K / 2) * uint64_t(N), 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  rc = tdb_host::make_tmap_2d(&p.tmB, qx, u8, 1, uint64_t(K / 2), uint64_t(rows), uint64_t(K / 2), 128, 64,
+                              CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  rc = tdb_host::make_tmap_2d(&p.tmSfa, sfw, u32, 4, 256, uint64_t(int64_t(groups) * w_blocks * pairs), 256, 256, 1,
+                              CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (rc) return rc;
+  rc = tdb_host::make_tmap_2d(&p.tmSfb, sfx, u32, 4, 256, uint64_t(x_blocks * pairs), 256, 256, 1,
+                              CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (rc) return rc;
+  rc = make_output_map(&p.tmC, C, rows, N, ldc);
+  if (rc) return rc;
+  p.offsets = offsets;
+  p.groups = groups;
+  p.rows = rows;
+  p.N = N;
+  p.K = K;
+  p.band = kBand;
+  p.a_blocks = int(w_blocks);
+  p.kpairs = int(pairs);
+  p.C = static_cast<uint16_t*>(C);
+  p.ldc = ldc;
+  p.bias = static_cast<const uint16_t*>(bias);
+  p.status = tdb_host::status_ptr();
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return tile == 512 ? launch_rows<2, 256, kForward, gemm::kBias, true>(p, s)
+                     : launch_rows<1, 128, kForward, gemm::kBias, true>(p, s);
+}

@@ -186,6 +186,16 @@ int tdb_grouped_weight_grad(const void* dY, int64_t ldy, const void* X, int64_t 
 int tdb_grouped_bias_grad(const void* dY, int64_t ldy, const int* offsets, int groups, float* out, int rows, int N,
                           int accumulate, void* stream);
 
+/* ---- microscaled 4-bit values and products (mx4.cu) ---------------------- */
+long long tdb_mx4_scale_bytes(long long matrices, long long rows, long long K, int groups);
+int tdb_mx4_quantize(const void* x, int64_t ldx, int64_t matrices, int64_t rows, int64_t K, const int* offsets,
+                     int groups, void* q, void* sf, void* stream);
+int tdb_mx4_dequantize(const void* q, const void* sf, int64_t matrices, int64_t rows, int64_t K, const int* offsets,
+                       int groups, void* out, int64_t ldo, void* stream);
+int tdb_mx4_pick_tile(long long rows, int groups, int N);
+int tdb_mx4_gemm(const void* qx, const void* sfx, const void* qw, const void* sfw, const int* offsets, int groups,
+                 void* C, int64_t ldc, int rows, int N, int K, const void* bias, int tile, void* stream);
+
 /* ---- optimizer (optim.cu) ----------------------------------------------- */
 int tdb_sumsq_partials_count(void);
 int tdb_sumsq(const float* g, int64_t n, double* partial, double* out, int accumulate, void* stream);

@@ -1,0 +1,168 @@
+"""Microscaled 4-bit floating point ("MXFP4"): quantizer, its inverse and
+products of two quantized operands (``csrc/mx4.cu``).
+
+Format: e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6, signed), one power-of-two
+scale (ue8m0 byte ``e + 127``) per 32 consecutive K values of a row.  The
+scale of a block with absolute maximum ``a`` is the smallest ``2^e`` (e >= -127)
+with ``a / 2^e <= 6``, so nothing saturates; values round to nearest even.  A
+block with an infinity or NaN decodes as NaN.  Two values share a byte (even K
+index low); scales are stored in 512-byte atoms as the tensor cores read them
+and are opaque to callers (``dequantize`` is the way back).
+
+Rows may be any number, K a multiple of 32, N of the products a multiple of 8.
+``offsets`` (int32 [groups + 1], on the device) are those of ``ops.grouped``:
+an operand quantized with offsets goes into ``grouped_linear`` with the same
+offsets.  Weights are quantized once, [N, K] or [groups, N, K].
+
+Against ``ops.mx`` (8-bit values): half the bytes and twice the tensor-core
+rate, at 2 significant bits per value.
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import native
+
+V, I, I64, LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_longlong
+
+native.register("tdb_mx4_scale_bytes", [LL, LL, LL, I], restype=LL)
+native.register("tdb_mx4_quantize", [V, I64, I64, I64, I64, V, I, V, V, V])
+native.register("tdb_mx4_dequantize", [V, V, I64, I64, I64, V, I, V, I64, V])
+native.register("tdb_mx4_pick_tile", [LL, I, I])
+native.register("tdb_mx4_gemm", [V, V, V, V, V, I, V, I64, I, I, I, V, I, V])
+
+E2M1_MAX = 6.0
+MAX_GROUPS = 1024
+
+
+def _need(cond, msg):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _groups(offsets, device):
+    import torch
+    if offsets is None:
+        return 0
+    _need(offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and
+          offsets.device == device, "offsets must be a contiguous int32 vector on the operands' device")
+    groups = offsets.numel() - 1
+    _need(1 <= groups <= MAX_GROUPS, f"the number of groups must be 1..{MAX_GROUPS}")
+    return groups
+
+
+def scale_bytes(rows: int, k: int, groups: int = 0, matrices: int = 1) -> int:
+    """Bytes of the scales of ``matrices`` [rows, k] operands, or of one whose
+    rows lie in ``groups`` groups."""
+    return int(native.lib().tdb_mx4_scale_bytes(matrices, rows, k, groups))
+
+
+def _operand(q, sf, groups, device, what):
+    """(matrices, rows, K) of a quantized operand."""
+    import torch
+    _need(q.dtype == torch.uint8 and q.dim() in (2, 3) and q.is_contiguous() and q.device == device and
+          q.shape[-1] % 16 == 0 and q.shape[-1] > 0,
+          f"{what} must be contiguous uint8 [..., K/2] as written by quantize, on the operands' device")
+    matrices = q.shape[0] if q.dim() == 3 else 1
+    rows, K = q.shape[-2], 2 * q.shape[-1]
+    _need(sf.dtype == torch.uint8 and sf.is_contiguous() and sf.device == device and
+          sf.numel() >= scale_bytes(rows, K, groups, matrices),
+          f"the scales of {what} must be the uint8 buffer that quantize wrote for these rows (and offsets)")
+    return matrices, rows, K
+
+
+def quantize(x, offsets=None, q=None, sf=None):
+    """bf16 ``x`` [rows, K] or [matrices, rows, K] -> (q uint8 [..., K/2], sf
+    uint8).  With ``offsets``, rows outside every group are not written."""
+    import torch
+    if x.dtype != torch.bfloat16:
+        raise TypeError("quantize expects bf16")
+    _need(x.is_cuda and x.dim() in (2, 3) and x.stride(-1) == 1, "x must be [rows, K] or [matrices, rows, K] on a CUDA "
+          "device with a contiguous last dimension")
+    rows, K = x.shape[-2:]
+    _need(K > 0 and K % 32 == 0, "K must be a positive multiple of 32")
+    dev = x.device
+    groups = _groups(offsets, dev)
+    matrices, ld = 1, x.stride(-2) if rows > 1 else K
+    if x.dim() == 3:
+        _need(x.is_contiguous() and offsets is None and x.shape[0] > 0,
+              "a [matrices, rows, K] operand must be contiguous and takes no offsets")
+        matrices, ld = x.shape[0], K
+    _need(ld >= K, "x: rows must not overlap")
+    lib = native.lib()
+    with native.on_device(dev):
+        need = int(lib.tdb_mx4_scale_bytes(matrices, rows, K, groups))
+        if q is None:
+            q = torch.empty(x.shape[:-1] + (K // 2,), dtype=torch.uint8, device=dev)
+        if sf is None:
+            sf = torch.empty(need, dtype=torch.uint8, device=dev)
+        _need(q.dtype == torch.uint8 and q.shape == x.shape[:-1] + (K // 2,) and q.is_contiguous() and q.device == dev,
+              "q must be contiguous uint8 [..., K/2] on x's device")
+        _need(sf.dtype == torch.uint8 and sf.numel() >= need and sf.is_contiguous() and sf.device == dev,
+              f"sf must be a contiguous uint8 buffer of at least {need} bytes on x's device")
+        native.check(lib.tdb_mx4_quantize(x.data_ptr(), ld, matrices, rows, K,
+                                          0 if offsets is None else offsets.data_ptr(), groups, q.data_ptr(),
+                                          sf.data_ptr(), native.stream_ptr()), "mx4 quantize")
+    return q, sf
+
+
+def dequantize(q, sf, offsets=None, out=None):
+    """The bf16 values of an operand produced by ``quantize`` with the same
+    ``offsets``: exact, but for a value of 2^128, which reads as an infinity."""
+    import torch
+    _need(q.is_cuda, "q must be on a CUDA device")
+    dev = q.device
+    groups = _groups(offsets, dev)
+    matrices, rows, K = _operand(q, sf, groups, dev, "q")
+    _need(offsets is None or q.dim() == 2, "a [matrices, rows, K] operand takes no offsets")
+    shape = q.shape[:-1] + (K,)
+    with native.on_device(dev):
+        out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if out is None else out
+        _need(out.dtype == torch.bfloat16 and out.shape == shape and out.device == dev and out.stride(-1) == 1 and
+              (out.is_contiguous() or (out.dim() == 2 and out.stride(0) >= K)),
+              "out must be bf16 [..., K] with a contiguous last dimension on q's device")
+        ld = out.stride(0) if out.dim() == 2 and rows > 1 else K
+        native.check(native.lib().tdb_mx4_dequantize(q.data_ptr(), sf.data_ptr(), matrices, rows, K,
+                                                     0 if offsets is None else offsets.data_ptr(), groups,
+                                                     out.data_ptr(), ld, native.stream_ptr()), "mx4 dequantize")
+    return out
+
+
+def _product(qx, sfx, qw, sfw, offsets, bias, out, tile):
+    import torch
+    _need(qx.is_cuda and qx.dim() == 2, "qx must be a quantized [rows, K] operand on a CUDA device")
+    dev = qx.device
+    groups = _groups(offsets, dev)
+    _, rows, K = _operand(qx, sfx, groups, dev, "qx")
+    matrices, N, Kw = _operand(qw, sfw, 0, dev, "qw")
+    _need(K == Kw, f"the K extents differ: {K} and {Kw}")
+    _need(matrices == max(groups, 1), "qw must hold one matrix per group")
+    _need(N > 0 and N % 8 == 0, "N must be a positive multiple of 8")
+    if bias is not None:
+        _need(bias.dtype == torch.bfloat16 and bias.numel() == matrices * N and bias.is_contiguous() and
+              bias.device == dev and bias.shape[-1] == N, "bias must be contiguous bf16 [N] or [groups, N]")
+    with native.on_device(dev):
+        out = torch.empty((rows, N), dtype=torch.bfloat16, device=dev) if out is None else out
+        _need(out.dtype == torch.bfloat16 and tuple(out.shape) == (rows, N) and out.stride(1) == 1 and
+              (rows <= 1 or out.stride(0) >= N) and out.device == dev,
+              f"out must be bf16 [{rows}, {N}] with a contiguous last dimension on the operands' device")
+        native.check(native.lib().tdb_mx4_gemm(
+            qx.data_ptr(), sfx.data_ptr(), qw.data_ptr(), sfw.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
+            matrices, out.data_ptr(), out.stride(0) if rows > 1 else N, rows, N, K,
+            0 if bias is None else bias.data_ptr(), tile, native.stream_ptr()), "mx4 product")
+    return out
+
+
+def linear(qx, sfx, qw, sfw, bias=None, out=None, tile=0):
+    """``values(qx) @ values(qw)^T (+ bias)`` in bf16 with fp32 accumulation;
+    qx [M, K], qw [N, K] from ``quantize``."""
+    _need(qw.dim() == 2, "qw must be a quantized [N, K] matrix")
+    return _product(qx, sfx, qw, sfw, None, bias, out, tile)
+
+
+def grouped_linear(qx, sfx, qw, sfw, offsets, bias=None, out=None, tile=0):
+    """``values(qx)[r] @ values(qw)[g]^T (+ bias[g])`` for the rows r of group
+    g; qx [R, K] quantized with these ``offsets``, qw [groups, N, K], bias
+    [groups, N].  Rows outside every group keep their contents."""
+    _need(offsets is not None and qw.dim() == 3, "grouped_linear needs offsets and a quantized [groups, N, K] operand")
+    return _product(qx, sfx, qw, sfw, offsets, bias, out, tile)

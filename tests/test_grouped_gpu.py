@@ -38,7 +38,7 @@ def _status_ok():
     assert native.read_status() == [0, 0, 0, 0]
 
 
-@pytest.mark.parametrize("tile", [0, 128, 512])
+@pytest.mark.parametrize("tile", [0, 32, 128, 512])
 @pytest.mark.parametrize("N,K", SHAPES)
 @pytest.mark.parametrize("sizes", list(SIZES))
 def test_linear(cuda, sizes, N, K, tile):
@@ -66,7 +66,7 @@ def test_linear(cuda, sizes, N, K, tile):
     _status_ok()
 
 
-@pytest.mark.parametrize("tile", [0, 128, 512])
+@pytest.mark.parametrize("tile", [0, 32, 128, 512])
 @pytest.mark.parametrize("N,K", SHAPES)
 @pytest.mark.parametrize("sizes", list(SIZES))
 def test_data_gradient(cuda, sizes, N, K, tile):
@@ -126,7 +126,7 @@ def test_weight_and_bias_gradient(cuda, sizes, N, K, tile):
     _status_ok()
 
 
-@pytest.mark.parametrize("tile", [128, 512])
+@pytest.mark.parametrize("tile", [32, 128, 512])
 def test_foreign_rows_hold_nan_and_stay_as_they_were(cuda, tile):
     """Rows before the first and behind the last group, and rows of other
     groups, are full of NaN and infinities; strided operands and outputs."""
@@ -160,7 +160,7 @@ def test_foreign_rows_hold_nan_and_stay_as_they_were(cuda, tile):
         assert _within(dx[lo:hi], dys[lo:hi].double() @ w[g].double(),
                        dys[lo:hi].double().abs() @ w[g].double().abs(), N)
         assert (dx[:lead] == 7).all() and (dx[R - trail:] == 7).all()
-        dw = grouped.weight_grad(dys, xs, off, tile=tile)
+        dw = grouped.weight_grad(dys, xs, off, tile=max(tile, 128))
         assert _within(dw[g], dys[lo:hi].double().t() @ xs[lo:hi].double(),
                        dys[lo:hi].double().abs().t() @ xs[lo:hi].double().abs(), hi - lo, 2.0 ** -24)
         assert (dw[2] == 0).all()
