@@ -8,7 +8,7 @@ namespace tdb {
 namespace grouped {
 
 template <int CG, int BN>
-__global__ void __launch_bounds__(kThreads, 1) weight_grad_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid_constant__ Params p) {
   mainloop<CG, BN>(p);
 }
 
@@ -18,8 +18,8 @@ static int launch_weight_grad(const Params& p, cudaStream_t stream) {
   static_assert(Cfg::smem_bytes(kMaxGroups) <= 227 * 1024, "shared memory budget");
   const int64_t tiles = int64_t(p.groups) * ((p.M + Cfg::kTileM - 1) / Cfg::kTileM) * ((p.N + BN - 1) / BN);
   static LaunchState state[64];
-  return launch_units<CG>(weight_grad_kernel<CG, BN>, p, tiles, Cfg::smem_bytes(p.groups), Cfg::smem_bytes(kMaxGroups),
-                          state, stream);
+  return launch_units<CG>(weight_grad_kernel<CG, BN>, p, kWgThreads, tiles, Cfg::smem_bytes(p.groups),
+                          Cfg::smem_bytes(kMaxGroups), state, stream);
 }
 
 template <int OP, int MODE>

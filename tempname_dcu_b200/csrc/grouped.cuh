@@ -3,37 +3,57 @@
 //
 //   dW_g[n, k] = sum_{r in group g} dY[r, n] X[r, k]     (both MN-major)
 //
-// for the groups' rows [offsets[g], offsets[g+1]), read on the device.  The
-// last 64-row step of a group whose size is not a multiple of 64 is fetched
-// apart (onto a barrier of this CTA), and the producer warp writes zeros over
-// the next group's rows of both operands before the MMA may read the step: a
-// foreign row may hold NaN, so zeroing one operand would not do.  In the
-// MN-major layout a row is a 128-byte line of each 64-column box, so the zeros
-// need no swizzle.  The fp32 output leaves by TMA stores or, when adding, TMA
-// reduce-adds (one writer per element: deterministic); an empty group's tiles
-// are zeros, or skipped when adding.
+// for the groups' rows [offsets[g], offsets[g+1]), read on the device.
 //
-// Roles and barriers are those of gemm.cuh (CG = 1: 128 x 128 tiles) and
-// gemm2.cuh (CG = 2: 256 x 256 tiles on SM pairs): warp 0 TMA producer, warp 1
-// MMA issuer, warps 2..5 epilogue; all waits are bounded.
+// Partial steps.  The last step of a group whose size is not a multiple of 64
+// holds rows of the next group.  The MMA issues only the K = 16 slices that
+// have rows of the group; when the last slice is partial too, the step's loads
+// complete on a barrier of their own CTA, and a warp writes zeros over the
+// slice's foreign rows in both operands before the MMA may read it (a foreign
+// row may hold NaN, so zeroing one operand would not do).  In the MN-major
+// layout a row is a 128-byte line of each 64-column box, so the zeros need no
+// swizzle.
+//
+// Sums.  The tensor core truncates when it adds to its fp32 accumulator, an
+// error that grows with the number of additions and has one sign: 1170 rows
+// were 2.2e-6 off (relative 2-norm), the output being fp32.  So a chain of
+// MMAs stops after kChain steps (512 rows) and the epilogue warps, which hold
+// the output tile in registers, add the chain's result rounding to nearest;
+// two TMEM accumulators alternate, so the MMAs do not wait.
+//
+// The output leaves by TMA stores or, when adding, TMA reduce-adds (one writer
+// per element: deterministic); an empty group's tiles are zeros, or skipped
+// when adding.
+//
+// Warps: 0 TMA producer, 1 MMA issuer, 2 zeroes foreign rows, 3 reads the
+// offsets, 4..11 epilogue (a quarter of the TMEM lanes and half of the columns
+// each).  CG = 1: 128 x 128 tiles, CG = 2: 256 x 256 tiles on SM pairs with the
+// barriers of gemm2.cuh.  All waits are bounded.
 #pragma once
 #include "grouped_rows.cuh"
 
 namespace tdb {
 namespace grouped {
 
+constexpr int kWgThreads = 384;
+// Registers per thread after the split, per warpgroup of 128 threads: the
+// launch holds 384 x 168 = 64512, and 128 x 72 + 256 x 208 = 62464.
+constexpr int kWgLightRegs = 72, kWgHeavyRegs = 208;
+constexpr int kChain = 8;
+
 template <int CG, int BN>
 struct Config {
   static constexpr int kTileM = 128 * CG;      // output rows per tile (128 per CTA)
-  static constexpr int kBRows = BN / CG;       // output columns whose operand rows this CTA stages
+  static constexpr int kBRows = BN / CG;       // output columns whose operand this CTA stages
   static constexpr int kABytes = 128 * BK * 2;
   static constexpr int kBBytes = kBRows * BK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kStages = 5;
   static constexpr int kTmemCols = 2 * BN;     // two accumulators
-  static constexpr int kEpiBuf = 4096;         // one staged block of an epilogue warp
-  static constexpr int kEpiBytes = 4 * 2 * kEpiBuf;
-  static constexpr int kBarBytes = 256;
+  static constexpr int kWarpCols = BN / 2;     // output columns of an epilogue warp
+  static constexpr int kBuf = 4096;            // 32 rows x 32 fp32 columns, one per epilogue warp
+  static constexpr int kEpiBytes = 8 * kBuf;
+  static constexpr int kBarBytes = 512;
   static_assert(kTmemCols == 256 || kTmemCols == 512, "TMEM columns");
   static constexpr int smem_bytes(int groups) {
     return 1024 + kStages * kStageBytes + kEpiBytes + kBarBytes + (groups + 1) * 4;
@@ -54,23 +74,24 @@ struct alignas(64) Params {
 struct alignas(8) Barriers {
   uint64_t full[8];
   uint64_t empty[8];
+  uint64_t part_full[8];   // this CTA's loads of a partial step, per stage
+  uint64_t part_fixed[8];  // every CTA has zeroed its foreign rows, per stage
   uint64_t tmem_full[2];
   uint64_t tmem_empty[2];
   uint64_t drain;
-  uint64_t tail_full;   // kWeightGrad: this CTA's loads of a partial step
-  uint64_t tail_fixed;  // kWeightGrad: both CTAs have zeroed the foreign rows
   uint32_t tmem_base;
   int abort_flag;
   uint32_t peer_done;
   int bad_offsets;
 };
-static_assert(sizeof(Barriers) <= 256, "barrier slot");
+static_assert(sizeof(Barriers) <= 512, "barrier slot");
 
 struct Tile {
   int g;
   int m0, n0;   // first output row and column
   int k0, kb;   // first summed row and number of BK steps
-  int tail;     // rows of the last step when it is partial, else 0
+  int last;     // rows of the last step, 1..64
+  __device__ __forceinline__ bool patched() const { return (last & 15) != 0; }
 };
 
 template <int CG, int BN>
@@ -89,7 +110,7 @@ __device__ __forceinline__ Tile locate(const Params& p, const int* off, int i) {
   const int count = off[r.g + 1] - off[r.g];
   r.k0 = off[r.g];
   r.kb = (count + BK - 1) / BK;
-  r.tail = count % BK;
+  r.last = count - (r.kb - 1) * BK;
   return r;
 }
 
@@ -148,14 +169,14 @@ __device__ __forceinline__ void mainloop(const Params& p) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 1);
+      mbar_init(&bars->part_full[s], 1);
+      mbar_init(&bars->part_fixed[s], CG);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->tmem_full[b], 1);
-      mbar_init(&bars->tmem_empty[b], 4 * CG);
+      mbar_init(&bars->tmem_empty[b], 8 * CG);
     }
     mbar_init(&bars->drain, 1);
-    mbar_init(&bars->tail_full, 1);
-    mbar_init(&bars->tail_fixed, CG);
     bars->abort_flag = 0;
     bars->peer_done = 0;
     fence_barrier_init();
@@ -171,7 +192,7 @@ __device__ __forceinline__ void mainloop(const Params& p) {
       tmem_relinquish();
     }
   }
-  if (warp == 2) {
+  if (warp == 3) {
     const bool bad = load_offsets(p.offsets, p.groups, p.rows, off, status);
     if (lane == 0) bars->bad_offsets = bad;
   }
@@ -184,162 +205,191 @@ __device__ __forceinline__ void mainloop(const Params& p) {
   const uint32_t tmem_base = bars->tmem_base;
   volatile int* abort_flag = &bars->abort_flag;
   // bad offsets: no tile is computed (both CTAs of a pair read the same offsets)
-  const int tiles = bars->bad_offsets ? 0 : p.groups * ((p.M + Cfg::kTileM - 1) / Cfg::kTileM) * ((p.N + BN - 1) / BN);
+  const int tiles =
+      bars->bad_offsets ? 0 : p.groups * ((p.M + Cfg::kTileM - 1) / Cfg::kTileM) * ((p.N + BN - 1) / BN);
 
-  if (warp == 0) {
-    // ---------------- TMA producer ----------------
-    {  // the whole warp runs this loop (it zeroes foreign rows), lane 0 issues the loads
-      uint32_t it = 0, tails = 0;
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWgLightRegs));
+    if (warp == 0 && lane == 0) {
+      // ---------------- TMA producer ----------------
+      Ring<S> ring;
+      uint32_t issued = 0, part = 0, partial = 0;  // per stage: phase bit of part_full, last use was partial
       bool ok = true;
       for (int i = unit; i < tiles && ok; i += units) {
         const Tile t = locate<CG, BN>(p, off, i);
-        if (t.kb == 0 && p.accumulate) continue;
         const int m0 = t.m0 + int(rank) * 128, n0 = t.n0 + int(rank) * Cfg::kBRows;
-        for (int kb = 0; kb < t.kb; ++kb, ++it) {
-          const int s = it % S;
-          bool go = mbar_wait(&bars->empty[s], ((it / S) & 1) ^ 1, status, 310) && !*abort_flag;
-          go = __all_sync(0xffffffffu, go);
-          if (!go) { ok = false; *abort_flag = 1; break; }
+        int k0 = t.k0;
+        for (int kb = 0; kb < t.kb; ++kb, k0 += BK, ring.next(), ++issued) {
+          const int s = ring.s;
+          if (!mbar_wait(&bars->empty[s], ring.phase ^ 1, status, 310)) {
+            ok = false;
+            *abort_flag = 1;
+            break;
+          }
           uint8_t* sa = smem + s * Cfg::kStageBytes;
           uint8_t* sb = sa + Cfg::kABytes;
-          const bool partial = t.tail != 0 && kb == t.kb - 1;
-          const int k0 = t.k0 + kb * BK;
-          if (lane == 0) {
-            if (!partial) {
-              uint64_t* bar = &bars->full[s];
-              if (rank == 0) mbar_arrive_expect_tx(bar, CG * Cfg::kStageBytes);
+          if (kb != t.kb - 1 || !t.patched()) {
+            uint64_t* bar = &bars->full[s];
+            partial &= ~(1u << s);
+            if (rank == 0) mbar_arrive_expect_tx(bar, CG * Cfg::kStageBytes);
 #pragma unroll
-              for (int j = 0; j < 2; ++j) load_2d<CG>(sa + j * (BK * 128), &p.tmA, bar, m0 + 64 * j, k0);
+            for (int j = 0; j < 2; ++j) load_2d<CG>(sa + j * (BK * 128), &p.tmA, bar, m0 + 64 * j, k0);
 #pragma unroll
-              for (int j = 0; j < Cfg::kBRows / 64; ++j) load_2d<CG>(sb + j * (BK * 128), &p.tmB, bar, n0 + 64 * j, k0);
-            } else {
-              uint64_t* bar = &bars->tail_full;
-              mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
+            for (int j = 0; j < Cfg::kBRows / 64; ++j) load_2d<CG>(sb + j * (BK * 128), &p.tmB, bar, n0 + 64 * j, k0);
+          } else {
+            uint64_t* bar = &bars->part_full[s];
+            partial |= 1u << s;
+            part ^= 1u << s;
+            mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
 #pragma unroll
-              for (int j = 0; j < 2; ++j) tma_load_2d(sa + j * (BK * 128), &p.tmA, bar, m0 + 64 * j, k0);
+            for (int j = 0; j < 2; ++j) tma_load_2d(sa + j * (BK * 128), &p.tmA, bar, m0 + 64 * j, k0);
 #pragma unroll
-              for (int j = 0; j < Cfg::kBRows / 64; ++j) tma_load_2d(sb + j * (BK * 128), &p.tmB, bar, n0 + 64 * j, k0);
-            }
-          }
-          if (partial) {
-            // zeros over the rows of the next group, in both operands
-            const bool landed = mbar_wait(&bars->tail_full, tails & 1, status, 311);
-            if (!__all_sync(0xffffffffu, landed)) { ok = false; *abort_flag = 1; break; }
-            ++tails;
-            constexpr int kBoxes = Cfg::kStageBytes / (BK * 128);
-            const int lines = (BK - t.tail) * 8;  // 16-byte lines of the foreign rows of one box
-            for (int j = lane; j < kBoxes * lines; j += 32) {
-              const int box = j / lines, q = j - box * lines;
-              *reinterpret_cast<uint4*>(sa + box * (BK * 128) + t.tail * 128 + q * 16) = make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-              arrive_leader<CG>(&bars->tail_fixed);
-              if (rank == 0) mbar_arrive(&bars->full[s]);  // keeps the ring's phases
-            }
+            for (int j = 0; j < Cfg::kBRows / 64; ++j) tma_load_2d(sb + j * (BK * 128), &p.tmB, bar, n0 + 64 * j, k0);
+            if (rank == 0) mbar_arrive(&bars->full[s]);  // keeps the ring's phases; the MMA waits for part_fixed
           }
         }
       }
-      if (!ok && rank == 0 && lane == 0) {
+      if (!ok) {
         // Drain: wait (bounded) for every stage that may still have bytes in flight.
-        for (uint32_t j = (it >= S ? it - S : 0); j < it; ++j) mbar_wait(&bars->full[j % S], (j / S) & 1, status, 312);
+        if (rank == 0)
+          for (uint32_t j = (issued >= S ? issued - S : 0); j < issued; ++j)
+            mbar_wait(&bars->full[j % S], (j / S) & 1, status, 312);
+        for (int s = 0; s < S; ++s)
+          if ((partial >> s) & 1) mbar_wait(&bars->part_full[s], ((part >> s) & 1) ^ 1, status, 313);
       }
-    }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0 && rank == 0) {
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      // ---------------- MMA issuer ----------------
       constexpr uint32_t idesc = idesc_bf16(Cfg::kTileM, BN, true, true);
-      uint32_t it = 0, tails = 0;
-      int tc = 0;
+      Ring<S> ring;
+      uint32_t part = 0;  // phase bit of each stage's part_fixed
+      int tc = 0;         // chains
       bool ok = true, issued = false;
+      const uint64_t a_desc = gemm::desc_mnmajor(smem_u32(smem));
+      const uint64_t b_desc = gemm::desc_mnmajor(smem_u32(smem) + Cfg::kABytes);
       for (int i = unit; i < tiles && ok; i += units) {
         const Tile t = locate<CG, BN>(p, off, i);
-        if (t.kb == 0 && p.accumulate) continue;
-        const int b = tc & 1;
-        if (!mbar_wait(&bars->tmem_empty[b], ((tc >> 1) & 1) ^ 1, status, 320)) { ok = false; *abort_flag = 1; break; }
-        tc_fence_after();
-        const uint32_t dcol = tmem_base + b * BN;
-        for (int kb = 0; kb < t.kb; ++kb, ++it) {
-          const int s = it % S;
-          if (!mbar_wait(&bars->full[s], (it / S) & 1, status, 321)) { ok = false; *abort_flag = 1; break; }
-          if (t.tail != 0 && kb == t.kb - 1) {
-            if (!mbar_wait_cluster(&bars->tail_fixed, tails & 1, status, 322)) { ok = false; *abort_flag = 1; break; }
-            ++tails;
-          }
-          if (*abort_flag) { ok = false; break; }
+        for (int c0 = 0; c0 < t.kb && ok; c0 += kChain, ++tc) {
+          const int b = tc & 1, c1 = min(c0 + kChain, t.kb);
+          if (!mbar_wait(&bars->tmem_empty[b], ((tc >> 1) & 1) ^ 1, status, 320)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * Cfg::kStageBytes);
-          const uint32_t sb = sa + Cfg::kABytes;
+          const uint32_t dcol = tmem_base + b * BN;
+          for (int kb = c0; kb < c1; ++kb, ring.next()) {
+            const int s = ring.s;
+            if (!mbar_wait(&bars->full[s], ring.phase, status, 321)) { ok = false; break; }
+            int slices = BK / 16;
+            if (kb == t.kb - 1) {
+              slices = (t.last + 15) >> 4;
+              if (t.patched()) {
+                if (!mbar_wait_cluster(&bars->part_fixed[s], (part >> s) & 1, status, 322)) { ok = false; break; }
+                part ^= 1u << s;
+              }
+            }
+            tc_fence_after();
+            const uint64_t ad = a_desc + uint32_t(s * (Cfg::kStageBytes >> 4));
+            const uint64_t bd = b_desc + uint32_t(s * (Cfg::kStageBytes >> 4));
+            issue<CG>(dcol, ad, bd, idesc, kb != c0 ? 1u : 0u);
+            if (slices == BK / 16) {
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            const uint64_t ad = gemm::desc_mnmajor(sa + k * 16 * 128);
-            const uint64_t bd = gemm::desc_mnmajor(sb + k * 16 * 128);
-            if (CG == 2)
-              gemm2::umma2_f16_ss(dcol, ad, bd, idesc, (kb | k) != 0 ? 1u : 0u);
-            else
-              umma_f16_ss(dcol, ad, bd, idesc, (kb | k) != 0 ? 1u : 0u);
+              for (int k = 1; k < BK / 16; ++k) issue<CG>(dcol, ad + k * 128, bd + k * 128, idesc, 1u);
+            } else {
+              for (int k = 1; k < slices; ++k) issue<CG>(dcol, ad + k * 128, bd + k * 128, idesc, 1u);
+            }
+            issued = true;
+            commit<CG>(&bars->empty[s]);
           }
-          issued = true;
-          commit<CG>(&bars->empty[s]);
+          if (ok) commit<CG>(&bars->tmem_full[b]);
         }
-        if (ok) commit<CG>(&bars->tmem_full[b]);
-        ++tc;
       }
+      if (!ok) *abort_flag = 1;
       // Every MMA has landed before TMEM is released.
       if (issued) {
         commit<CG>(&bars->drain);
         mbar_wait(&bars->drain, 0, status, 323);
       }
-    }
-  } else {
-    // ---------------- Epilogue (warps 2..5) ----------------
-    const int quarter = warp & 3;  // TMEM lanes [32*quarter, 32*quarter+32)
-    const uint32_t base = smem_u32(epi_smem) + uint32_t(quarter * 2 * Cfg::kEpiBuf);
-    int tc = 0, staged = 0;
-    for (int i = unit; i < tiles; i += units) {
-      const Tile t = locate<CG, BN>(p, off, i);
-      if (t.kb == 0 && p.accumulate) continue;
-      const int b = tc & 1;
-      bool ok = mbar_wait(&bars->tmem_full[b], (tc >> 1) & 1, status, 330);
-      if (*abort_flag) ok = false;
-      if (!ok) { *abort_flag = 1; break; }
-      tc_fence_after();
-      const int row0 = t.m0 + int(rank) * 128 + quarter * 32;
-#pragma unroll 1
-      for (int c = 0; c < BN / 32; ++c) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tmem_base + (uint32_t(quarter * 32) << 16) + b * BN + c * 32, r);
-        tmem_wait_ld();
-        if (c == BN / 32 - 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_leader<CG>(&bars->tmem_empty[b]);
-        }
-        const int col = t.n0 + c * 32;
-        if (row0 >= p.M || col >= p.N) continue;
-        const uint32_t buf = base + uint32_t((staged & 1) * Cfg::kEpiBuf);
-        if (staged >= 2) {  // the bulk store that last read the buffer is done with it
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          __syncwarp();
-        }
-        const uint32_t rowa = buf + uint32_t(lane * 128), sw = uint32_t(lane & 7);
-        const bool zero = t.kb == 0;
+    } else if (warp == 2) {
+      // ---------------- Foreign rows ----------------
+      uint32_t it = 0, part = 0;  // steps before and in this tile; phase bit of each stage's part_full
+      for (int i = unit; i < tiles; i += units) {
+        const Tile t = locate<CG, BN>(p, off, i);
+        it += t.kb;
+        if (t.kb == 0 || !t.patched()) continue;
+        const int s = (it - 1) % S;
+        bool go = mbar_wait(&bars->part_full[s], (part >> s) & 1, status, 311) && !*abort_flag;
+        if (!__all_sync(0xffffffffu, go)) { *abort_flag = 1; break; }
+        part ^= 1u << s;
+        constexpr int kBoxes = Cfg::kStageBytes / (BK * 128);
+        const int lines = (16 - (t.last & 15)) * 8;  // 16-byte lines of a box up to the slice's end
+        uint8_t* from = smem + s * Cfg::kStageBytes + t.last * 128;
+        for (int j = lane; j < lines; j += 32) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(rowa + ((uint32_t(k) ^ sw) << 4)),
-                       "r"(zero ? 0u : r[4 * k]), "r"(zero ? 0u : r[4 * k + 1]), "r"(zero ? 0u : r[4 * k + 2]),
-                       "r"(zero ? 0u : r[4 * k + 3])
-                       : "memory");
+          for (int box = 0; box < kBoxes; ++box)
+            *reinterpret_cast<uint4*>(from + box * (BK * 128) + j * 16) = make_uint4(0, 0, 0, 0);
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) {
-          bulk_store_3d(&p.tmC, buf, col, row0, t.g, p.accumulate != 0);
-          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        }
-        ++staged;
+        if (lane == 0) arrive_leader<CG>(&bars->part_fixed[s]);
       }
-      ++tc;
+    }
+  } else {
+    // ---------------- Epilogue (warps 4..11) ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWgHeavyRegs));
+    constexpr int kCols = Cfg::kWarpCols;
+    const int quarter = warp & 3;  // TMEM lanes [32*quarter, 32*quarter+32)
+    const int half = (warp - 4) >> 2;
+    const uint32_t buf = smem_u32(epi_smem) + uint32_t((warp - 4) * Cfg::kBuf);
+    int tc = 0;
+    bool ok = true;
+    for (int i = unit; i < tiles && ok; i += units) {
+      const Tile t = locate<CG, BN>(p, off, i);
+      if (t.kb == 0 && p.accumulate) continue;
+      float acc[kCols];
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
+      for (int kb = 0; kb < t.kb; kb += kChain, ++tc) {
+        const int b = tc & 1;
+        ok = mbar_wait(&bars->tmem_full[b], (tc >> 1) & 1, status, 330);
+        if (*abort_flag) ok = false;
+        if (!ok) { *abort_flag = 1; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(tmem_base + (uint32_t(quarter * 32) << 16) + b * BN + half * kCols + c * 32, r);
+          tmem_wait_ld();
+          if (c == kCols / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_leader<CG>(&bars->tmem_empty[b]);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[c * 32 + j] += __uint_as_float(r[j]);
+        }
+      }
+      if (!ok) break;
+      const int row0 = t.m0 + int(rank) * 128 + quarter * 32;
+      if (row0 >= p.M) continue;
+#pragma unroll
+      for (int c = 0; c < kCols / 32; ++c) {
+        const int col = t.n0 + half * kCols + c * 32;
+        if (col < p.N) {
+          // the bulk store that last read the buffer is done with it
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+          const uint32_t rowa = buf + uint32_t(lane * 128), sw = uint32_t(lane & 7);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(rowa + ((uint32_t(k) ^ sw) << 4)),
+                         "f"(acc[c * 32 + 4 * k]), "f"(acc[c * 32 + 4 * k + 1]), "f"(acc[c * 32 + 4 * k + 2]),
+                         "f"(acc[c * 32 + 4 * k + 3])
+                         : "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            bulk_store_3d(&p.tmC, buf, col, row0, t.g, p.accumulate != 0);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        }
+      }
     }
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }

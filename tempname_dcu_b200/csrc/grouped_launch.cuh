@@ -16,7 +16,7 @@ struct LaunchState {
 // Launches `kern` on as many CTAs (CG = 1) or SM pairs (CG = 2) as there are
 // tiles, at most one per SM of the caller's share.
 template <int CG, class P>
-static int launch_units(void (*kern)(P), const P& p, int64_t tiles, int smem, int max_smem, LaunchState* states,
+static int launch_units(void (*kern)(P), const P& p, int threads, int64_t tiles, int smem, int max_smem, LaunchState* states,
                         cudaStream_t stream) {
   if (tiles >= (int64_t(1) << 31)) return tdb_host::fail(int(cudaErrorInvalidValue), "grouped: more than 2^31 output tiles");
   int dev = 0;
@@ -28,7 +28,7 @@ static int launch_units(void (*kern)(P), const P& p, int64_t tiles, int smem, in
   attr[0].val.clusterDim.x = CG;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(unsigned(threads));
   cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -69,7 +69,7 @@ static int launch_rows(const RowsParams& p, cudaStream_t stream) {
   const int64_t row_tiles = p.rows / BT + (p.rows < p.groups ? p.rows : p.groups);
   const int64_t tiles = row_tiles * ((p.N + Cfg::kTileN - 1) / Cfg::kTileN);
   static LaunchState state[64];
-  return launch_units<CG>(rows_kernel<CG, BT, OP, MODE, MX4>, p, tiles, Cfg::smem_bytes(p.groups),
+  return launch_units<CG>(rows_kernel<CG, BT, OP, MODE, MX4>, p, kThreads, tiles, Cfg::smem_bytes(p.groups),
                           Cfg::smem_bytes(kMaxGroups), state, stream);
 }
 

@@ -213,6 +213,20 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
       : "memory");
 }
 
+// Position in the ring of S stages.  The issuing threads have a few hundred
+// cycles per step, so it is stepped, not divided.
+template <int S>
+struct Ring {
+  int s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == S) {
+      s = 0;
+      phase ^= 1;
+    }
+  }
+};
+
 template <int CG>
 __device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
   if (CG == 2)
@@ -233,6 +247,13 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
     gemm2::umma2_commit_both(bar);
   else
     umma_commit(bar);
+}
+template <int CG>
+__device__ __forceinline__ void issue(uint32_t tmem_d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
+  if (CG == 2)
+    gemm2::umma2_f16_ss(tmem_d, ad, bd, idesc, accumulate);
+  else
+    umma_f16_ss(tmem_d, ad, bd, idesc, accumulate);
 }
 template <int CG>
 __device__ __forceinline__ void arrive_leader(uint64_t* bar) {
@@ -499,6 +520,7 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     if (lane == 0) {
+      Ring<S> ring;
       uint32_t it = 0;
       bool ok = true;
       for (int i = unit; i < tiles && ok; i += units) {
@@ -507,10 +529,9 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
         const int share = t.mma_n / CG;
         const int b0 = t.r0 + int(rank) * share;  // and its share of the token rows
         const int boxes = (share + Cfg::kBox - 1) / Cfg::kBox;
-        for (int kb = 0; kb < num_kb; ++kb, ++it) {
-          const int s = it % S;
-          if (!mbar_wait(&bars->empty[s], ((it / S) & 1) ^ 1, status, 310)) { ok = false; *abort_flag = 1; break; }
-          if (*abort_flag) { ok = false; break; }
+        for (int kb = 0; kb < num_kb; ++kb, ++it, ring.next()) {
+          const int s = ring.s;
+          if (!mbar_wait(&bars->empty[s], ring.phase ^ 1, status, 310)) { ok = false; *abort_flag = 1; break; }
           uint8_t* sa = smem + s * Cfg::kStageBytes;
           uint8_t* sb = sa + Cfg::kABytes;
           uint64_t* bar = &bars->full[s];
@@ -546,27 +567,30 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     if (lane == 0 && rank == 0) {
-      uint32_t it = 0;
+      Ring<S> ring;
       int tc = 0;
       bool ok = true, issued = false;
+      const uint32_t smem0 = smem_u32(smem);
+      const uint64_t a_desc = kAMn ? gemm::desc_mnmajor(smem0) : gemm::desc_kmajor(smem0);
+      const uint64_t b_desc = gemm::desc_kmajor(smem0 + Cfg::kABytes);
+      constexpr int kAStep = (kAMn ? 16 * 128 : 32) >> 4, kBStep = 32 >> 4;  // descriptor units per MMA
       for (int i = unit; i < tiles && ok; i += units) {
         const RowsTile t = rows_locate<CG, BT, MX4>(p, table, i);
         const int b = Cfg::kAccums == 2 ? (tc & 1) : 0;
         const int use = Cfg::kAccums == 2 ? (tc >> 1) : tc;
-        if (!mbar_wait(&bars->tmem_empty[b], (use & 1) ^ 1, status, 320)) { ok = false; *abort_flag = 1; break; }
+        if (!mbar_wait(&bars->tmem_empty[b], (use & 1) ^ 1, status, 320)) { ok = false; break; }
         tc_fence_after();
         const uint32_t dcol = tmem_base + b * BT;
         const uint32_t idesc = MX4 ? idesc_mxf4(128 * CG, t.mma_n)
                                    : (idesc_bf16(128 * CG, 0, kAMn, false) | (uint32_t(t.mma_n >> 3) << 17));
-        for (int kb = 0; kb < num_kb; ++kb, ++it) {
-          const int s = it % S;
-          if (!mbar_wait(&bars->full[s], (it / S) & 1, status, 321)) { ok = false; *abort_flag = 1; break; }
-          if (*abort_flag) { ok = false; break; }
+        for (int kb = 0; kb < num_kb; ++kb, ring.next()) {
+          const int s = ring.s;
+          if (!mbar_wait(&bars->full[s], ring.phase, status, 321)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * Cfg::kStageBytes);
-          const uint32_t sb = sa + Cfg::kABytes;
+          const uint64_t ad = a_desc + uint32_t(s * (Cfg::kStageBytes >> 4));
+          const uint64_t bd = b_desc + uint32_t(s * (Cfg::kStageBytes >> 4));
           if (MX4) {
-            const uint32_t sf = sb + Cfg::kBBytes;
+            const uint32_t sf = smem0 + s * Cfg::kStageBytes + Cfg::kABytes + Cfg::kBBytes;
             const uint32_t sfa = tmem_base + Cfg::kAccums * BT + s * Cfg::kSfCols, sfb = sfa + 8;
             // columns: [atom 0 | atom 1] of A, then per atom the blocks of B side by side
 #pragma unroll
@@ -578,19 +602,12 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_mxf4<CG>(dcol, gemm::desc_kmajor(sa + k * 32), gemm::desc_kmajor(sb + k * 32), idesc,
-                            sfa + 4 * (k >> 1), sfb + 4 * Cfg::kBlocksB * (k >> 1), uint32_t(2 * (k & 1)),
-                            (kb | k) != 0 ? 1u : 0u);
+              umma_mxf4<CG>(dcol, ad + k * kAStep, bd + k * kBStep, idesc, sfa + 4 * (k >> 1),
+                            sfb + 4 * Cfg::kBlocksB * (k >> 1), uint32_t(2 * (k & 1)), k != 0 || kb != 0 ? 1u : 0u);
           } else {
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k) {
-              const uint64_t ad = kAMn ? gemm::desc_mnmajor(sa + k * 16 * 128) : gemm::desc_kmajor(sa + k * 32);
-              const uint64_t bd = gemm::desc_kmajor(sb + k * 32);
-              if (CG == 2)
-                gemm2::umma2_f16_ss(dcol, ad, bd, idesc, (kb | k) != 0 ? 1u : 0u);
-              else
-                umma_f16_ss(dcol, ad, bd, idesc, (kb | k) != 0 ? 1u : 0u);
-            }
+            for (int k = 0; k < BK / 16; ++k)
+              issue<CG>(dcol, ad + k * kAStep, bd + k * kBStep, idesc, k != 0 || kb != 0 ? 1u : 0u);
           }
           issued = true;
           commit<CG>(&bars->empty[s]);
@@ -598,6 +615,7 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
         if (ok) commit<CG>(&bars->tmem_full[b]);
         ++tc;
       }
+      if (!ok) *abort_flag = 1;
       // Every MMA has landed before TMEM is released.
       if (issued) {
         commit<CG>(&bars->drain);

@@ -26,7 +26,9 @@ constexpr int kMaxExperts = 512;
 constexpr int kMaxTopK = 16;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kTokensPerBlock = 64;  // routing: 8 tokens per warp; up to 64 tokens are routed by one launch
+constexpr int kRouteThreads = 1024;    // routing: 32 warps
+constexpr int kTokensPerBlock = 128;   // four tokens per warp; up to 128 tokens are routed by one launch
+constexpr int kRankWarps = 8;          // warps that rank a block's choices
 
 // Monotone map float -> uint32 (larger float, larger key); both zeros map to
 // the same key, NaN to the largest.  Every key of a float is > 0.
@@ -134,20 +136,21 @@ __device__ __forceinline__ void scan_experts(const int* total, int* start, int E
 }
 
 // Stable ranks of the block's choices [c0, c1): base[e] is the first slot of
-// the block's choices of expert e.  Warp w owns a contiguous share, so ranks
-// follow the choice index.  wh: [kWarps][E] shared ints.
+// the block's choices of expert e.  Warp w < kRankWarps owns a contiguous
+// share, so ranks follow the choice index.  wh: [kRankWarps][E] shared ints.
 __device__ __forceinline__ void rank_choices(const int* ids, int c0, int c1, int E, const int* base, int* wh,
                                              int* __restrict__ order, int* __restrict__ slots) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int share = ((c1 - c0 + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int lo = min(c0 + warp * share, c1), hi = min(lo + share, c1);
-  for (int i = threadIdx.x; i < kWarps * E; i += kThreads) wh[i] = 0;
+  const int share = ((c1 - c0 + kRankWarps - 1) / kRankWarps + 31) / 32 * 32;
+  const int lo = warp < kRankWarps ? min(c0 + warp * share, c1) : c1, hi = min(lo + share, c1);
+  for (int i = threadIdx.x; i < kRankWarps * E; i += kRouteThreads) wh[i] = 0;
   __syncthreads();
   for (int c = lo + lane; c < hi; c += 32) atomicAdd(&wh[warp * E + ids[c]], 1);
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kThreads) {
+  for (int e = threadIdx.x; e < E; e += kRouteThreads) {
     int run = base[e];
-    for (int w = 0; w < kWarps; ++w) {
+#pragma unroll
+    for (int w = 0; w < kRankWarps; ++w) {
       const int n = wh[w * E + e];
       wh[w * E + e] = run;
       run += n;
@@ -175,17 +178,18 @@ __device__ __forceinline__ void rank_choices(const int* ids, int c0, int c1, int
 // Top k, weights and the block's expert counts; with one block also the
 // grouping (hist unused).
 template <int NP, typename T>
-__global__ void __launch_bounds__(kThreads) choose_kernel(const T* __restrict__ logits, int64_t ld, int tokens, int E,
-                                                          int k, int normalize, int* ids, float* __restrict__ weights,
-                                                          int* __restrict__ hist, int* __restrict__ offsets,
-                                                          int* __restrict__ order, int* __restrict__ slots) {
+__global__ void __launch_bounds__(kRouteThreads) choose_kernel(const T* __restrict__ logits, int64_t ld, int tokens, int E,
+                                                               int k, int normalize, int* ids,
+                                                               float* __restrict__ weights, int* __restrict__ hist,
+                                                               int* __restrict__ offsets, int* __restrict__ order,
+                                                               int* __restrict__ slots) {
   extern __shared__ int sh[];
   int* count = sh;  // [E]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < E; e += kThreads) count[e] = 0;
+  for (int e = threadIdx.x; e < E; e += kRouteThreads) count[e] = 0;
   __syncthreads();
   const int t0 = blockIdx.x * kTokensPerBlock, t1 = min(t0 + kTokensPerBlock, tokens);
-  for (int t = t0 + warp; t < t1; t += kWarps) {
+  for (int t = t0 + warp; t < t1; t += kRouteThreads / 32) {
     int id;
     float w;
     choose<NP, T>(logits + int64_t(t) * ld, E, k, normalize, id, w);
@@ -197,51 +201,58 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const T* __restrict__ 
   }
   __syncthreads();
   if (gridDim.x > 1) {
-    for (int e = threadIdx.x; e < E; e += kThreads) hist[int64_t(blockIdx.x) * E + e] = count[e];
+    for (int e = threadIdx.x; e < E; e += kRouteThreads) hist[int64_t(blockIdx.x) * E + e] = count[e];
     return;
   }
   int* start = sh + E;           // [E + 1]
-  int* wh = start + E + 1;       // [kWarps][E]
+  int* wh = start + E + 1;       // [kRankWarps][E]
   if (warp == 0) scan_experts(count, start, E);
   __syncthreads();
-  for (int e = threadIdx.x; e <= E; e += kThreads) offsets[e] = start[e];
+  for (int e = threadIdx.x; e <= E; e += kRouteThreads) offsets[e] = start[e];
   rank_choices(ids, 0, tokens * k, E, start, wh, order, slots);
 }
 
 // Slots of one block's choices from every block's counts.
-__global__ void __launch_bounds__(kThreads) group_kernel(const int* __restrict__ ids, const int* __restrict__ hist,
-                                                         int blocks, int tokens, int E, int k, int* __restrict__ offsets,
-                                                         int* __restrict__ order, int* __restrict__ slots) {
+__global__ void __launch_bounds__(kRouteThreads) group_kernel(const int* __restrict__ ids, const int* __restrict__ hist,
+                                                              int blocks, int tokens, int E, int k,
+                                                              int* __restrict__ offsets, int* __restrict__ order,
+                                                              int* __restrict__ slots) {
   extern __shared__ int sh[];
   int* total = sh;          // [E]
   int* before = sh + E;     // [E]
   int* start = before + E;  // [E + 1]
-  int* wh = start + E + 1;  // [kWarps][E]
-  for (int e = threadIdx.x; e < E; e += kThreads) total[e] = before[e] = 0;
+  int* wh = start + E + 1;  // [kRankWarps][E]
+  for (int e = threadIdx.x; e < E; e += kRouteThreads) total[e] = before[e] = 0;
   __syncthreads();
-  // thread (lane over experts, group over blocks): coalesced rows of hist
-  const int wide = E < kThreads ? (E + 31) / 32 * 32 : kThreads;
-  const int groups = kThreads / wide;
-  const int part = threadIdx.x / wide;
-  if (part < groups) {
-    for (int e = threadIdx.x % wide; e < E; e += wide) {
-      int all = 0, mine = 0;
-#pragma unroll 8
-      for (int b = part; b < blocks; b += groups) {
-        const int n = __ldg(hist + int64_t(b) * E + e);
-        all += n;
-        mine += b < int(blockIdx.x) ? n : 0;
+  // A thread sums the counts of one expert over every `groups`-th block, eight
+  // loads at a time (each is an L2 round trip).
+  const int wide = (E + 31) / 32 * 32;
+  const int groups = kRouteThreads / wide;
+  const int part = threadIdx.x / wide, e = threadIdx.x % wide;
+  if (part < groups && e < E) {
+    int all = 0, mine = 0;
+    for (int b0 = part; b0 < blocks; b0 += 8 * groups) {
+      int n[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int b = b0 + i * groups;
+        n[i] = b < blocks ? __ldg(hist + int64_t(b) * E + e) : 0;
       }
-      atomicAdd(&total[e], all);
-      atomicAdd(&before[e], mine);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        all += n[i];
+        mine += b0 + i * groups < int(blockIdx.x) ? n[i] : 0;
+      }
     }
+    atomicAdd(&total[e], all);
+    atomicAdd(&before[e], mine);
   }
   __syncthreads();
   if (threadIdx.x < 32) scan_experts(total, start, E);
   __syncthreads();
   if (blockIdx.x == 0)
-    for (int e = threadIdx.x; e <= E; e += kThreads) offsets[e] = start[e];
-  for (int e = threadIdx.x; e < E; e += kThreads) before[e] += start[e];
+    for (int i = threadIdx.x; i <= E; i += kRouteThreads) offsets[i] = start[i];
+  for (int i = threadIdx.x; i < E; i += kRouteThreads) before[i] += start[i];
   __syncthreads();
   const int t0 = blockIdx.x * kTokensPerBlock, t1 = min(t0 + kTokensPerBlock, tokens);
   rank_choices(ids, t0 * k, t1 * k, E, before, wh, order, slots);
@@ -478,10 +489,10 @@ template <typename T>
 static int route(const T* logits, int64_t ld, int tokens, int E, int k, int normalize, int* ids, float* weights,
                  int* offsets, int* order, int* slots, int* hist, cudaStream_t s) {
   const int blocks = tokens > 0 ? (tokens + kTokensPerBlock - 1) / kTokensPerBlock : 1;
-  const size_t one = size_t(2 * E + 1 + kWarps * E) * 4, many = size_t(E) * 4;
+  const size_t one = size_t(2 * E + 1 + kRankWarps * E) * 4, many = size_t(E) * 4;
   const size_t smem = blocks == 1 ? one : many;
 #define TDB_CHOOSE(NP) \
-  choose_kernel<NP, T><<<blocks, kThreads, smem, s>>>(logits, ld, tokens, E, k, normalize, ids, weights, hist, offsets, order, slots)
+  choose_kernel<NP, T><<<blocks, kRouteThreads, smem, s>>>(logits, ld, tokens, E, k, normalize, ids, weights, hist, offsets, order, slots)
   if (E <= 32) TDB_CHOOSE(1);
   else if (E <= 64) TDB_CHOOSE(2);
   else if (E <= 128) TDB_CHOOSE(4);
@@ -490,8 +501,8 @@ static int route(const T* logits, int64_t ld, int tokens, int E, int k, int norm
 #undef TDB_CHOOSE
   tdb_host::launched(1);
   if (blocks > 1) {
-    group_kernel<<<blocks, kThreads, size_t(3 * E + 1 + kWarps * E) * 4, s>>>(ids, hist, blocks, tokens, E, k, offsets,
-                                                                             order, slots);
+    group_kernel<<<blocks, kRouteThreads, size_t(3 * E + 1 + kRankWarps * E) * 4, s>>>(ids, hist, blocks, tokens, E, k,
+                                                                                      offsets, order, slots);
     tdb_host::launched(1);
   }
   return int(cudaGetLastError());

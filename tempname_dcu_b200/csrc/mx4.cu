@@ -15,6 +15,8 @@
 // step of the product is 256 values); blocks past K hold byte 0.  With
 // offsets the rows of each group start a new 128-row block, so that a tile of
 // the grouped product starts at a block wherever its group starts.
+#include <cuda_fp16.h>
+
 #include "grouped_launch.cuh"
 
 namespace tdb {
@@ -23,7 +25,7 @@ namespace mx4 {
 using grouped::kMaxGroups;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBatch = 4;  // 256-value pieces in flight per warp
+constexpr int kBatch = 4;  // 256-value pieces of a row in flight per warp
 
 // Block exponent from the bits of the largest |bf16|: the smallest e with
 // a <= 6 * 2^e = 1.5 * 2^(e + 2), at least -127 (also for 0 and subnormals).
@@ -47,11 +49,22 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
   return r;
 }
 
-// Magnitude code m (3 bits) as a float: m * 0.5 below 2, else (1 + m % 2 / 2) * 2^(m / 2 - 1).
-__device__ __forceinline__ float e2m1_value(uint32_t code) {
-  const uint32_t m = code & 7u;
-  const float a = m < 2u ? 0.5f * float(m) : __uint_as_float(((126u + (m >> 1)) << 23) | ((m & 1u) << 22));
-  return __uint_as_float(__float_as_uint(a) | ((code & 8u) << 28));
+__device__ __forceinline__ void e2m1x8_values(uint32_t q, float (&v)[8]) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(q));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
+  }
 }
 
 struct Layout {
@@ -60,11 +73,11 @@ struct Layout {
   int groups;
   int rows, mat_blocks;  // without offsets: rows and blocks of one matrix
   // Scale block and row in it of row `r`; false for a row outside every group.
-  __device__ __forceinline__ bool find(int64_t r, int64_t& blk, int& in) const {
+  __device__ __forceinline__ bool find(int r, int64_t& blk, int& in) const {
     if (!off) {
-      const int64_t m = r / rows;
-      const int local = int(r - m * rows);
-      blk = m * mat_blocks + local / 128;
+      const int m = r / rows;
+      const int local = r - m * rows;
+      blk = int64_t(m) * mat_blocks + local / 128;
       in = local % 128;
       return true;
     }
@@ -72,9 +85,9 @@ struct Layout {
     int lo = 0, hi = groups - 1;  // the last group that starts at or before r holds it
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (off[mid] <= int(r)) lo = mid; else hi = mid - 1;
+      if (off[mid] <= r) lo = mid; else hi = mid - 1;
     }
-    const int local = int(r) - off[lo];
+    const int local = r - off[lo];
     blk = block[lo] + local / 128;
     in = local % 128;
     return true;
@@ -106,8 +119,10 @@ __device__ __forceinline__ bool make_layout(Layout& l, const int* offsets, int g
   return !bad_offsets;
 }
 
-// A warp takes 256 consecutive values of a row (two scale words), a lane 8.
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, int64_t total_rows,
+// A warp takes up to kBatch pieces of 256 consecutive values of a row (a pair
+// of atoms' words each) at once, a lane 8 values of each.  Bound by the memory:
+// no division on the way (the row comes from the block, the pieces from its y).
+__global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, int total_rows,
                                                             int K, uint8_t* __restrict__ q, uint8_t* __restrict__ sf,
                                                             const int* offsets, int groups, int rows, int mat_blocks,
                                                             int* status) {
@@ -116,27 +131,22 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __re
   if (!make_layout(l, offsets, groups, rows, mat_blocks, sh, status)) return;
   const int lane = threadIdx.x & 31;
   const int pieces = (K + 255) / 256;
-  const int64_t total = total_rows * pieces;
-  const int64_t step = int64_t(gridDim.x) * kWarps;
-  for (int64_t i0 = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); i0 < total; i0 += step * kBatch) {
+  const int first = blockIdx.y * kBatch;
+  for (int r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < total_rows; r += gridDim.x * kWarps) {
+    const int k0 = first * 256 + lane * 8;
+    const uint16_t* src = x + int64_t(r) * ldx + k0;
     uint4 in[kBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int64_t i = i0 + b * step;
-      in[b] = make_uint4(0, 0, 0, 0);
-      if (i < total) {
-        const int64_t r = i / pieces;
-        const int k = int(i - r * pieces) * 256 + lane * 8;
-        if (k < K) in[b] = __ldg(reinterpret_cast<const uint4*>(x + r * ldx + k));
-      }
-    }
+    for (int b = 0; b < kBatch; ++b)
+      in[b] = k0 + b * 256 < K ? __ldg(reinterpret_cast<const uint4*>(src + b * 256)) : make_uint4(0, 0, 0, 0);
+    int64_t blk;
+    int row;
+    if (!l.find(r, blk, row)) continue;
+    uint8_t* dst = q + int64_t(r) * (K / 2) + k0 / 2;
+    uint8_t* scale = sf + (blk * pieces + first) * 1024 + (lane >> 4) * 512 + (row & 31) * 16 + (row >> 5) * 4;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int64_t i = i0 + b * step;
-      if (i >= total) break;
-      const int64_t r = i / pieces;
-      const int piece = int(i - r * pieces);
-      const int k = piece * 256 + lane * 8;
+      if (first + b >= pieces) break;
       const uint32_t w[4] = {in[b].x, in[b].y, in[b].z, in[b].w};
       uint32_t top = 0;
 #pragma unroll
@@ -146,29 +156,24 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __re
       const bool finite = top < 0x7f80u;
       const int e = finite ? block_exponent(top) : 128;
       uint32_t byte = uint32_t(e + 127);
-      const float inv = finite ? __uint_as_float(uint32_t(127 - e) << 23) : 0.f;  // 2^-e, normal for e in [-127, 126]
+      const float inv = __uint_as_float(uint32_t(127 - e) << 23);  // 2^-e, normal for e in [-127, 126]
       float v[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        v[2 * j] = finite ? __uint_as_float(w[j] << 16) * inv : 0.f;
-        v[2 * j + 1] = finite ? __uint_as_float(w[j] & 0xffff0000u) * inv : 0.f;
+        v[2 * j] = __uint_as_float(w[j] << 16) * inv;
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) * inv;
       }
-      int64_t blk;
-      int row;
-      if (!l.find(r, blk, row)) continue;
-      if (k < K) *reinterpret_cast<uint32_t*>(q + r * (K / 2) + k / 2) = e2m1x8(v);
-      // four blocks' bytes -> one word of the atom
+      if (k0 + b * 256 < K) *reinterpret_cast<uint32_t*>(dst + b * 128) = finite ? e2m1x8(v) : 0u;
+      // four blocks' bytes -> one word of the atom (0 past K)
       byte |= __shfl_down_sync(0xffffffffu, byte, 4) << 8;
       byte |= __shfl_down_sync(0xffffffffu, byte, 8) << 16;
-      if ((lane & 15) == 0)
-        *reinterpret_cast<uint32_t*>(sf + ((blk * pieces + piece) * 2 + (lane >> 4)) * 512 + (row & 31) * 16 +
-                                     (row >> 5) * 4) = byte;
+      if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scale + b * 1024) = byte;
     }
   }
 }
 
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf,
-                                                              int64_t total_rows, int K, uint16_t* __restrict__ out,
+                                                              int total_rows, int K, uint16_t* __restrict__ out,
                                                               int64_t ldo, const int* offsets, int groups, int rows,
                                                               int mat_blocks, int* status) {
   extern __shared__ int sh[];
@@ -176,41 +181,32 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __r
   if (!make_layout(l, offsets, groups, rows, mat_blocks, sh, status)) return;
   const int lane = threadIdx.x & 31;
   const int pieces = (K + 255) / 256;
-  const int64_t total = total_rows * pieces;
-  const int64_t step = int64_t(gridDim.x) * kWarps;
-  for (int64_t i0 = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); i0 < total; i0 += step * kBatch) {
+  const int first = blockIdx.y * kBatch;
+  for (int r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < total_rows; r += gridDim.x * kWarps) {
+    int64_t blk;
+    int row;
+    if (!l.find(r, blk, row)) continue;
+    const int k0 = first * 256 + lane * 8;
+    const uint8_t* src = q + int64_t(r) * (K / 2) + k0 / 2;
+    const uint8_t* scale = sf + (blk * pieces + first) * 1024 + (lane >> 4) * 512 + (row & 31) * 16 + (row >> 5) * 4 +
+                           ((lane >> 2) & 3);
     uint32_t in[kBatch], byte[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int64_t i = i0 + b * step;
-      in[b] = 0;
-      byte[b] = 0;
-      if (i < total) {
-        const int64_t r = i / pieces;
-        const int piece = int(i - r * pieces);
-        const int k = piece * 256 + lane * 8;
-        int64_t blk;
-        int row;
-        if (k < K && l.find(r, blk, row)) {
-          in[b] = __ldg(reinterpret_cast<const uint32_t*>(q + r * (K / 2) + k / 2));
-          byte[b] = __ldg(sf + ((blk * pieces + piece) * 2 + (lane >> 4)) * 512 + (row & 31) * 16 + (row >> 5) * 4 +
-                          ((lane >> 2) & 3));
-        }
-      }
+      const bool on = k0 + b * 256 < K;
+      in[b] = on ? __ldg(reinterpret_cast<const uint32_t*>(src + b * 128)) : 0u;
+      byte[b] = on ? __ldg(scale + b * 1024) : 0u;
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int64_t i = i0 + b * step;
-      if (i >= total) break;
-      const int64_t r = i / pieces;
-      const int k = int(i - r * pieces) * 256 + lane * 8;
-      if (k >= K || (l.off && (r < l.off[0] || r >= l.off[groups]))) continue;
-      const float scale = __uint_as_float(byte[b] == 255u ? 0x7fffffffu : byte[b] == 0u ? 0x00400000u : byte[b] << 23);
+      if (k0 + b * 256 >= K) break;
+      const float s = __uint_as_float(byte[b] == 255u ? 0x7fffffffu : byte[b] == 0u ? 0x00400000u : byte[b] << 23);
+      float v[8];
+      e2m1x8_values(in[b], v);
       uint32_t o[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o[j] = pack_bf16x2(e2m1_value(in[b] >> (8 * j)) * scale, e2m1_value(in[b] >> (8 * j + 4)) * scale);
-      *reinterpret_cast<uint4*>(out + r * ldo + k) = make_uint4(o[0], o[1], o[2], o[3]);
+      for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(v[2 * j] * s, v[2 * j + 1] * s);
+      *reinterpret_cast<uint4*>(out + int64_t(r) * ldo + k0 + b * 256) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
 }
@@ -224,16 +220,20 @@ static int64_t blocks_of(int64_t matrices, int64_t rows, int64_t groups) {
   return matrices * ((rows + 127) / 128);
 }
 
-static unsigned grid_for(int64_t rows, int64_t K) {
-  const int64_t blocks = (rows * pairs_of(K) + kWarps * kBatch - 1) / (kWarps * kBatch);
-  const int64_t most = int64_t(tdb_host::sm_count()) * 8;
-  return unsigned(blocks < most ? (blocks > 0 ? blocks : 1) : most);
+// With offsets every block builds the groups' table first: fewer, longer blocks.
+static dim3 grid_for(int64_t rows, int64_t K, bool offsets) {
+  const int64_t y = (pairs_of(K) + kBatch - 1) / kBatch;
+  int64_t x = (rows + kWarps - 1) / kWarps;
+  const int64_t most = int64_t(tdb_host::sm_count()) * 8 / y;
+  if (offsets && x > most) x = most > 0 ? most : 1;
+  return dim3(unsigned(x), unsigned(y));
 }
 
 static int check(const char* what, int64_t matrices, int64_t rows, int64_t K, int groups, const void* offsets) {
-  if (matrices < 1 || rows < 0 || K < 32 || K % 32 || K >= (int64_t(1) << 31) || rows >= (int64_t(1) << 31) ||
+  if (matrices < 1 || rows < 0 || K < 32 || K % 32 || K >= (int64_t(1) << 26) || rows >= (int64_t(1) << 31) ||
+      matrices >= (int64_t(1) << 31) || matrices * rows >= (int64_t(1) << 31) ||
       (offsets && (groups < 1 || groups > kMaxGroups || matrices != 1)))
-    return tdb_host::fail(int(cudaErrorInvalidValue), "%s: K must be a multiple of 32; 1..%d groups of one matrix's rows",
+    return tdb_host::fail(int(cudaErrorInvalidValue), "%s: K must be a multiple of 32 below 2^26; 1..%d groups of one matrix's rows",
                           what, kMaxGroups);
   return 0;
 }
@@ -258,9 +258,9 @@ TDB_API int tdb_mx4_quantize(const void* x, int64_t ldx, int64_t matrices, int64
   if (!x || !q || !sf || ldx % 8 || ldx < K || reinterpret_cast<uintptr_t>(x) % 16 ||
       (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(sf)) % 16)
     return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 quantize: rows must be 16-byte aligned");
-  mx4::quantize_kernel<<<mx4::grid_for(matrices * rows, K), mx4::kThreads,
+  mx4::quantize_kernel<<<mx4::grid_for(matrices * rows, K, offsets != nullptr), mx4::kThreads,
                          offsets ? size_t(3 * (groups + 1)) * 4 : 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(x), ldx, matrices * rows, int(K), static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf),
+      static_cast<const uint16_t*>(x), ldx, int(matrices * rows), int(K), static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf),
       offsets, groups, int(rows), int((rows + 127) / 128), tdb_host::status_ptr());
   tdb_host::launched(1);
   return int(cudaGetLastError());
@@ -275,9 +275,9 @@ TDB_API int tdb_mx4_dequantize(const void* q, const void* sf, int64_t matrices, 
   if (!out || !q || !sf || ldo % 8 || ldo < K || reinterpret_cast<uintptr_t>(out) % 16 ||
       (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(sf)) % 16)
     return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 dequantize: rows must be 16-byte aligned");
-  mx4::dequantize_kernel<<<mx4::grid_for(matrices * rows, K), mx4::kThreads,
+  mx4::dequantize_kernel<<<mx4::grid_for(matrices * rows, K, offsets != nullptr), mx4::kThreads,
                            offsets ? size_t(3 * (groups + 1)) * 4 : 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(sf), matrices * rows, int(K), static_cast<uint16_t*>(out),
+      static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(sf), int(matrices * rows), int(K), static_cast<uint16_t*>(out),
       ldo, offsets, groups, int(rows), int((rows + 127) / 128), tdb_host::status_ptr());
   tdb_host::launched(1);
   return int(cudaGetLastError());
