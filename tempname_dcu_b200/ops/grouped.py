@@ -42,124 +42,129 @@ def _need(cond, msg):
 def _rows(t, rows, cols, device, what):
     """Row stride of a bf16 [rows, cols] matrix with contiguous rows."""
     import torch
-    if t.dtype != torch.bfloat16:
+    if t.dtype is not torch.bfloat16:
         raise TypeError(f"{what} must be bf16")
-    _need(t.dim() == 2 and tuple(t.shape) == (rows, cols) and t.stride(1) == 1 and t.device == device,
-          f"{what} must be [{rows}, {cols}] with a contiguous last dimension on the operands' device")
-    _need(rows <= 1 or t.stride(0) >= cols, f"{what}: rows must not overlap")
-    return t.stride(0) if rows > 1 else cols
+    ld, step = t.stride() if t.dim() == 2 else (0, 0)
+    if rows <= 1:
+        ld = cols
+    _need(t.shape == (rows, cols) and step == 1 and ld >= cols and t.get_device() == device,
+          f"{what} must be [{rows}, {cols}] with contiguous rows that do not overlap, on the operands' device")
+    return ld
 
 
 def _offsets(offsets, groups, device):
     import torch
-    _need(offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and
-          offsets.device == device, "offsets must be a contiguous int32 vector on the operands' device")
+    _need(offsets.dtype is torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and
+          offsets.get_device() == device, "offsets must be a contiguous int32 vector on the operands' device")
     _need(offsets.numel() == groups + 1, f"offsets must have groups + 1 = {groups + 1} entries")
     _need(1 <= groups <= MAX_GROUPS, f"the number of groups must be 1..{MAX_GROUPS}")
 
 
-def _operands(a, w, what):
+def _fp32(out, shape, device, what):
     import torch
-    _need(a.dim() == 2 and a.is_cuda, f"{what} must be a matrix on a CUDA device")
-    if w.dtype != torch.bfloat16:
+    if out.dtype is not torch.float32:
+        raise TypeError(f"{what} is fp32")
+    _need(out.shape == shape and out.is_contiguous() and out.get_device() == device,
+          f"out_f32 must be contiguous {list(shape)} on the operands' device")
+
+
+def _gemm(a, w, offsets, data_grad, mode, out, bias, aux, aux_out, tile):
+    import torch
+    _need(a.dim() == 2 and a.is_cuda, "the row operand must be a matrix on a CUDA device")
+    index = a.get_device()
+    if w.dtype is not torch.bfloat16:
         raise TypeError("w must be bf16")
-    _need(w.dim() == 3 and w.is_contiguous() and w.device == a.device,
+    _need(w.dim() == 3 and w.is_contiguous() and w.get_device() == index,
           "w must be a contiguous [groups, N, K] tensor on the operands' device")
-
-
-def _gemm(a, w, offsets, data_grad, mode, out, bias=None, aux=None, aux_out=None, tile=0):
-    import torch
-    groups = w.shape[0]
-    K, N = (w.shape[1], w.shape[2]) if data_grad else (w.shape[2], w.shape[1])
-    dev = a.device
+    groups, N, K = w.shape
+    if data_grad:
+        N, K = K, N
     rows = a.shape[0]
     _need(N > 0 and K > 0 and N % 8 == 0 and K % 8 == 0, "N and K must be positive multiples of 8")
-    lda = _rows(a, rows, K, dev, "dy" if data_grad else "x")
-    _offsets(offsets, groups, dev)
+    lda = _rows(a, rows, K, index, "dy" if data_grad else "x")
+    _offsets(offsets, groups, index)
     if bias is not None:
-        _need(bias.dtype == torch.bfloat16 and tuple(bias.shape) == (groups, N) and bias.is_contiguous() and
-              bias.device == dev, f"bias must be contiguous bf16 [{groups}, {N}] on the operands' device")
-    with native.on_device(dev):
-        out = torch.empty((rows, N), dtype=torch.bfloat16, device=dev) if out is None else out
-        ldc = _rows(out, rows, N, dev, "out")
-        pre = aux_out if aux_out is not None else aux
-        ld_aux = 0 if pre is None else _rows(pre, rows, N, dev, "the pre-activation")
-        native.check(native.lib().tdb_grouped_gemm(
-            a.data_ptr(), lda, w.data_ptr(), int(data_grad), offsets.data_ptr(), groups, out.data_ptr(), ldc, rows, N, K,
-            mode, 0 if bias is None else bias.data_ptr(), 0 if aux is None else aux.data_ptr(), ld_aux,
-            0 if aux_out is None else aux_out.data_ptr(), tile, native.stream_ptr()), "grouped gemm")
+        _need(bias.dtype is torch.bfloat16 and bias.shape == (groups, N) and bias.is_contiguous() and
+              bias.get_device() == index, f"bias must be contiguous bf16 [{groups}, {N}] on the operands' device")
+    if out is None:
+        out = torch.empty((rows, N), dtype=torch.bfloat16, device=a.device)
+    ldc = _rows(out, rows, N, index, "out")
+    pre = aux_out if aux_out is not None else aux
+    ld_aux = 0 if pre is None else _rows(pre, rows, N, index, "the pre-activation")
+    native.check(native.lib().tdb_grouped_gemm(
+        a.data_ptr(), lda, w.data_ptr(), data_grad, offsets.data_ptr(), groups, out.data_ptr(), ldc, rows, N, K, mode,
+        None if bias is None else bias.data_ptr(), None if aux is None else aux.data_ptr(), ld_aux,
+        None if aux_out is None else aux_out.data_ptr(), tile, native.current_stream(index)), "grouped gemm")
     return out
 
 
+@native.on_tensor_device
 def linear(x, w, offsets, bias=None, out=None, tile=0):
     """``x[r] @ w[g]^T (+ bias[g])`` for the rows r of group g; x [R, K],
     w [groups, N, K], bias [groups, N] -> [R, N]."""
-    _operands(x, w, "x")
-    return _gemm(x, w, offsets, False, STORE if bias is None else BIAS, out, bias=bias, tile=tile)
+    return _gemm(x, w, offsets, 0, STORE if bias is None else BIAS, out, bias, None, None, tile)
 
 
+@native.on_tensor_device
 def linear_gelu(x, w, offsets, bias=None, pre_out=None, out=None, tile=0):
     """Returns (gelu(z), z) with z = x[r] @ w[g]^T (+ bias[g]) from one kernel.
     The activation is taken of the fp32 sum; z is its bf16 rounding."""
     import torch
-    _operands(x, w, "x")
+    _need(x.dim() == 2 and w.dim() == 3, "x must be [R, K] and w [groups, N, K]")
     if pre_out is None:
         pre_out = torch.empty((x.shape[0], w.shape[1]), dtype=torch.bfloat16, device=x.device)
-    y = _gemm(x, w, offsets, False, BIAS_GELU, out, bias=bias, aux_out=pre_out, tile=tile)
-    return y, pre_out
+    if out is None:
+        out = torch.empty_like(pre_out, memory_format=torch.contiguous_format)
+    return _gemm(x, w, offsets, 0, BIAS_GELU, out, bias, None, pre_out, tile), pre_out
 
 
+@native.on_tensor_device
 def matmul_nt(dy, w, offsets, out=None, gelu_pre=None, tile=0):
     """``dy[r] @ w[g]`` (optionally times gelu'(gelu_pre)); dy [R, N],
     w [groups, N, K] -> [R, K]."""
-    _operands(dy, w, "dy")
-    return _gemm(dy, w, offsets, True, STORE if gelu_pre is None else GELU_BWD, out, aux=gelu_pre, tile=tile)
+    return _gemm(dy, w, offsets, 1, STORE if gelu_pre is None else GELU_BWD, out, None, gelu_pre, None, tile)
 
 
+@native.on_tensor_device
 def weight_grad(dy, x, offsets, out_f32=None, accumulate=True, tile=0):
     """``out_f32[g] (+)= dy_g^T @ x_g`` in fp32, [groups, N, K]; an empty group
     adds nothing (or gets zeros without ``accumulate``)."""
     import torch
     _need(dy.dim() == 2 and x.dim() == 2 and dy.is_cuda, "dy and x must be matrices on a CUDA device")
-    dev, rows = dy.device, dy.shape[0]
-    N, K = dy.shape[1], x.shape[1]
+    index = dy.get_device()
+    rows, N = dy.shape
+    K = x.shape[1]
     groups = offsets.numel() - 1
-    _offsets(offsets, groups, dev)
+    _offsets(offsets, groups, index)
     _need(N > 0 and K > 0 and N % 8 == 0 and K % 8 == 0, "N and K must be positive multiples of 8")
-    ldy = _rows(dy, rows, N, dev, "dy")
-    ldx = _rows(x, rows, K, dev, "x")
-    with native.on_device(dev):
-        if out_f32 is None:
-            out_f32 = torch.empty((groups, N, K), dtype=torch.float32, device=dev)
-            accumulate = False
-        if out_f32.dtype != torch.float32:
-            raise TypeError("the weight gradient is fp32")
-        _need(tuple(out_f32.shape) == (groups, N, K) and out_f32.is_contiguous() and out_f32.device == dev,
-              f"out_f32 must be contiguous [{groups}, {N}, {K}] on the operands' device")
-        native.check(native.lib().tdb_grouped_weight_grad(
-            dy.data_ptr(), ldy, x.data_ptr(), ldx, offsets.data_ptr(), groups, out_f32.data_ptr(), rows, N, K,
-            int(bool(accumulate)), tile, native.stream_ptr()), "grouped weight gradient")
+    ldy = _rows(dy, rows, N, index, "dy")
+    ldx = _rows(x, rows, K, index, "x")
+    if out_f32 is None:
+        out_f32 = torch.empty((groups, N, K), dtype=torch.float32, device=dy.device)
+        accumulate = False
+    _fp32(out_f32, (groups, N, K), index, "the weight gradient")
+    native.check(native.lib().tdb_grouped_weight_grad(
+        dy.data_ptr(), ldy, x.data_ptr(), ldx, offsets.data_ptr(), groups, out_f32.data_ptr(), rows, N, K,
+        bool(accumulate), tile, native.current_stream(index)), "grouped weight gradient")
     return out_f32
 
 
+@native.on_tensor_device
 def bias_grad(dy, offsets, out_f32=None, accumulate=True):
     """``out_f32[g] (+)= `` the sum of dy's rows of group g, fp32 [groups, N]."""
     import torch
     _need(dy.dim() == 2 and dy.is_cuda, "dy must be a matrix on a CUDA device")
-    dev, (rows, N) = dy.device, dy.shape
+    index = dy.get_device()
+    rows, N = dy.shape
     groups = offsets.numel() - 1
-    _offsets(offsets, groups, dev)
+    _offsets(offsets, groups, index)
     _need(N > 0 and N % 8 == 0, "N must be a positive multiple of 8")
-    ldy = _rows(dy, rows, N, dev, "dy")
-    with native.on_device(dev):
-        if out_f32 is None:
-            out_f32 = torch.empty((groups, N), dtype=torch.float32, device=dev)
-            accumulate = False
-        if out_f32.dtype != torch.float32:
-            raise TypeError("the bias gradient is fp32")
-        _need(tuple(out_f32.shape) == (groups, N) and out_f32.is_contiguous() and out_f32.device == dev,
-              f"out_f32 must be contiguous [{groups}, {N}] on the operands' device")
-        native.check(native.lib().tdb_grouped_bias_grad(dy.data_ptr(), ldy, offsets.data_ptr(), groups,
-                                                        out_f32.data_ptr(), rows, N, int(bool(accumulate)),
-                                                        native.stream_ptr()), "grouped bias gradient")
+    ldy = _rows(dy, rows, N, index, "dy")
+    if out_f32 is None:
+        out_f32 = torch.empty((groups, N), dtype=torch.float32, device=dy.device)
+        accumulate = False
+    _fp32(out_f32, (groups, N), index, "the bias gradient")
+    native.check(native.lib().tdb_grouped_bias_grad(dy.data_ptr(), ldy, offsets.data_ptr(), groups, out_f32.data_ptr(),
+                                                    rows, N, bool(accumulate), native.current_stream(index)),
+                 "grouped bias gradient")
     return out_f32

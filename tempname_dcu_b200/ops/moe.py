@@ -79,35 +79,54 @@ def _need(cond, msg):
 
 
 def _check_routing(r, device):
+    """(tokens, k) of a routing whose tensors are fit for the kernels."""
     import torch
-    _need(r.ids.dim() == 2 and r.ids.dtype == torch.int32 and r.ids.is_contiguous() and r.ids.device == device,
+    ids, weights, slots = r.ids, r.weights, r.slots
+    _need(ids.dim() == 2 and ids.dtype is torch.int32 and ids.is_contiguous() and ids.get_device() == device,
           "routing ids must be contiguous int32 [tokens, k] on the tensors' device")
-    _need(r.weights.shape == r.ids.shape and r.weights.dtype == torch.float32 and r.weights.is_contiguous() and
-          r.weights.device == device, "routing weights must be contiguous fp32 [tokens, k] on the tensors' device")
-    _need(r.slots.numel() == r.ids.numel() and r.slots.dtype == torch.int32 and r.slots.is_contiguous() and
-          r.slots.device == device, "routing slots must be contiguous int32 [tokens * k] on the tensors' device")
+    _need(weights.shape == ids.shape and weights.dtype is torch.float32 and weights.is_contiguous() and
+          weights.get_device() == device, "routing weights must be contiguous fp32 [tokens, k] on the tensors' device")
+    _need(slots.numel() == ids.numel() and slots.dtype is torch.int32 and slots.is_contiguous() and
+          slots.get_device() == device, "routing slots must be contiguous int32 [tokens * k] on the tensors' device")
+    return ids.shape
 
 
 def _rows(t, rows, cols, device, what):
+    """Row stride of a bf16 [rows, cols] matrix with contiguous rows."""
     import torch
-    _need(t.dim() == 2 and t.dtype == torch.bfloat16 and tuple(t.shape) == (rows, cols) and
-          (t.stride(1) == 1 or cols == 1) and t.device == device,
-          f"{what} must be bf16 [{rows}, {cols}] with a contiguous last dimension on the tensors' device")
-    _need(rows <= 1 or t.stride(0) >= cols, f"{what}: rows must not overlap")
-    return t.stride(0) if rows > 1 else cols
+    ld, step = t.stride() if t.dim() == 2 else (0, 0)
+    if rows <= 1:
+        ld = cols
+    _need(t.dtype is torch.bfloat16 and t.shape == (rows, cols) and step == 1 and ld >= cols and
+          t.get_device() == device,
+          f"{what} must be bf16 [{rows}, {cols}] with contiguous rows that do not overlap, on the tensors' device")
+    return ld
 
 
-def _logits(logits):
+def _columns(t, what):
+    """(rows, columns, device) of a row operand."""
+    _need(t.dim() == 2 and t.is_cuda, f"{what} must be a matrix on a CUDA device")
+    rows, cols = t.shape
+    _need(cols > 0 and cols % 8 == 0, f"{what} needs a multiple of 8 columns")
+    return rows, cols, t.get_device()
+
+
+def _logits(logits, what="logits"):
+    """(tokens, experts, row stride, is bf16, device)."""
     import torch
-    _need(logits.dim() == 2 and logits.is_cuda and logits.dtype in (torch.float32, torch.bfloat16),
-          "logits must be an fp32 or bf16 [tokens, experts] matrix on a CUDA device")
+    _need(logits.dim() == 2 and logits.is_cuda, f"{what} must be a [tokens, experts] matrix on a CUDA device")
+    bf16 = logits.dtype is torch.bfloat16
+    _need(bf16 or logits.dtype is torch.float32, f"{what} must be fp32 or bf16")
     tokens, experts = logits.shape
     _need(1 <= experts <= MAX_EXPERTS, f"the number of experts must be 1..{MAX_EXPERTS}")
-    _need(logits.stride(1) == 1 or experts == 1, "logits need a contiguous last dimension")
-    _need(tokens <= 1 or logits.stride(0) >= experts, "logits: rows must not overlap")
-    return tokens, experts, logits.stride(0) if tokens > 1 else experts
+    ld, step = logits.stride()
+    if tokens <= 1:
+        ld = experts
+    _need((step == 1 or experts == 1) and ld >= experts, f"{what} needs contiguous rows that do not overlap")
+    return tokens, experts, ld, int(bf16), logits.get_device()
 
 
+@native.on_tensor_device
 def route(logits, top_k, normalize=True):
     """Top-k experts of each token -> ``Routing``.
 
@@ -115,121 +134,112 @@ def route(logits, top_k, normalize=True):
     index first; NaN counts as the largest) with softmax weights over the
     chosen ones (``normalize``) or over all experts."""
     import torch
-    tokens, experts, ld = _logits(logits)
+    tokens, experts, ld, bf16, index = _logits(logits)
     _need(type(top_k) is int and 1 <= top_k <= min(experts, MAX_TOP_K),
           f"top_k must be 1..{MAX_TOP_K} and at most the number of experts")
+    normalize = bool(normalize)
     dev = logits.device
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
+    ids = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
+    order = torch.empty(tokens * top_k, dtype=torch.int32, device=dev)
+    slots = torch.empty_like(order)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
     lib = native.lib()
-    with native.on_device(dev):
-        ids = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
-        weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
-        offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
-        order = torch.empty(tokens * top_k, dtype=torch.int32, device=dev)
-        slots = torch.empty(tokens * top_k, dtype=torch.int32, device=dev)
-        ints = int(lib.tdb_moe_route_scratch_ints(tokens, experts))
-        scratch = torch.empty(ints, dtype=torch.int32, device=dev) if ints else None
-        native.check(lib.tdb_moe_route(logits.data_ptr(), int(logits.dtype == torch.bfloat16), ld, tokens, experts,
-                                       top_k, int(bool(normalize)), ids.data_ptr(), weights.data_ptr(),
-                                       offsets.data_ptr(), order.data_ptr(), slots.data_ptr(),
-                                       0 if scratch is None else scratch.data_ptr(), native.stream_ptr()),
-                     "moe route")
-    return Routing(ids=ids, weights=weights, offsets=offsets, order=order, slots=slots, normalize=bool(normalize))
+    ints = lib.tdb_moe_route_scratch_ints(tokens, experts)
+    scratch = torch.empty(ints, dtype=torch.int32, device=dev) if ints else None
+    native.check(lib.tdb_moe_route(logits.data_ptr(), bf16, ld, tokens, experts, top_k, normalize, ids.data_ptr(),
+                                   weights.data_ptr(), offsets.data_ptr(), order.data_ptr(), slots.data_ptr(),
+                                   None if scratch is None else scratch.data_ptr(), native.current_stream(index)),
+                 "moe route")
+    return Routing(ids, weights, offsets, order, slots, normalize)
 
 
+@native.on_tensor_device
 def route_bwd(logits, routing, dweights, out=None):
     """Gradient of ``route``'s weights with respect to the logits.  ``out``
     (fp32 or bf16 [tokens, experts], default: the logits' type) is written
     whole: 0 for experts that were not chosen when the weights are
     normalised."""
     import torch
-    tokens, experts, ld = _logits(logits)
-    dev = logits.device
-    _check_routing(routing, dev)
-    top_k = routing.top_k
-    _need(routing.tokens == tokens and routing.experts == experts, "routing and logits have different sizes")
-    _need(dweights.shape == routing.ids.shape and dweights.dtype == torch.float32 and dweights.is_contiguous() and
-          dweights.device == dev, "dweights must be contiguous fp32 [tokens, k] on the logits' device")
-    with native.on_device(dev):
-        out = torch.empty((tokens, experts), dtype=logits.dtype, device=dev) if out is None else out
-        _need(out.dtype in (torch.float32, torch.bfloat16) and tuple(out.shape) == (tokens, experts) and
-              (out.stride(1) == 1 or experts == 1) and (tokens <= 1 or out.stride(0) >= experts) and
-              out.device == dev, "out must be fp32 or bf16 [tokens, experts] with a contiguous last dimension")
-        native.check(native.lib().tdb_moe_route_bwd(logits.data_ptr(), int(logits.dtype == torch.bfloat16), ld, tokens,
-                                                    experts, top_k, int(routing.normalize), routing.ids.data_ptr(),
-                                                    routing.weights.data_ptr(), dweights.data_ptr(), out.data_ptr(),
-                                                    int(out.dtype == torch.bfloat16),
-                                                    out.stride(0) if tokens > 1 else experts,
-                                                    native.stream_ptr()), "moe route backward")
+    tokens, experts, ld, bf16, index = _logits(logits)
+    shape = _check_routing(routing, index)
+    _need(shape[0] == tokens and routing.experts == experts, "routing and logits have different sizes")
+    _need(dweights.shape == shape and dweights.dtype is torch.float32 and dweights.is_contiguous() and
+          dweights.get_device() == index, "dweights must be contiguous fp32 [tokens, k] on the logits' device")
+    if out is None:
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    _need(out.shape == (tokens, experts), "out must be [tokens, experts]")
+    _, _, ld_out, out_bf16, out_index = _logits(out, "out")
+    _need(out_index == index, "out must be on the logits' device")
+    native.check(native.lib().tdb_moe_route_bwd(logits.data_ptr(), bf16, ld, tokens, experts, shape[1],
+                                                bool(routing.normalize), routing.ids.data_ptr(),
+                                                routing.weights.data_ptr(), dweights.data_ptr(), out.data_ptr(),
+                                                out_bf16, ld_out, native.current_stream(index)), "moe route backward")
     return out
 
 
+@native.on_tensor_device
 def dispatch(x, routing, out=None):
     """Rows grouped by expert: ``out[slots[t*k + j]] = x[t]``, [tokens*k, H]."""
     import torch
-    _need(x.dim() == 2 and x.is_cuda and x.shape[1] % 8 == 0 and x.shape[1] > 0,
-          "x must be [tokens, H] on a CUDA device with H a multiple of 8")
-    tokens, H = x.shape
-    dev = x.device
-    _check_routing(routing, dev)
-    k = routing.top_k
-    _need(routing.tokens == tokens, "routing and x have different numbers of tokens")
-    ldx = _rows(x, tokens, H, dev, "x")
-    with native.on_device(dev):
-        out = torch.empty((tokens * k, H), dtype=torch.bfloat16, device=dev) if out is None else out
-        ldo = _rows(out, tokens * k, H, dev, "out")
-        native.check(native.lib().tdb_moe_dispatch(x.data_ptr(), ldx, tokens, k, H, routing.slots.data_ptr(),
-                                                   out.data_ptr(), ldo, native.stream_ptr()), "moe dispatch")
+    tokens, H, index = _columns(x, "x")
+    shape = _check_routing(routing, index)
+    _need(shape[0] == tokens, "routing and x have different numbers of tokens")
+    k = shape[1]
+    ldx = _rows(x, tokens, H, index, "x")
+    if out is None:
+        out = torch.empty((tokens * k, H), dtype=torch.bfloat16, device=x.device)
+    ldo = _rows(out, tokens * k, H, index, "out")
+    native.check(native.lib().tdb_moe_dispatch(x.data_ptr(), ldx, tokens, k, H, routing.slots.data_ptr(),
+                                               out.data_ptr(), ldo, native.current_stream(index)), "moe dispatch")
     return out
 
 
 def _combine(y, routing, weighted, residual, out, what):
     import torch
-    _need(y.dim() == 2 and y.is_cuda and y.shape[1] % 8 == 0 and y.shape[1] > 0,
-          "the grouped rows must be [tokens*k, H] on a CUDA device with H a multiple of 8")
-    dev = y.device
-    _check_routing(routing, dev)
-    tokens, k, H = routing.tokens, routing.top_k, y.shape[1]
-    ldy = _rows(y, tokens * k, H, dev, "the grouped rows")
-    ldr = 0 if residual is None else _rows(residual, tokens, H, dev, "residual")
-    with native.on_device(dev):
-        out = torch.empty((tokens, H), dtype=torch.bfloat16, device=dev) if out is None else out
-        ldo = _rows(out, tokens, H, dev, "out")
-        native.check(native.lib().tdb_moe_combine(y.data_ptr(), ldy, tokens, k, H, routing.slots.data_ptr(),
-                                                  routing.weights.data_ptr() if weighted else 0,
-                                                  0 if residual is None else residual.data_ptr(), ldr, out.data_ptr(),
-                                                  ldo, native.stream_ptr()), what)
+    rows, H, index = _columns(y, "the grouped rows")
+    tokens, k = _check_routing(routing, index)
+    ldy = _rows(y, tokens * k, H, index, "the grouped rows")
+    ldr = 0 if residual is None else _rows(residual, tokens, H, index, "residual")
+    if out is None:
+        out = torch.empty((tokens, H), dtype=torch.bfloat16, device=y.device)
+    ldo = _rows(out, tokens, H, index, "out")
+    native.check(native.lib().tdb_moe_combine(y.data_ptr(), ldy, tokens, k, H, routing.slots.data_ptr(),
+                                              routing.weights.data_ptr() if weighted else None,
+                                              None if residual is None else residual.data_ptr(), ldr, out.data_ptr(),
+                                              ldo, native.current_stream(index)), what)
     return out
 
 
+@native.on_tensor_device
 def dispatch_bwd(dxs, routing, residual=None, out=None):
     """Gradient of ``dispatch``: ``out[t] = (residual[t] +) sum_j dxs[slots[t*k + j]]``."""
     return _combine(dxs, routing, False, residual, out, "moe dispatch backward")
 
 
+@native.on_tensor_device
 def combine(ys, routing, residual=None, out=None):
     """``out[t] = (residual[t] +) sum_j weights[t, j] * ys[slots[t*k + j]]``, [tokens, H]."""
     return _combine(ys, routing, True, residual, out, "moe combine")
 
 
+@native.on_tensor_device
 def combine_bwd(dout, ys, routing, out=None):
     """Gradients of ``combine``: (dys [tokens*k, H] bf16, dweights [tokens, k]
     fp32).  The residual's gradient is ``dout`` itself."""
     import torch
-    _need(dout.dim() == 2 and dout.is_cuda and dout.shape[1] % 8 == 0 and dout.shape[1] > 0,
-          "dout must be [tokens, H] on a CUDA device with H a multiple of 8")
-    tokens, H = dout.shape
-    dev = dout.device
-    _check_routing(routing, dev)
-    k = routing.top_k
-    _need(routing.tokens == tokens, "routing and dout have different numbers of tokens")
-    ldd = _rows(dout, tokens, H, dev, "dout")
-    ldy = _rows(ys, tokens * k, H, dev, "ys")
-    with native.on_device(dev):
-        out = torch.empty((tokens * k, H), dtype=torch.bfloat16, device=dev) if out is None else out
-        ldo = _rows(out, tokens * k, H, dev, "out")
-        dweights = torch.empty((tokens, k), dtype=torch.float32, device=dev)
-        native.check(native.lib().tdb_moe_combine_bwd(dout.data_ptr(), ldd, ys.data_ptr(), ldy, tokens, k, H,
-                                                      routing.slots.data_ptr(), routing.weights.data_ptr(),
-                                                      out.data_ptr(), ldo, dweights.data_ptr(), native.stream_ptr()),
-                     "moe combine backward")
+    tokens, H, index = _columns(dout, "dout")
+    shape = _check_routing(routing, index)
+    _need(shape[0] == tokens, "routing and dout have different numbers of tokens")
+    k = shape[1]
+    ldd = _rows(dout, tokens, H, index, "dout")
+    ldy = _rows(ys, tokens * k, H, index, "ys")
+    if out is None:
+        out = torch.empty((tokens * k, H), dtype=torch.bfloat16, device=dout.device)
+    ldo = _rows(out, tokens * k, H, index, "out")
+    dweights = torch.empty_like(routing.weights)
+    native.check(native.lib().tdb_moe_combine_bwd(dout.data_ptr(), ldd, ys.data_ptr(), ldy, tokens, k, H,
+                                                  routing.slots.data_ptr(), routing.weights.data_ptr(),
+                                                  out.data_ptr(), ldo, dweights.data_ptr(),
+                                                  native.current_stream(index)), "moe combine backward")
     return out, dweights

@@ -44,8 +44,8 @@ def _groups(offsets, device):
     import torch
     if offsets is None:
         return 0
-    _need(offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and
-          offsets.device == device, "offsets must be a contiguous int32 vector on the operands' device")
+    _need(offsets.dtype is torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and
+          offsets.get_device() == device, "offsets must be a contiguous int32 vector on the operands' device")
     groups = offsets.numel() - 1
     _need(1 <= groups <= MAX_GROUPS, f"the number of groups must be 1..{MAX_GROUPS}")
     return groups
@@ -54,105 +54,114 @@ def _groups(offsets, device):
 def scale_bytes(rows: int, k: int, groups: int = 0, matrices: int = 1) -> int:
     """Bytes of the scales of ``matrices`` [rows, k] operands, or of one whose
     rows lie in ``groups`` groups."""
-    return int(native.lib().tdb_mx4_scale_bytes(matrices, rows, k, groups))
+    return native.lib().tdb_mx4_scale_bytes(matrices, rows, k, groups)
 
 
 def _operand(q, sf, groups, device, what):
     """(matrices, rows, K) of a quantized operand."""
     import torch
-    _need(q.dtype == torch.uint8 and q.dim() in (2, 3) and q.is_contiguous() and q.device == device and
-          q.shape[-1] % 16 == 0 and q.shape[-1] > 0,
+    _need(q.dtype is torch.uint8 and q.dim() in (2, 3) and q.is_contiguous() and q.get_device() == device,
           f"{what} must be contiguous uint8 [..., K/2] as written by quantize, on the operands' device")
-    matrices = q.shape[0] if q.dim() == 3 else 1
-    rows, K = q.shape[-2], 2 * q.shape[-1]
-    _need(sf.dtype == torch.uint8 and sf.is_contiguous() and sf.device == device and
+    shape = q.shape
+    matrices = shape[0] if len(shape) == 3 else 1
+    rows, K = shape[-2], 2 * shape[-1]
+    _need(K > 0 and K % 32 == 0, f"{what}: K must be a positive multiple of 32")
+    _need(sf.dtype is torch.uint8 and sf.is_contiguous() and sf.get_device() == device and
           sf.numel() >= scale_bytes(rows, K, groups, matrices),
           f"the scales of {what} must be the uint8 buffer that quantize wrote for these rows (and offsets)")
     return matrices, rows, K
 
 
+@native.on_tensor_device
 def quantize(x, offsets=None, q=None, sf=None):
     """bf16 ``x`` [rows, K] or [matrices, rows, K] -> (q uint8 [..., K/2], sf
     uint8).  With ``offsets``, rows outside every group are not written."""
     import torch
-    if x.dtype != torch.bfloat16:
+    if x.dtype is not torch.bfloat16:
         raise TypeError("quantize expects bf16")
-    _need(x.is_cuda and x.dim() in (2, 3) and x.stride(-1) == 1, "x must be [rows, K] or [matrices, rows, K] on a CUDA "
-          "device with a contiguous last dimension")
-    rows, K = x.shape[-2:]
-    _need(K > 0 and K % 32 == 0, "K must be a positive multiple of 32")
-    dev = x.device
-    groups = _groups(offsets, dev)
-    matrices, ld = 1, x.stride(-2) if rows > 1 else K
-    if x.dim() == 3:
-        _need(x.is_contiguous() and offsets is None and x.shape[0] > 0,
+    dims = x.dim()
+    _need(x.is_cuda and dims in (2, 3), "x must be [rows, K] or [matrices, rows, K] on a CUDA device")
+    shape, stride = x.shape, x.stride()
+    rows, K = shape[-2:]
+    _need(K > 0 and K % 32 == 0 and stride[-1] == 1, "K must be a positive multiple of 32, the last dimension contiguous")
+    index = x.get_device()
+    groups = _groups(offsets, index)
+    matrices, ld = 1, stride[0] if rows > 1 else K
+    if dims == 3:
+        _need(x.is_contiguous() and offsets is None and shape[0] > 0,
               "a [matrices, rows, K] operand must be contiguous and takes no offsets")
-        matrices, ld = x.shape[0], K
+        matrices, ld = shape[0], K
     _need(ld >= K, "x: rows must not overlap")
     lib = native.lib()
-    with native.on_device(dev):
-        need = int(lib.tdb_mx4_scale_bytes(matrices, rows, K, groups))
-        if q is None:
-            q = torch.empty(x.shape[:-1] + (K // 2,), dtype=torch.uint8, device=dev)
-        if sf is None:
-            sf = torch.empty(need, dtype=torch.uint8, device=dev)
-        _need(q.dtype == torch.uint8 and q.shape == x.shape[:-1] + (K // 2,) and q.is_contiguous() and q.device == dev,
+    need = lib.tdb_mx4_scale_bytes(matrices, rows, K, groups)
+    packed = shape[:-1] + (K // 2,)
+    if q is None:
+        q = torch.empty(packed, dtype=torch.uint8, device=x.device)
+    else:
+        _need(q.dtype is torch.uint8 and q.shape == packed and q.is_contiguous() and q.get_device() == index,
               "q must be contiguous uint8 [..., K/2] on x's device")
-        _need(sf.dtype == torch.uint8 and sf.numel() >= need and sf.is_contiguous() and sf.device == dev,
+    if sf is None:
+        sf = torch.empty(need, dtype=torch.uint8, device=x.device)
+    else:
+        _need(sf.dtype is torch.uint8 and sf.numel() >= need and sf.is_contiguous() and sf.get_device() == index,
               f"sf must be a contiguous uint8 buffer of at least {need} bytes on x's device")
-        native.check(lib.tdb_mx4_quantize(x.data_ptr(), ld, matrices, rows, K,
-                                          0 if offsets is None else offsets.data_ptr(), groups, q.data_ptr(),
-                                          sf.data_ptr(), native.stream_ptr()), "mx4 quantize")
+    native.check(lib.tdb_mx4_quantize(x.data_ptr(), ld, matrices, rows, K, None if offsets is None else offsets.data_ptr(),
+                                      groups, q.data_ptr(), sf.data_ptr(), native.current_stream(index)), "mx4 quantize")
     return q, sf
 
 
+@native.on_tensor_device
 def dequantize(q, sf, offsets=None, out=None):
     """The bf16 values of an operand produced by ``quantize`` with the same
     ``offsets``: exact, but for a value of 2^128, which reads as an infinity."""
     import torch
     _need(q.is_cuda, "q must be on a CUDA device")
-    dev = q.device
-    groups = _groups(offsets, dev)
-    matrices, rows, K = _operand(q, sf, groups, dev, "q")
+    index = q.get_device()
+    groups = _groups(offsets, index)
+    matrices, rows, K = _operand(q, sf, groups, index, "q")
     _need(offsets is None or q.dim() == 2, "a [matrices, rows, K] operand takes no offsets")
     shape = q.shape[:-1] + (K,)
-    with native.on_device(dev):
-        out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if out is None else out
-        _need(out.dtype == torch.bfloat16 and out.shape == shape and out.device == dev and out.stride(-1) == 1 and
-              (out.is_contiguous() or (out.dim() == 2 and out.stride(0) >= K)),
-              "out must be bf16 [..., K] with a contiguous last dimension on q's device")
-        ld = out.stride(0) if out.dim() == 2 and rows > 1 else K
-        native.check(native.lib().tdb_mx4_dequantize(q.data_ptr(), sf.data_ptr(), matrices, rows, K,
-                                                     0 if offsets is None else offsets.data_ptr(), groups,
-                                                     out.data_ptr(), ld, native.stream_ptr()), "mx4 dequantize")
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+    _need(out.dtype is torch.bfloat16 and out.shape == shape and out.get_device() == index and out.stride(-1) == 1 and
+          (out.is_contiguous() or (out.dim() == 2 and out.stride(0) >= K)),
+          "out must be bf16 [..., K] with contiguous rows that do not overlap, on q's device")
+    ld = out.stride(0) if out.dim() == 2 and rows > 1 else K
+    native.check(native.lib().tdb_mx4_dequantize(q.data_ptr(), sf.data_ptr(), matrices, rows, K,
+                                                 None if offsets is None else offsets.data_ptr(), groups,
+                                                 out.data_ptr(), ld, native.current_stream(index)), "mx4 dequantize")
     return out
 
 
 def _product(qx, sfx, qw, sfw, offsets, bias, out, tile):
     import torch
     _need(qx.is_cuda and qx.dim() == 2, "qx must be a quantized [rows, K] operand on a CUDA device")
-    dev = qx.device
-    groups = _groups(offsets, dev)
-    _, rows, K = _operand(qx, sfx, groups, dev, "qx")
-    matrices, N, Kw = _operand(qw, sfw, 0, dev, "qw")
+    index = qx.get_device()
+    groups = _groups(offsets, index)
+    _, rows, K = _operand(qx, sfx, groups, index, "qx")
+    matrices, N, Kw = _operand(qw, sfw, 0, index, "qw")
     _need(K == Kw, f"the K extents differ: {K} and {Kw}")
     _need(matrices == max(groups, 1), "qw must hold one matrix per group")
     _need(N > 0 and N % 8 == 0, "N must be a positive multiple of 8")
     if bias is not None:
-        _need(bias.dtype == torch.bfloat16 and bias.numel() == matrices * N and bias.is_contiguous() and
-              bias.device == dev and bias.shape[-1] == N, "bias must be contiguous bf16 [N] or [groups, N]")
-    with native.on_device(dev):
-        out = torch.empty((rows, N), dtype=torch.bfloat16, device=dev) if out is None else out
-        _need(out.dtype == torch.bfloat16 and tuple(out.shape) == (rows, N) and out.stride(1) == 1 and
-              (rows <= 1 or out.stride(0) >= N) and out.device == dev,
-              f"out must be bf16 [{rows}, {N}] with a contiguous last dimension on the operands' device")
-        native.check(native.lib().tdb_mx4_gemm(
-            qx.data_ptr(), sfx.data_ptr(), qw.data_ptr(), sfw.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
-            matrices, out.data_ptr(), out.stride(0) if rows > 1 else N, rows, N, K,
-            0 if bias is None else bias.data_ptr(), tile, native.stream_ptr()), "mx4 product")
+        _need(bias.dtype is torch.bfloat16 and bias.numel() == matrices * N and bias.shape[-1] == N and
+              bias.is_contiguous() and bias.get_device() == index, "bias must be contiguous bf16 [N] or [groups, N]")
+    if out is None:
+        out = torch.empty((rows, N), dtype=torch.bfloat16, device=qx.device)
+    ld, step = out.stride() if out.dim() == 2 else (0, 0)
+    if rows <= 1:
+        ld = N
+    _need(out.dtype is torch.bfloat16 and out.shape == (rows, N) and step == 1 and ld >= N and
+          out.get_device() == index,
+          f"out must be bf16 [{rows}, {N}] with contiguous rows that do not overlap, on the operands' device")
+    native.check(native.lib().tdb_mx4_gemm(
+        qx.data_ptr(), sfx.data_ptr(), qw.data_ptr(), sfw.data_ptr(), None if offsets is None else offsets.data_ptr(),
+        matrices, out.data_ptr(), ld, rows, N, K, None if bias is None else bias.data_ptr(), tile,
+        native.current_stream(index)), "mx4 product")
     return out
 
 
+@native.on_tensor_device
 def linear(qx, sfx, qw, sfw, bias=None, out=None, tile=0):
     """``values(qx) @ values(qw)^T (+ bias)`` in bf16 with fp32 accumulation;
     qx [M, K], qw [N, K] from ``quantize``."""
@@ -160,6 +169,7 @@ def linear(qx, sfx, qw, sfw, bias=None, out=None, tile=0):
     return _product(qx, sfx, qw, sfw, None, bias, out, tile)
 
 
+@native.on_tensor_device
 def grouped_linear(qx, sfx, qw, sfw, offsets, bias=None, out=None, tile=0):
     """``values(qx)[r] @ values(qw)[g]^T (+ bias[g])`` for the rows r of group
     g; qx [R, K] quantized with these ``offsets``, qw [groups, N, K], bias

@@ -12,6 +12,7 @@ tensor contract checks, error text from the library).
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 
 from . import _build
@@ -102,26 +103,27 @@ def stream_ptr(stream=None) -> int:
     return int(stream.cuda_stream)
 
 
-class on_device:
-    """``with on_device(t.device):`` -- the calls inside launch on ``t``'s device
-    and its current stream.  Free of CUDA calls when that is the current device."""
+def current_stream(device_index: int) -> int:
+    """The current stream of a device as the integer that the entry points
+    take.  (``stream_ptr`` builds a Stream object first, which costs as much as
+    a small launch.)"""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
-    def __init__(self, device):
-        self.device = device
-        self.guard = None
 
-    def __enter__(self):
+def on_tensor_device(fn):
+    """Run ``fn(tensor, ...)`` with the tensor's CUDA device current, so that its
+    allocations and launches go there.  A tensor that is not on a CUDA device
+    is left to the function's own checks."""
+    @functools.wraps(fn)
+    def call(tensor, *args, **kwargs):
         import torch
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return self
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-            self.guard = None
-        return False
+        index = tensor.get_device() if isinstance(tensor, torch.Tensor) else -1
+        if index < 0 or index == torch.cuda.current_device():
+            return fn(tensor, *args, **kwargs)
+        with torch.cuda.device(index):
+            return fn(tensor, *args, **kwargs)
+    return call
 
 
 def read_status() -> list[int]:
