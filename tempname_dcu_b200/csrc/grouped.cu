@@ -117,7 +117,7 @@ TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data
   if (tile == 0) tile = tdb::grouped::pick_tile(data_grad ? kDataGrad : kForward, rows, groups, 0, N);
   if (tile != 32 && tile != 128 && tile != 512) return bad("grouped: tile must be 0, 32, 128 or 512");
   RowsParams p = {};
-  const uint32_t box_rows = tile == 32 ? 32 : 64;
+  const uint32_t box_rows = tile == 512 ? 64 : 32;
   int rc = tdb_host::make_tmap_2d(&p.tmB, A, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(K), uint64_t(rows),
                                   uint64_t(lda), gemm::BK, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;

@@ -54,59 +54,69 @@ __device__ __forceinline__ float load_logit<float>(const float* p) { return __ld
 template <>
 __device__ __forceinline__ float load_logit<uint16_t>(const uint16_t* p) { return bf16_bits_to_float(__ldg(p)); }
 
-// One warp: the top k of one token.  Lane j < k returns the j-th choice's id
-// and weight.  NP = experts per lane (expert i*32 + lane).
-template <int NP, typename T>
-__device__ __forceinline__ void choose(const T* row, int E, int k, int normalize, int& my_id, float& my_w) {
+// One warp: the top k of TT tokens at once (the rounds of one token depend on
+// each other, those of several overlap).  Lane j < k returns the j-th choice's
+// id and weight.  NP = experts per lane (expert i*32 + lane); rows past the
+// last token repeat it.
+template <int NP, int TT, typename T>
+__device__ __forceinline__ void choose(const T* logits, int64_t ld, int t0, int t_step, int tokens, int E, int k,
+                                       int normalize, int (&my_id)[TT], float (&my_w)[TT]) {
   const int lane = threadIdx.x & 31;
-  float v[NP];
-  uint32_t key[NP];
+  float v[TT][NP];
+  uint32_t key[TT][NP];
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int e = i * 32 + lane;
-    v[i] = e < E ? load_logit<T>(row + e) : -INFINITY;
-    key[i] = e < E ? order_key(v[i]) : 0u;
+  for (int q = 0; q < TT; ++q) {
+    const T* row = logits + int64_t(min(t0 + q * t_step, tokens - 1)) * ld;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int e = i * 32 + lane;
+      v[q][i] = e < E ? load_logit<T>(row + e) : -INFINITY;
+    }
   }
-  float my_z = -INFINITY, top = -INFINITY;
-  my_id = 0;
+#pragma unroll
+  for (int q = 0; q < TT; ++q)
+#pragma unroll
+    for (int i = 0; i < NP; ++i) key[q][i] = i * 32 + lane < E ? order_key(v[q][i]) : 0u;
+  float my_z[TT], top[TT];
   for (int j = 0; j < k; ++j) {
-    uint32_t best = key[0];
-    int at = 0;
 #pragma unroll
-    for (int i = 1; i < NP; ++i)
-      if (key[i] > best) {
-        best = key[i];
-        at = i;
+    for (int q = 0; q < TT; ++q) {
+      uint32_t best = key[q][0];
+      int at = 0;
+#pragma unroll
+      for (int i = 1; i < NP; ++i)
+        if (key[q][i] > best) {
+          best = key[q][i];
+          at = i;
+        }
+      const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+      const uint32_t id = __reduce_min_sync(0xffffffffu, best == m ? uint32_t(at * 32 + lane) : 0x7fffffffu);
+      if ((id & 31u) == uint32_t(lane)) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          if (uint32_t(i) == id >> 5) key[q][i] = 0u;
       }
-    const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-    const uint32_t id = __reduce_min_sync(0xffffffffu, best == m ? uint32_t(at * 32 + lane) : 0x7fffffffu);
-    if ((id & 31u) == uint32_t(lane)) {
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        if (uint32_t(i) == id >> 5) key[i] = 0u;
-    }
-    const float z = key_value(m);
-    if (j == 0) top = z;
-    if (lane == j) {
-      my_id = int(id);
-      my_z = z;
+      const float z = key_value(m);
+      if (j == 0) top[q] = z;
+      if (j == 0 || lane == j) {
+        my_id[q] = int(id);
+        my_z[q] = z;
+      }
     }
   }
-  if (top == -INFINITY) {  // no expert is open to this token
-    my_w = 0.f;
-    return;
-  }
-  const float e = lane < k ? expf(my_z - top) : 0.f;
-  float s;
-  if (normalize) {
-    s = warp_sum(e);
-  } else {
-    float part = 0.f;
 #pragma unroll
-    for (int i = 0; i < NP; ++i) part += i * 32 + lane < E ? expf(v[i] - top) : 0.f;
-    s = warp_sum(part);
+  for (int q = 0; q < TT; ++q) {
+    const bool open = top[q] != -INFINITY;  // else no expert is open to this token
+    const float e = open && lane < k ? expf(my_z[q] - top[q]) : 0.f;
+    float part = e;
+    if (!normalize) {
+      part = 0.f;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) part += i * 32 + lane < E ? expf(v[q][i] - top[q]) : 0.f;
+    }
+    const float s = warp_sum(part);
+    my_w[q] = open ? e / s : 0.f;
   }
-  my_w = e / s;
 }
 
 // Exclusive scan of total[0..E) into start[0..E], by one warp.
@@ -189,14 +199,20 @@ __global__ void __launch_bounds__(kRouteThreads) choose_kernel(const T* __restri
   for (int e = threadIdx.x; e < E; e += kRouteThreads) count[e] = 0;
   __syncthreads();
   const int t0 = blockIdx.x * kTokensPerBlock, t1 = min(t0 + kTokensPerBlock, tokens);
-  for (int t = t0 + warp; t < t1; t += kRouteThreads / 32) {
-    int id;
-    float w;
-    choose<NP, T>(logits + int64_t(t) * ld, E, k, normalize, id, w);
-    if (lane < k) {
-      ids[int64_t(t) * k + lane] = id;
-      weights[int64_t(t) * k + lane] = w;
-      atomicAdd(&count[id], 1);
+  constexpr int kStep = kRouteThreads / 32;
+  constexpr int TT = NP <= 2 ? 4 : NP == 4 ? 2 : 1;  // 64 registers per thread
+  for (int t = t0 + warp; t < t1; t += kStep * TT) {
+    int id[TT];
+    float w[TT];
+    choose<NP, TT, T>(logits, ld, t, kStep, t1, E, k, normalize, id, w);
+#pragma unroll
+    for (int q = 0; q < TT; ++q) {
+      const int tq = t + q * kStep;
+      if (lane < k && tq < t1) {
+        ids[int64_t(tq) * k + lane] = id[q];
+        weights[int64_t(tq) * k + lane] = w[q];
+        atomicAdd(&count[id[q]], 1);
+      }
     }
   }
   __syncthreads();
@@ -327,9 +343,13 @@ __global__ void __launch_bounds__(kThreads) route_bwd_kernel(const T* __restrict
 }
 
 // ---------------------------------------------------------------------------
-// Exchange.  Block (x: threads of a token, y: tokens); 8 bf16 columns per
-// thread and step.
+// Exchange.  Bound by the memory, so what matters is how many loads a thread
+// has in flight: a block takes up to kTokens tokens per row of threads (a token
+// narrower than the block takes only a part of its threads), reads all their
+// slots at once, and each thread works on two 16-byte pieces of a row at a time.
 // ---------------------------------------------------------------------------
+constexpr int kTokens = 4;  // at most; fewer where the tokens would not fill the SMs
+
 __device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
   const uint32_t a[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -341,137 +361,189 @@ __device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
 __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
+__device__ __forceinline__ uint4 load16(const uint16_t* row, int v) { return __ldg(reinterpret_cast<const uint4*>(row) + v); }
 
-// The token's k slots (and weights) into shared memory; a slot outside the
-// grouped rows is recorded and becomes -1.
-__device__ __forceinline__ void load_choices(const int* __restrict__ slots, const float* __restrict__ weights, int64_t t,
-                                             int tokens, int k, int* s_slot, float* s_w, int* status) {
-  for (int j = threadIdx.x; j < k; j += blockDim.x) {
+struct Choices {
+  int slot[8 * kTokens][kMaxTopK];
+  float w[8 * kTokens][kMaxTopK];
+};
+
+// The slots (and weights) of the block's tokens [t0, t0 + n) into shared
+// memory; a slot outside the grouped rows is recorded and becomes -1.
+__device__ __forceinline__ void load_choices(const int* __restrict__ slots, const float* __restrict__ weights, int64_t t0,
+                                             int n, int tokens, int k, Choices& c, int* status) {
+  const int threads = blockDim.x * blockDim.y;
+  for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < n * k; i += threads) {
+    const int tt = i / k, j = i - tt * k;
     int s = -1;
-    if (t < tokens) {
-      s = slots[t * k + j];
+    float w = 0.f;
+    if (t0 + tt < tokens) {
+      s = slots[t0 * k + i];
+      if (weights) w = weights[t0 * k + i];
       if (uint32_t(s) >= uint32_t(tokens) * uint32_t(k)) {
-        record_status(status, kBadArgument, 200, int(t), s);
+        record_status(status, kBadArgument, 200, int(t0 + tt), s);
         s = -1;
       }
     }
-    s_slot[j] = s;
-    if (weights) s_w[j] = t < tokens ? weights[t * k + j] : 0.f;
+    c.slot[tt][j] = s;
+    c.w[tt][j] = w;
   }
   __syncthreads();
 }
 
 __global__ void __launch_bounds__(kThreads) dispatch_kernel(const uint16_t* __restrict__ x, int64_t ldx, int tokens, int k,
-                                                            int vecs, const int* __restrict__ slots,
+                                                            int vecs, int turns, const int* __restrict__ slots,
                                                             uint16_t* __restrict__ out, int64_t ldo, int* status) {
-  __shared__ int s_slot[8][kMaxTopK];
-  const int64_t t = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  load_choices(slots, nullptr, t, tokens, k, s_slot[threadIdx.y], nullptr, status);
-  if (t >= tokens) return;
-  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(x + t * ldx) + v);
-    for (int j = 0; j < k; ++j) {
-      const int s = s_slot[threadIdx.y][j];
-      if (s >= 0) reinterpret_cast<uint4*>(out + int64_t(s) * ldo)[v] = q;
+  __shared__ Choices c;
+  const int per = blockDim.y * turns;
+  const int64_t t0 = int64_t(blockIdx.x) * per;
+  load_choices(slots, nullptr, t0, per, tokens, k, c, status);
+  for (int tt = threadIdx.y; tt < per && t0 + tt < tokens; tt += blockDim.y) {
+    const uint16_t* src = x + (t0 + tt) * ldx;
+    for (int v = threadIdx.x; v < vecs; v += 2 * blockDim.x) {
+      const int v2 = v + blockDim.x;
+      const uint4 q = load16(src, v);
+      const uint4 q2 = v2 < vecs ? load16(src, v2) : q;
+      for (int j = 0; j < k; ++j) {
+        const int s = c.slot[tt][j];
+        if (s < 0) continue;
+        uint4* dst = reinterpret_cast<uint4*>(out + int64_t(s) * ldo);
+        dst[v] = q;
+        if (v2 < vecs) dst[v2] = q2;
+      }
     }
   }
 }
 
 // out[t] = residual[t] + sum_j w_j y[slot_j] (weights null: all 1).
 __global__ void __launch_bounds__(kThreads) combine_kernel(const uint16_t* __restrict__ y, int64_t ldy, int tokens, int k,
-                                                           int vecs, const int* __restrict__ slots,
+                                                           int vecs, int turns, const int* __restrict__ slots,
                                                            const float* __restrict__ weights,
                                                            const uint16_t* __restrict__ residual, int64_t ldr,
                                                            uint16_t* __restrict__ out, int64_t ldo, int* status) {
-  __shared__ int s_slot[8][kMaxTopK];
-  __shared__ float s_w[8][kMaxTopK];
-  const int64_t t = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  load_choices(slots, weights, t, tokens, k, s_slot[threadIdx.y], s_w[threadIdx.y], status);
-  if (t >= tokens) return;
-  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-    float acc[8] = {};
-    for (int j0 = 0; j0 < k; j0 += 4) {
-      uint4 q[4];
+  __shared__ Choices c;
+  const int per = blockDim.y * turns;
+  const int64_t t0 = int64_t(blockIdx.x) * per;
+  load_choices(slots, weights, t0, per, tokens, k, c, status);
+  for (int tt = threadIdx.y; tt < per && t0 + tt < tokens; tt += blockDim.y) {
+    for (int v = threadIdx.x; v < vecs; v += 2 * blockDim.x) {
+      const int v2 = v + blockDim.x;
+      const bool two = v2 < vecs;
+      float a0[8] = {}, a1[8] = {};
+      for (int j0 = 0; j0 < k; j0 += 4) {
+        uint4 q0[4], q1[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int s = j0 + i < k ? s_slot[threadIdx.y][j0 + i] : -1;
-        q[i] = s >= 0 ? __ldg(reinterpret_cast<const uint4*>(y + int64_t(s) * ldy) + v) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 4; ++i) {
+          const int s = j0 + i < k ? c.slot[tt][j0 + i] : -1;
+          const uint16_t* row = y + int64_t(s) * ldy;
+          q0[i] = q1[i] = make_uint4(0, 0, 0, 0);
+          if (s >= 0) q0[i] = load16(row, v);
+          if (s >= 0 && two) q1[i] = load16(row, v2);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (j0 + i >= k) break;
+          const float w = weights ? c.w[tt][j0 + i] : 1.f;
+          float f[8];
+          unpack8(q0[i], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a0[e] += w * f[e];
+          unpack8(q1[i], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a1[e] += w * f[e];
+        }
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (j0 + i >= k) break;
+      if (residual) {
+        const uint16_t* row = residual + (t0 + tt) * ldr;
         float f[8];
-        unpack8(q[i], f);
-        const float w = weights ? s_w[threadIdx.y][j0 + i] : 1.f;
+        unpack8(load16(row, v), f);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) acc[c] += w * f[c];
+        for (int e = 0; e < 8; ++e) a0[e] += f[e];
+        if (two) {
+          unpack8(load16(row, v2), f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a1[e] += f[e];
+        }
       }
+      uint4* dst = reinterpret_cast<uint4*>(out + (t0 + tt) * ldo);
+      dst[v] = pack8(a0);
+      if (two) dst[v2] = pack8(a1);
     }
-    if (residual) {
-      float f[8];
-      unpack8(__ldg(reinterpret_cast<const uint4*>(residual + t * ldr) + v), f);
-#pragma unroll
-      for (int c = 0; c < 8; ++c) acc[c] += f[c];
-    }
-    reinterpret_cast<uint4*>(out + t * ldo)[v] = pack8(acc);
   }
 }
 
 // dy[slot_j] = w_j dout[t];  dw_j = <dout[t], y[slot_j]> (fp32).
 __global__ void __launch_bounds__(kThreads) combine_bwd_kernel(const uint16_t* __restrict__ dout, int64_t ldd,
                                                                const uint16_t* __restrict__ y, int64_t ldy, int tokens,
-                                                               int k, int vecs, const int* __restrict__ slots,
+                                                               int k, int vecs, int turns, const int* __restrict__ slots,
                                                                const float* __restrict__ weights,
                                                                uint16_t* __restrict__ dy, int64_t lddy,
                                                                float* __restrict__ dweights, int* status) {
-  __shared__ int s_slot[8][kMaxTopK];
-  __shared__ float s_w[8][kMaxTopK];
-  __shared__ float s_dot[kWarps][kMaxTopK];
-  const int64_t t = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  load_choices(slots, weights, t, tokens, k, s_slot[threadIdx.y], s_w[threadIdx.y], status);
+  __shared__ Choices c;
+  __shared__ float s_dot[kTokens][kWarps][kMaxTopK];
+  const int per = blockDim.y * turns;
+  const int64_t t0 = int64_t(blockIdx.x) * per;
+  load_choices(slots, weights, t0, per, tokens, k, c, status);
   const int lane = threadIdx.x & 31;
   const int warps = blockDim.x >> 5, warp = threadIdx.y * warps + (threadIdx.x >> 5);
-  for (int j0 = 0; j0 < k; j0 += 4) {  // four choices at a time: dout is read again from L1/L2 for k > 4
-    float dot[4] = {};
-    if (t < tokens) {
-      for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-        uint4 q[4];
-        int s[4];
+#pragma unroll 1
+  for (int r = 0; r < turns; ++r) {
+    const int tt = r * blockDim.y + threadIdx.y;
+    const bool on = t0 + tt < tokens;
+    for (int j0 = 0; j0 < k; j0 += 2) {  // two choices at a time; dout comes from L1 again for k > 2
+      float dot[2] = {};
+      const int s0 = on ? c.slot[tt][j0] : -1, s1 = on && j0 + 1 < k ? c.slot[tt][j0 + 1] : -1;
+      if (on) {
+        const float w0 = c.w[tt][j0], w1 = j0 + 1 < k ? c.w[tt][j0 + 1] : 0.f;
+        const uint16_t* src = dout + (t0 + tt) * ldd;
+        for (int v = threadIdx.x; v < vecs; v += 2 * blockDim.x) {
+          const int at[2] = {v, v + int(blockDim.x)};
+          uint4 qd[2], q0[2], q1[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[i] = j0 + i < k ? s_slot[threadIdx.y][j0 + i] : -1;
-          q[i] = s[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(y + int64_t(s[i]) * ldy) + v) : make_uint4(0, 0, 0, 0);
-        }
-        float d[8];
-        unpack8(__ldg(reinterpret_cast<const uint4*>(dout + t * ldd) + v), d);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (s[i] < 0) continue;
-          float f[8], g[8];
-          unpack8(q[i], f);
-          const float w = s_w[threadIdx.y][j0 + i];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            dot[i] += d[c] * f[c];
-            g[c] = w * d[c];
+          for (int u = 0; u < 2; ++u) {
+            const bool in = at[u] < vecs;
+            qd[u] = q0[u] = q1[u] = make_uint4(0, 0, 0, 0);
+            if (in) qd[u] = load16(src, at[u]);
+            if (in && s0 >= 0) q0[u] = load16(y + int64_t(s0) * ldy, at[u]);
+            if (in && s1 >= 0) q1[u] = load16(y + int64_t(s1) * ldy, at[u]);
           }
-          reinterpret_cast<uint4*>(dy + int64_t(s[i]) * lddy)[v] = pack8(g);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if (at[u] >= vecs) break;
+            float d[8], f[8], g[8];
+            unpack8(qd[u], d);
+            unpack8(q0[u], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              dot[0] += d[e] * f[e];
+              g[e] = w0 * d[e];
+            }
+            if (s0 >= 0) reinterpret_cast<uint4*>(dy + int64_t(s0) * lddy)[at[u]] = pack8(g);
+            unpack8(q1[u], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              dot[1] += d[e] * f[e];
+              g[e] = w1 * d[e];
+            }
+            if (s1 >= 0) reinterpret_cast<uint4*>(dy + int64_t(s1) * lddy)[at[u]] = pack8(g);
+          }
         }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float sum = warp_sum(dot[i]);
-      if (lane == 0 && j0 + i < k) s_dot[warp][j0 + i] = sum;
+      for (int i = 0; i < 2; ++i) {
+        const float sum = warp_sum(dot[i]);
+        if (lane == 0 && j0 + i < k) s_dot[r][warp][j0 + i] = sum;
+      }
     }
   }
   __syncthreads();
-  if (t < tokens)
-    for (int j = threadIdx.x; j < k; j += blockDim.x) {
-      float sum = 0.f;
-      for (int w = 0; w < warps; ++w) sum += s_dot[threadIdx.y * warps + w][j];
-      dweights[t * k + j] = sum;
-    }
+  for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < per * k; i += blockDim.x * blockDim.y) {
+    const int tt = i / k, j = i - tt * k;
+    if (t0 + tt >= tokens) break;
+    float sum = 0.f;
+    for (int w = 0; w < warps; ++w) sum += s_dot[tt / blockDim.y][(tt % blockDim.y) * warps + w][j];
+    dweights[t0 * k + i] = sum;
+  }
 }
 
 static dim3 exchange_block(int vecs) {
@@ -479,6 +551,17 @@ static dim3 exchange_block(int vecs) {
   if (x > kThreads) x = kThreads;
   int y = kThreads / x;
   return dim3(x, y > 8 ? 8 : y);
+}
+
+// Tokens per row of threads: more than one only while the blocks still fill
+// every SM eight times (2048 threads).
+static int exchange_turns(int tokens, const dim3& block) {
+  const int64_t turns = tokens / (int64_t(block.y) * tdb_host::sm_count() * 8);
+  return turns < 1 ? 1 : turns > kTokens ? kTokens : int(turns);
+}
+static unsigned exchange_grid(int tokens, const dim3& block, int turns) {
+  const int per = int(block.y) * turns;
+  return unsigned((int64_t(tokens) + per - 1) / per);
 }
 
 static bool bad_rows(const void* p, int64_t ld, int H) {
@@ -599,8 +682,9 @@ TDB_API int tdb_moe_dispatch(const void* x, int64_t ldx, int tokens, int k, int 
   if (tokens == 0) return 0;
   if (!slots || bad_rows(x, ldx, H) || bad_rows(out, ldo, H)) return bad_alignment("moe dispatch");
   const dim3 block = exchange_block(H / 8);
-  dispatch_kernel<<<(tokens + block.y - 1) / block.y, block, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(x), ldx, tokens, k, H / 8, slots, static_cast<uint16_t*>(out), ldo,
+  const int turns = exchange_turns(tokens, block);
+  dispatch_kernel<<<exchange_grid(tokens, block, turns), block, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint16_t*>(x), ldx, tokens, k, H / 8, turns, slots, static_cast<uint16_t*>(out), ldo,
       tdb_host::status_ptr());
   tdb_host::launched(1);
   return int(cudaGetLastError());
@@ -614,8 +698,9 @@ TDB_API int tdb_moe_combine(const void* y, int64_t ldy, int tokens, int k, int H
   if (!slots || bad_rows(y, ldy, H) || bad_rows(out, ldo, H) || (residual && bad_rows(residual, ldr, H)))
     return bad_alignment("moe combine");
   const dim3 block = exchange_block(H / 8);
-  combine_kernel<<<(tokens + block.y - 1) / block.y, block, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(y), ldy, tokens, k, H / 8, slots, weights, static_cast<const uint16_t*>(residual), ldr,
+  const int turns = exchange_turns(tokens, block);
+  combine_kernel<<<exchange_grid(tokens, block, turns), block, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint16_t*>(y), ldy, tokens, k, H / 8, turns, slots, weights, static_cast<const uint16_t*>(residual), ldr,
       static_cast<uint16_t*>(out), ldo, tdb_host::status_ptr());
   tdb_host::launched(1);
   return int(cudaGetLastError());
@@ -630,8 +715,9 @@ TDB_API int tdb_moe_combine_bwd(const void* dout, int64_t ldd, const void* y, in
   if (!slots || !weights || !dweights || bad_rows(dout, ldd, H) || bad_rows(y, ldy, H) || bad_rows(dy, lddy, H))
     return bad_alignment("moe combine backward");
   const dim3 block = exchange_block(H / 8);
-  combine_bwd_kernel<<<(tokens + block.y - 1) / block.y, block, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(dout), ldd, static_cast<const uint16_t*>(y), ldy, tokens, k, H / 8, slots, weights,
+  const int turns = exchange_turns(tokens, block);
+  combine_bwd_kernel<<<exchange_grid(tokens, block, turns), block, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint16_t*>(dout), ldd, static_cast<const uint16_t*>(y), ldy, tokens, k, H / 8, turns, slots, weights,
       static_cast<uint16_t*>(dy), lddy, dweights, tdb_host::status_ptr());
   tdb_host::launched(1);
   return int(cudaGetLastError());

@@ -21,6 +21,8 @@ from __future__ import annotations
 
 import ctypes
 
+import torch
+
 from . import native
 from .gemm import BIAS, BIAS_GELU, GELU_BWD, STORE
 
@@ -41,7 +43,6 @@ def _need(cond, msg):
 
 def _rows(t, rows, cols, device, what):
     """Row stride of a bf16 [rows, cols] matrix with contiguous rows."""
-    import torch
     if t.dtype is not torch.bfloat16:
         raise TypeError(f"{what} must be bf16")
     ld, step = t.stride() if t.dim() == 2 else (0, 0)
@@ -53,7 +54,6 @@ def _rows(t, rows, cols, device, what):
 
 
 def _offsets(offsets, groups, device):
-    import torch
     _need(offsets.dtype is torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and
           offsets.get_device() == device, "offsets must be a contiguous int32 vector on the operands' device")
     _need(offsets.numel() == groups + 1, f"offsets must have groups + 1 = {groups + 1} entries")
@@ -61,7 +61,6 @@ def _offsets(offsets, groups, device):
 
 
 def _fp32(out, shape, device, what):
-    import torch
     if out.dtype is not torch.float32:
         raise TypeError(f"{what} is fp32")
     _need(out.shape == shape and out.is_contiguous() and out.get_device() == device,
@@ -69,7 +68,6 @@ def _fp32(out, shape, device, what):
 
 
 def _gemm(a, w, offsets, data_grad, mode, out, bias, aux, aux_out, tile):
-    import torch
     _need(a.dim() == 2 and a.is_cuda, "the row operand must be a matrix on a CUDA device")
     index = a.get_device()
     if w.dtype is not torch.bfloat16:
@@ -87,7 +85,7 @@ def _gemm(a, w, offsets, data_grad, mode, out, bias, aux, aux_out, tile):
         _need(bias.dtype is torch.bfloat16 and bias.shape == (groups, N) and bias.is_contiguous() and
               bias.get_device() == index, f"bias must be contiguous bf16 [{groups}, {N}] on the operands' device")
     if out is None:
-        out = torch.empty((rows, N), dtype=torch.bfloat16, device=a.device)
+        out = a.new_empty((rows, N))
     ldc = _rows(out, rows, N, index, "out")
     pre = aux_out if aux_out is not None else aux
     ld_aux = 0 if pre is None else _rows(pre, rows, N, index, "the pre-activation")
@@ -109,10 +107,9 @@ def linear(x, w, offsets, bias=None, out=None, tile=0):
 def linear_gelu(x, w, offsets, bias=None, pre_out=None, out=None, tile=0):
     """Returns (gelu(z), z) with z = x[r] @ w[g]^T (+ bias[g]) from one kernel.
     The activation is taken of the fp32 sum; z is its bf16 rounding."""
-    import torch
     _need(x.dim() == 2 and w.dim() == 3, "x must be [R, K] and w [groups, N, K]")
     if pre_out is None:
-        pre_out = torch.empty((x.shape[0], w.shape[1]), dtype=torch.bfloat16, device=x.device)
+        pre_out = x.new_empty((x.shape[0], w.shape[1]))
     if out is None:
         out = torch.empty_like(pre_out, memory_format=torch.contiguous_format)
     return _gemm(x, w, offsets, 0, BIAS_GELU, out, bias, None, pre_out, tile), pre_out
@@ -129,7 +126,6 @@ def matmul_nt(dy, w, offsets, out=None, gelu_pre=None, tile=0):
 def weight_grad(dy, x, offsets, out_f32=None, accumulate=True, tile=0):
     """``out_f32[g] (+)= dy_g^T @ x_g`` in fp32, [groups, N, K]; an empty group
     adds nothing (or gets zeros without ``accumulate``)."""
-    import torch
     _need(dy.dim() == 2 and x.dim() == 2 and dy.is_cuda, "dy and x must be matrices on a CUDA device")
     index = dy.get_device()
     rows, N = dy.shape
@@ -152,7 +148,6 @@ def weight_grad(dy, x, offsets, out_f32=None, accumulate=True, tile=0):
 @native.on_tensor_device
 def bias_grad(dy, offsets, out_f32=None, accumulate=True):
     """``out_f32[g] (+)= `` the sum of dy's rows of group g, fp32 [groups, N]."""
-    import torch
     _need(dy.dim() == 2 and dy.is_cuda, "dy must be a matrix on a CUDA device")
     index = dy.get_device()
     rows, N = dy.shape

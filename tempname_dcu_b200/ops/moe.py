@@ -28,6 +28,8 @@ import ctypes
 from dataclasses import dataclass
 from typing import Any
 
+import torch
+
 from . import native
 
 V, I, I64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
@@ -43,7 +45,12 @@ MAX_EXPERTS = 512
 MAX_TOP_K = 16
 
 
-@dataclass
+def _need(cond, msg):
+    if not cond:
+        raise ValueError(msg)
+
+
+@dataclass(frozen=True)
 class Routing:
     """A batch's choices of experts, grouped.
 
@@ -52,6 +59,9 @@ class Routing:
     offsets  int32 [experts + 1]  expert e holds grouped rows [offsets[e], offsets[e + 1])
     order    int32 [tokens * k]   grouped row -> choice (t * k + j); stable within an expert
     slots    int32 [tokens * k]   choice -> grouped row
+
+    Checked when it is made; a slot outside the grouped rows is found by the
+    kernels that use it and reported through the status word.
     """
     ids: Any
     weights: Any
@@ -59,6 +69,20 @@ class Routing:
     order: Any
     slots: Any
     normalize: bool = True
+
+    def __post_init__(self):
+        ids, weights, index = self.ids, self.weights, self.ids.get_device()
+        _need(ids.dim() == 2 and ids.dtype is torch.int32 and ids.is_contiguous(),
+              "ids must be contiguous int32 [tokens, k]")
+        _need(weights.shape == ids.shape and weights.dtype is torch.float32 and weights.is_contiguous(),
+              "weights must be contiguous fp32 [tokens, k]")
+        for t in (self.offsets, self.order, self.slots):
+            _need(t.dtype is torch.int32 and t.dim() == 1 and t.is_contiguous(),
+                  "offsets, order and slots must be contiguous int32 vectors")
+            _need(t.get_device() == index, "the tensors must be on one device")
+        _need(weights.get_device() == index, "the tensors must be on one device")
+        _need(self.slots.numel() == ids.numel() and self.order.numel() == ids.numel() and self.offsets.numel() > 1,
+              "order and slots must have tokens * k entries, offsets experts + 1")
 
     @property
     def tokens(self):
@@ -73,27 +97,22 @@ class Routing:
         return self.offsets.numel() - 1
 
 
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
+def _routing(ids, weights, offsets, order, slots, normalize):
+    """A Routing of tensors that ``route`` has just made itself."""
+    r = object.__new__(Routing)
+    r.__dict__.update(ids=ids, weights=weights, offsets=offsets, order=order, slots=slots, normalize=normalize)
+    return r
 
 
 def _check_routing(r, device):
-    """(tokens, k) of a routing whose tensors are fit for the kernels."""
-    import torch
-    ids, weights, slots = r.ids, r.weights, r.slots
-    _need(ids.dim() == 2 and ids.dtype is torch.int32 and ids.is_contiguous() and ids.get_device() == device,
-          "routing ids must be contiguous int32 [tokens, k] on the tensors' device")
-    _need(weights.shape == ids.shape and weights.dtype is torch.float32 and weights.is_contiguous() and
-          weights.get_device() == device, "routing weights must be contiguous fp32 [tokens, k] on the tensors' device")
-    _need(slots.numel() == ids.numel() and slots.dtype is torch.int32 and slots.is_contiguous() and
-          slots.get_device() == device, "routing slots must be contiguous int32 [tokens * k] on the tensors' device")
+    """(tokens, k) of a routing on the device of a call's tensors."""
+    ids = r.ids
+    _need(ids.get_device() == device, "the routing must be on the tensors' device")
     return ids.shape
 
 
 def _rows(t, rows, cols, device, what):
     """Row stride of a bf16 [rows, cols] matrix with contiguous rows."""
-    import torch
     ld, step = t.stride() if t.dim() == 2 else (0, 0)
     if rows <= 1:
         ld = cols
@@ -113,7 +132,6 @@ def _columns(t, what):
 
 def _logits(logits, what="logits"):
     """(tokens, experts, row stride, is bf16, device)."""
-    import torch
     _need(logits.dim() == 2 and logits.is_cuda, f"{what} must be a [tokens, experts] matrix on a CUDA device")
     bf16 = logits.dtype is torch.bfloat16
     _need(bf16 or logits.dtype is torch.float32, f"{what} must be fp32 or bf16")
@@ -133,16 +151,15 @@ def route(logits, top_k, normalize=True):
     The experts of the ``top_k`` largest logits (equal logits: the lower
     index first; NaN counts as the largest) with softmax weights over the
     chosen ones (``normalize``) or over all experts."""
-    import torch
     tokens, experts, ld, bf16, index = _logits(logits)
     _need(type(top_k) is int and 1 <= top_k <= min(experts, MAX_TOP_K),
           f"top_k must be 1..{MAX_TOP_K} and at most the number of experts")
     normalize = bool(normalize)
     dev = logits.device
     weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
-    ids = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
     order = torch.empty(tokens * top_k, dtype=torch.int32, device=dev)
     slots = torch.empty_like(order)
+    ids = torch.empty_like(weights, dtype=torch.int32)
     offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
     lib = native.lib()
     ints = lib.tdb_moe_route_scratch_ints(tokens, experts)
@@ -151,7 +168,7 @@ def route(logits, top_k, normalize=True):
                                    weights.data_ptr(), offsets.data_ptr(), order.data_ptr(), slots.data_ptr(),
                                    None if scratch is None else scratch.data_ptr(), native.current_stream(index)),
                  "moe route")
-    return Routing(ids, weights, offsets, order, slots, normalize)
+    return _routing(ids, weights, offsets, order, slots, normalize)
 
 
 @native.on_tensor_device
@@ -160,7 +177,6 @@ def route_bwd(logits, routing, dweights, out=None):
     (fp32 or bf16 [tokens, experts], default: the logits' type) is written
     whole: 0 for experts that were not chosen when the weights are
     normalised."""
-    import torch
     tokens, experts, ld, bf16, index = _logits(logits)
     shape = _check_routing(routing, index)
     _need(shape[0] == tokens and routing.experts == experts, "routing and logits have different sizes")
@@ -181,14 +197,13 @@ def route_bwd(logits, routing, dweights, out=None):
 @native.on_tensor_device
 def dispatch(x, routing, out=None):
     """Rows grouped by expert: ``out[slots[t*k + j]] = x[t]``, [tokens*k, H]."""
-    import torch
     tokens, H, index = _columns(x, "x")
     shape = _check_routing(routing, index)
     _need(shape[0] == tokens, "routing and x have different numbers of tokens")
     k = shape[1]
     ldx = _rows(x, tokens, H, index, "x")
     if out is None:
-        out = torch.empty((tokens * k, H), dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty((tokens * k, H))
     ldo = _rows(out, tokens * k, H, index, "out")
     native.check(native.lib().tdb_moe_dispatch(x.data_ptr(), ldx, tokens, k, H, routing.slots.data_ptr(),
                                                out.data_ptr(), ldo, native.current_stream(index)), "moe dispatch")
@@ -196,13 +211,12 @@ def dispatch(x, routing, out=None):
 
 
 def _combine(y, routing, weighted, residual, out, what):
-    import torch
     rows, H, index = _columns(y, "the grouped rows")
     tokens, k = _check_routing(routing, index)
     ldy = _rows(y, tokens * k, H, index, "the grouped rows")
     ldr = 0 if residual is None else _rows(residual, tokens, H, index, "residual")
     if out is None:
-        out = torch.empty((tokens, H), dtype=torch.bfloat16, device=y.device)
+        out = y.new_empty((tokens, H))
     ldo = _rows(out, tokens, H, index, "out")
     native.check(native.lib().tdb_moe_combine(y.data_ptr(), ldy, tokens, k, H, routing.slots.data_ptr(),
                                               routing.weights.data_ptr() if weighted else None,
@@ -227,7 +241,6 @@ def combine(ys, routing, residual=None, out=None):
 def combine_bwd(dout, ys, routing, out=None):
     """Gradients of ``combine``: (dys [tokens*k, H] bf16, dweights [tokens, k]
     fp32).  The residual's gradient is ``dout`` itself."""
-    import torch
     tokens, H, index = _columns(dout, "dout")
     shape = _check_routing(routing, index)
     _need(shape[0] == tokens, "routing and dout have different numbers of tokens")
@@ -235,7 +248,7 @@ def combine_bwd(dout, ys, routing, out=None):
     ldd = _rows(dout, tokens, H, index, "dout")
     ldy = _rows(ys, tokens * k, H, index, "ys")
     if out is None:
-        out = torch.empty((tokens * k, H), dtype=torch.bfloat16, device=dout.device)
+        out = dout.new_empty((tokens * k, H))
     ldo = _rows(out, tokens * k, H, index, "out")
     dweights = torch.empty_like(routing.weights)
     native.check(native.lib().tdb_moe_combine_bwd(dout.data_ptr(), ldd, ys.data_ptr(), ldy, tokens, k, H,

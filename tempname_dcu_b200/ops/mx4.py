@@ -21,6 +21,8 @@ from __future__ import annotations
 
 import ctypes
 
+import torch
+
 from . import native
 
 V, I, I64, LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_longlong
@@ -41,7 +43,6 @@ def _need(cond, msg):
 
 
 def _groups(offsets, device):
-    import torch
     if offsets is None:
         return 0
     _need(offsets.dtype is torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and
@@ -59,7 +60,6 @@ def scale_bytes(rows: int, k: int, groups: int = 0, matrices: int = 1) -> int:
 
 def _operand(q, sf, groups, device, what):
     """(matrices, rows, K) of a quantized operand."""
-    import torch
     _need(q.dtype is torch.uint8 and q.dim() in (2, 3) and q.is_contiguous() and q.get_device() == device,
           f"{what} must be contiguous uint8 [..., K/2] as written by quantize, on the operands' device")
     shape = q.shape
@@ -76,7 +76,6 @@ def _operand(q, sf, groups, device, what):
 def quantize(x, offsets=None, q=None, sf=None):
     """bf16 ``x`` [rows, K] or [matrices, rows, K] -> (q uint8 [..., K/2], sf
     uint8).  With ``offsets``, rows outside every group are not written."""
-    import torch
     if x.dtype is not torch.bfloat16:
         raise TypeError("quantize expects bf16")
     dims = x.dim()
@@ -114,7 +113,6 @@ def quantize(x, offsets=None, q=None, sf=None):
 def dequantize(q, sf, offsets=None, out=None):
     """The bf16 values of an operand produced by ``quantize`` with the same
     ``offsets``: exact, but for a value of 2^128, which reads as an infinity."""
-    import torch
     _need(q.is_cuda, "q must be on a CUDA device")
     index = q.get_device()
     groups = _groups(offsets, index)
@@ -134,7 +132,6 @@ def dequantize(q, sf, offsets=None, out=None):
 
 
 def _product(qx, sfx, qw, sfw, offsets, bias, out, tile):
-    import torch
     _need(qx.is_cuda and qx.dim() == 2, "qx must be a quantized [rows, K] operand on a CUDA device")
     index = qx.get_device()
     groups = _groups(offsets, index)

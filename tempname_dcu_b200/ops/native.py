@@ -103,12 +103,18 @@ def stream_ptr(stream=None) -> int:
     return int(stream.cuda_stream)
 
 
+_raw_stream = None
+
+
 def current_stream(device_index: int) -> int:
     """The current stream of a device as the integer that the entry points
     take.  (``stream_ptr`` builds a Stream object first, which costs as much as
     a small launch.)"""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(device_index)
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = torch._C._cuda_getCurrentRawStream
+    return _raw_stream(device_index)
 
 
 def on_tensor_device(fn):
