@@ -1,6 +1,7 @@
 // Entry points of the products grouped by expert (grouped.cuh) and the
 // grouped bias gradient.
 #include "grouped.cuh"
+#include "grouped_few.cuh"
 #include "grouped_launch.cuh"
 #include "tensor_map.h"
 
@@ -29,13 +30,26 @@ static int launch_rows_tile(int tile, const RowsParams& p, cudaStream_t s) {
   return launch_rows<1, 32, OP, MODE, false>(p, s);
 }
 
-// Tile of a call.  Forward and data gradient: up to 256 rows x 256 columns on
-// SM pairs (512), 128 x 128 (128) or 32 x 128 (32), the smallest whose rows
-// hold an average group.
+// Tile of a call.  Forward with few rows: the streaming kernel (16).  Forward
+// and data gradient: up to 256 rows x 256 columns on SM pairs (512), 128 x 128
+// (128) or 32 x 128 (32), the smallest whose rows hold an average group.
 static int pick_tile(int op, int64_t rows, int groups, int M, int N) {
   if (op == kWeightGrad) return M >= 256 && N >= 256 ? 512 : 128;
+  if (op == kForward && rows <= kFewRows) return 16;
   if (rows <= int64_t(groups) * 32) return 32;
   return rows >= int64_t(groups) * 192 && N >= 256 ? 512 : 128;
+}
+
+template <int MODE>
+static int launch_few(const RowsParams& p, const void* A, int64_t lda, const void* W, cudaStream_t s) {
+  const int64_t units = int64_t((p.N + 15) / 16) * (p.rows < p.groups ? p.rows : p.groups);
+  const int64_t most = int64_t(tdb_host::sm_count()) * 2;
+  const unsigned grid = unsigned(units < most ? units : most);
+  few_rows_kernel<MODE><<<grid, kFewThreads, 0, s>>>(static_cast<const uint16_t*>(A), lda, static_cast<const uint16_t*>(W),
+                                                     p.offsets, p.groups, p.rows, p.N, p.K, p.bias, p.C, p.ldc, p.aux_out,
+                                                     p.ld_aux, p.status);
+  tdb_host::launched(1);
+  return int(cudaGetLastError());
 }
 
 // Sums of dy's rows per group and column.  One block per group and 64
@@ -115,8 +129,25 @@ TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data
       (mode == gemm::kGeluBwd && (!aux || misaligned(aux) || ld_aux % 8 || ld_aux < N)))
     return bad("grouped: the pre-activation must be 16-byte aligned with 16-byte row strides");
   if (tile == 0) tile = tdb::grouped::pick_tile(data_grad ? kDataGrad : kForward, rows, groups, 0, N);
-  if (tile != 32 && tile != 128 && tile != 512) return bad("grouped: tile must be 0, 32, 128 or 512");
+  if (tile != 32 && tile != 128 && tile != 512 && (tile != 16 || data_grad || rows > kFewRows))
+    return bad("grouped: tile must be 0, 32, 128 or 512 (16: forward with at most 16 rows)");
   RowsParams p = {};
+  p.offsets = offsets;
+  p.groups = groups;
+  p.rows = rows;
+  p.N = N;
+  p.K = K;
+  p.band = kBand;
+  p.C = static_cast<uint16_t*>(C);
+  p.ldc = ldc;
+  p.aux_out = static_cast<uint16_t*>(aux_out);
+  p.aux = static_cast<const uint16_t*>(aux);
+  p.ld_aux = ld_aux;
+  p.bias = static_cast<const uint16_t*>(bias);
+  p.status = tdb_host::status_ptr();
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (tile == 16)
+    return mode == gemm::kBiasGelu ? launch_few<gemm::kBiasGelu>(p, A, lda, W, s) : launch_few<gemm::kBias>(p, A, lda, W, s);
   const uint32_t box_rows = tile == 512 ? 64 : 32;
   int rc = tdb_host::make_tmap_2d(&p.tmB, A, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(K), uint64_t(rows),
                                   uint64_t(lda), gemm::BK, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -136,20 +167,6 @@ TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data
     rc = make_output_map(&p.tmAux, aux_out, rows, N, ld_aux);
     if (rc) return rc;
   }
-  p.offsets = offsets;
-  p.groups = groups;
-  p.rows = rows;
-  p.N = N;
-  p.K = K;
-  p.band = kBand;
-  p.C = static_cast<uint16_t*>(C);
-  p.ldc = ldc;
-  p.aux_out = static_cast<uint16_t*>(aux_out);
-  p.aux = static_cast<const uint16_t*>(aux);
-  p.ld_aux = ld_aux;
-  p.bias = static_cast<const uint16_t*>(bias);
-  p.status = tdb_host::status_ptr();
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (data_grad)
     return mode == gemm::kGeluBwd ? launch_rows_tile<kDataGrad, gemm::kGeluBwd>(tile, p, s)
                                   : launch_rows_tile<kDataGrad, gemm::kStore>(tile, p, s);

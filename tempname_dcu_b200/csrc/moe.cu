@@ -77,32 +77,71 @@ __device__ __forceinline__ void choose(const T* logits, int64_t ld, int t0, int 
   for (int q = 0; q < TT; ++q)
 #pragma unroll
     for (int i = 0; i < NP; ++i) key[q][i] = i * 32 + lane < E ? order_key(v[q][i]) : 0u;
-  float my_z[TT], top[TT];
+  // Up to four experts per lane are sorted first (equal keys keep their order),
+  // so a round looks at each lane's head only; more are searched every round.
+  constexpr bool kSort = NP <= 4;
+  int idx[TT][NP];
+#pragma unroll
+  for (int q = 0; q < TT; ++q) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) idx[q][i] = i * 32 + lane;
+    if (kSort) {
+#pragma unroll
+      for (int end = NP - 1; end > 0; --end)
+#pragma unroll
+        for (int i = 0; i < end; ++i) {
+          const bool swap = key[q][i + 1] > key[q][i];
+          const uint32_t hi = swap ? key[q][i + 1] : key[q][i], lo = swap ? key[q][i] : key[q][i + 1];
+          const int ih = swap ? idx[q][i + 1] : idx[q][i], il = swap ? idx[q][i] : idx[q][i + 1];
+          key[q][i] = hi;
+          key[q][i + 1] = lo;
+          idx[q][i] = ih;
+          idx[q][i + 1] = il;
+        }
+    }
+  }
+  uint32_t top_key[TT], my_key[TT];
   for (int j = 0; j < k; ++j) {
 #pragma unroll
     for (int q = 0; q < TT; ++q) {
       uint32_t best = key[q][0];
-      int at = 0;
+      int at = idx[q][0];
+      if (!kSort) {
 #pragma unroll
-      for (int i = 1; i < NP; ++i)
-        if (key[q][i] > best) {
-          best = key[q][i];
-          at = i;
-        }
-      const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-      const uint32_t id = __reduce_min_sync(0xffffffffu, best == m ? uint32_t(at * 32 + lane) : 0x7fffffffu);
-      if ((id & 31u) == uint32_t(lane)) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-          if (uint32_t(i) == id >> 5) key[q][i] = 0u;
+        for (int i = 1; i < NP; ++i)
+          if (key[q][i] > best) {
+            best = key[q][i];
+            at = idx[q][i];
+          }
       }
-      const float z = key_value(m);
-      if (j == 0) top[q] = z;
+      const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+      const uint32_t id = __reduce_min_sync(0xffffffffu, best == m ? uint32_t(at) : 0x7fffffffu);
+      if ((id & 31u) == uint32_t(lane)) {
+        if (kSort) {
+#pragma unroll
+          for (int i = 0; i + 1 < NP; ++i) {
+            key[q][i] = key[q][i + 1];
+            idx[q][i] = idx[q][i + 1];
+          }
+          key[q][NP - 1] = 0u;
+        } else {
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+            if (uint32_t(i) == id >> 5) key[q][i] = 0u;
+        }
+      }
+      if (j == 0) top_key[q] = m;
       if (j == 0 || lane == j) {
         my_id[q] = int(id);
-        my_z[q] = z;
+        my_key[q] = m;
       }
     }
+  }
+  float my_z[TT], top[TT];
+#pragma unroll
+  for (int q = 0; q < TT; ++q) {
+    my_z[q] = key_value(my_key[q]);
+    top[q] = key_value(top_key[q]);
   }
 #pragma unroll
   for (int q = 0; q < TT; ++q) {
@@ -148,6 +187,7 @@ __device__ __forceinline__ void scan_experts(const int* total, int* start, int E
 // Stable ranks of the block's choices [c0, c1): base[e] is the first slot of
 // the block's choices of expert e.  Warp w < kRankWarps owns a contiguous
 // share, so ranks follow the choice index.  wh: [kRankWarps][E] shared ints.
+// ids: the block's choices in shared memory, ids[c - c0].
 __device__ __forceinline__ void rank_choices(const int* ids, int c0, int c1, int E, const int* base, int* wh,
                                              int* __restrict__ order, int* __restrict__ slots) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -155,7 +195,7 @@ __device__ __forceinline__ void rank_choices(const int* ids, int c0, int c1, int
   const int lo = warp < kRankWarps ? min(c0 + warp * share, c1) : c1, hi = min(lo + share, c1);
   for (int i = threadIdx.x; i < kRankWarps * E; i += kRouteThreads) wh[i] = 0;
   __syncthreads();
-  for (int c = lo + lane; c < hi; c += 32) atomicAdd(&wh[warp * E + ids[c]], 1);
+  for (int c = lo + lane; c < hi; c += 32) atomicAdd(&wh[warp * E + ids[c - c0]], 1);
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kRouteThreads) {
     int run = base[e];
@@ -170,7 +210,7 @@ __device__ __forceinline__ void rank_choices(const int* ids, int c0, int c1, int
   for (int c = lo; c < hi; c += 32) {
     const int mine = c + lane;
     const bool on = mine < hi;
-    const int id = on ? ids[mine] : -1;
+    const int id = on ? ids[mine - c0] : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, id);
     int first = 0;
     if (on) first = wh[warp * E + id];
@@ -194,6 +234,7 @@ __global__ void __launch_bounds__(kRouteThreads) choose_kernel(const T* __restri
                                                                int* __restrict__ offsets, int* __restrict__ order,
                                                                int* __restrict__ slots) {
   extern __shared__ int sh[];
+  __shared__ int s_ids[kTokensPerBlock * kMaxTopK];
   int* count = sh;  // [E]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < E; e += kRouteThreads) count[e] = 0;
@@ -210,6 +251,7 @@ __global__ void __launch_bounds__(kRouteThreads) choose_kernel(const T* __restri
       const int tq = t + q * kStep;
       if (lane < k && tq < t1) {
         ids[int64_t(tq) * k + lane] = id[q];
+        if (gridDim.x == 1) s_ids[tq * k + lane] = id[q];
         weights[int64_t(tq) * k + lane] = w[q];
         atomicAdd(&count[id[q]], 1);
       }
@@ -225,7 +267,7 @@ __global__ void __launch_bounds__(kRouteThreads) choose_kernel(const T* __restri
   if (warp == 0) scan_experts(count, start, E);
   __syncthreads();
   for (int e = threadIdx.x; e <= E; e += kRouteThreads) offsets[e] = start[e];
-  rank_choices(ids, 0, tokens * k, E, start, wh, order, slots);
+  rank_choices(s_ids, 0, tokens * k, E, start, wh, order, slots);
 }
 
 // Slots of one block's choices from every block's counts.
@@ -238,6 +280,9 @@ __global__ void __launch_bounds__(kRouteThreads) group_kernel(const int* __restr
   int* before = sh + E;     // [E]
   int* start = before + E;  // [E + 1]
   int* wh = start + E + 1;  // [kRankWarps][E]
+  __shared__ int s_ids[kTokensPerBlock * kMaxTopK];
+  const int t0 = blockIdx.x * kTokensPerBlock, t1 = min(t0 + kTokensPerBlock, tokens);
+  for (int i = threadIdx.x; i < (t1 - t0) * k; i += kRouteThreads) s_ids[i] = ids[int64_t(t0) * k + i];
   for (int e = threadIdx.x; e < E; e += kRouteThreads) total[e] = before[e] = 0;
   __syncthreads();
   // A thread sums the counts of one expert over every `groups`-th block, eight
@@ -270,8 +315,7 @@ __global__ void __launch_bounds__(kRouteThreads) group_kernel(const int* __restr
     for (int i = threadIdx.x; i <= E; i += kRouteThreads) offsets[i] = start[i];
   for (int i = threadIdx.x; i < E; i += kRouteThreads) before[i] += start[i];
   __syncthreads();
-  const int t0 = blockIdx.x * kTokensPerBlock, t1 = min(t0 + kTokensPerBlock, tokens);
-  rank_choices(ids, t0 * k, t1 * k, E, before, wh, order, slots);
+  rank_choices(s_ids, t0 * k, t1 * k, E, before, wh, order, slots);
 }
 
 __device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
@@ -346,7 +390,7 @@ __global__ void __launch_bounds__(kThreads) route_bwd_kernel(const T* __restrict
 // Exchange.  Bound by the memory, so what matters is how many loads a thread
 // has in flight: a block takes up to kTokens tokens per row of threads (a token
 // narrower than the block takes only a part of its threads), reads all their
-// slots at once, and each thread works on two 16-byte pieces of a row at a time.
+// slots at once, and each thread issues all its loads of a step before it uses any.
 // ---------------------------------------------------------------------------
 constexpr int kTokens = 4;  // at most; fewer where the tokens would not fill the SMs
 
@@ -391,94 +435,103 @@ __device__ __forceinline__ void load_choices(const int* __restrict__ slots, cons
   __syncthreads();
 }
 
+// U: 16-byte pieces of a row per thread and step.
+constexpr int kDispatchPieces = 4;
+
 __global__ void __launch_bounds__(kThreads) dispatch_kernel(const uint16_t* __restrict__ x, int64_t ldx, int tokens, int k,
                                                             int vecs, int turns, const int* __restrict__ slots,
                                                             uint16_t* __restrict__ out, int64_t ldo, int* status) {
+  constexpr int U = kDispatchPieces;
   __shared__ Choices c;
   const int per = blockDim.y * turns;
   const int64_t t0 = int64_t(blockIdx.x) * per;
   load_choices(slots, nullptr, t0, per, tokens, k, c, status);
   for (int tt = threadIdx.y; tt < per && t0 + tt < tokens; tt += blockDim.y) {
     const uint16_t* src = x + (t0 + tt) * ldx;
-    for (int v = threadIdx.x; v < vecs; v += 2 * blockDim.x) {
-      const int v2 = v + blockDim.x;
-      const uint4 q = load16(src, v);
-      const uint4 q2 = v2 < vecs ? load16(src, v2) : q;
+    for (int v = threadIdx.x; v < vecs; v += U * blockDim.x) {
+      uint4 q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = v + u * blockDim.x;
+        if (at < vecs) q[u] = load16(src, at);
+      }
       for (int j = 0; j < k; ++j) {
         const int s = c.slot[tt][j];
         if (s < 0) continue;
         uint4* dst = reinterpret_cast<uint4*>(out + int64_t(s) * ldo);
-        dst[v] = q;
-        if (v2 < vecs) dst[v2] = q2;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int at = v + u * blockDim.x;
+          if (at < vecs) dst[at] = q[u];
+        }
       }
     }
   }
 }
 
+// Pieces per thread when KC >= k rows are read for each: eight loads in flight.
+template <int KC>
+constexpr int kCombinePieces = KC >= 8 ? 1 : 8 / KC;
+
 // out[t] = residual[t] + sum_j w_j y[slot_j] (weights null: all 1).
+template <int KC>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const uint16_t* __restrict__ y, int64_t ldy, int tokens, int k,
                                                            int vecs, int turns, const int* __restrict__ slots,
                                                            const float* __restrict__ weights,
                                                            const uint16_t* __restrict__ residual, int64_t ldr,
                                                            uint16_t* __restrict__ out, int64_t ldo, int* status) {
+  constexpr int U = kCombinePieces<KC>;
   __shared__ Choices c;
   const int per = blockDim.y * turns;
   const int64_t t0 = int64_t(blockIdx.x) * per;
   load_choices(slots, weights, t0, per, tokens, k, c, status);
   for (int tt = threadIdx.y; tt < per && t0 + tt < tokens; tt += blockDim.y) {
-    for (int v = threadIdx.x; v < vecs; v += 2 * blockDim.x) {
-      const int v2 = v + blockDim.x;
-      const bool two = v2 < vecs;
-      float a0[8] = {}, a1[8] = {};
-      for (int j0 = 0; j0 < k; j0 += 4) {
-        uint4 q0[4], q1[4];
+    for (int v = threadIdx.x; v < vecs; v += U * blockDim.x) {
+      uint4 q[U][KC];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int s = j0 + i < k ? c.slot[tt][j0 + i] : -1;
-          const uint16_t* row = y + int64_t(s) * ldy;
-          q0[i] = q1[i] = make_uint4(0, 0, 0, 0);
-          if (s >= 0) q0[i] = load16(row, v);
-          if (s >= 0 && two) q1[i] = load16(row, v2);
-        }
+      for (int j = 0; j < KC; ++j) {
+        const int s = j < k ? c.slot[tt][j] : -1;
+        const uint16_t* row = y + int64_t(s) * ldy;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (j0 + i >= k) break;
-          const float w = weights ? c.w[tt][j0 + i] : 1.f;
-          float f[8];
-          unpack8(q0[i], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) a0[e] += w * f[e];
-          unpack8(q1[i], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) a1[e] += w * f[e];
+        for (int u = 0; u < U; ++u) {
+          const int at = v + u * blockDim.x;
+          q[u][j] = make_uint4(0, 0, 0, 0);
+          if (s >= 0 && at < vecs) q[u][j] = load16(row, at);
         }
       }
-      if (residual) {
-        const uint16_t* row = residual + (t0 + tt) * ldr;
-        float f[8];
-        unpack8(load16(row, v), f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a0[e] += f[e];
-        if (two) {
-          unpack8(load16(row, v2), f);
+      for (int u = 0; u < U; ++u) {
+        const int at = v + u * blockDim.x;
+        if (at >= vecs) break;
+        float acc[8] = {}, f[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) a1[e] += f[e];
+        for (int j = 0; j < KC; ++j) {
+          if (j >= k) break;
+          const float w = weights ? c.w[tt][j] : 1.f;
+          unpack8(q[u][j], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] += w * f[e];
         }
+        if (residual) {
+          unpack8(load16(residual + (t0 + tt) * ldr, at), f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] += f[e];
+        }
+        reinterpret_cast<uint4*>(out + (t0 + tt) * ldo)[at] = pack8(acc);
       }
-      uint4* dst = reinterpret_cast<uint4*>(out + (t0 + tt) * ldo);
-      dst[v] = pack8(a0);
-      if (two) dst[v2] = pack8(a1);
     }
   }
 }
 
 // dy[slot_j] = w_j dout[t];  dw_j = <dout[t], y[slot_j]> (fp32).
+template <int KC>
 __global__ void __launch_bounds__(kThreads) combine_bwd_kernel(const uint16_t* __restrict__ dout, int64_t ldd,
                                                                const uint16_t* __restrict__ y, int64_t ldy, int tokens,
                                                                int k, int vecs, int turns, const int* __restrict__ slots,
                                                                const float* __restrict__ weights,
                                                                uint16_t* __restrict__ dy, int64_t lddy,
                                                                float* __restrict__ dweights, int* status) {
+  constexpr int U = kCombinePieces<KC>;
   __shared__ Choices c;
   __shared__ float s_dot[kTokens][kWarps][kMaxTopK];
   const int per = blockDim.y * turns;
@@ -489,51 +542,56 @@ __global__ void __launch_bounds__(kThreads) combine_bwd_kernel(const uint16_t* _
 #pragma unroll 1
   for (int r = 0; r < turns; ++r) {
     const int tt = r * blockDim.y + threadIdx.y;
-    const bool on = t0 + tt < tokens;
-    for (int j0 = 0; j0 < k; j0 += 2) {  // two choices at a time; dout comes from L1 again for k > 2
-      float dot[2] = {};
-      const int s0 = on ? c.slot[tt][j0] : -1, s1 = on && j0 + 1 < k ? c.slot[tt][j0 + 1] : -1;
-      if (on) {
-        const float w0 = c.w[tt][j0], w1 = j0 + 1 < k ? c.w[tt][j0 + 1] : 0.f;
-        const uint16_t* src = dout + (t0 + tt) * ldd;
-        for (int v = threadIdx.x; v < vecs; v += 2 * blockDim.x) {
-          const int at[2] = {v, v + int(blockDim.x)};
-          uint4 qd[2], q0[2], q1[2];
+    float dot[KC] = {};
+    if (t0 + tt < tokens) {
+      const uint16_t* src = dout + (t0 + tt) * ldd;
+      for (int v = threadIdx.x; v < vecs; v += U * blockDim.x) {
+        uint4 q[U][KC], qd[U];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const bool in = at[u] < vecs;
-            qd[u] = q0[u] = q1[u] = make_uint4(0, 0, 0, 0);
-            if (in) qd[u] = load16(src, at[u]);
-            if (in && s0 >= 0) q0[u] = load16(y + int64_t(s0) * ldy, at[u]);
-            if (in && s1 >= 0) q1[u] = load16(y + int64_t(s1) * ldy, at[u]);
+        for (int u = 0; u < U; ++u) {
+          const int at = v + u * blockDim.x;
+          qd[u] = make_uint4(0, 0, 0, 0);
+          if (at < vecs) qd[u] = load16(src, at);
+        }
+#pragma unroll
+        for (int j = 0; j < KC; ++j) {
+          const int s = j < k ? c.slot[tt][j] : -1;
+          const uint16_t* row = y + int64_t(s) * ldy;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int at = v + u * blockDim.x;
+            q[u][j] = make_uint4(0, 0, 0, 0);
+            if (s >= 0 && at < vecs) q[u][j] = load16(row, at);
           }
+        }
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            if (at[u] >= vecs) break;
-            float d[8], f[8], g[8];
-            unpack8(qd[u], d);
-            unpack8(q0[u], f);
+        for (int u = 0; u < U; ++u) {
+          const int at = v + u * blockDim.x;
+          if (at >= vecs) break;
+          float d[8], f[8];
+          unpack8(qd[u], d);
+#pragma unroll
+          for (int j = 0; j < KC; ++j) {
+            if (j >= k) break;
+            const int s = c.slot[tt][j];
+            if (s < 0) continue;
+            const float w = c.w[tt][j];
+            unpack8(q[u][j], f);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              dot[0] += d[e] * f[e];
-              g[e] = w0 * d[e];
+              dot[j] += d[e] * f[e];
+              f[e] = w * d[e];
             }
-            if (s0 >= 0) reinterpret_cast<uint4*>(dy + int64_t(s0) * lddy)[at[u]] = pack8(g);
-            unpack8(q1[u], f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              dot[1] += d[e] * f[e];
-              g[e] = w1 * d[e];
-            }
-            if (s1 >= 0) reinterpret_cast<uint4*>(dy + int64_t(s1) * lddy)[at[u]] = pack8(g);
+            reinterpret_cast<uint4*>(dy + int64_t(s) * lddy)[at] = pack8(f);
           }
         }
       }
+    }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float sum = warp_sum(dot[i]);
-        if (lane == 0 && j0 + i < k) s_dot[r][warp][j0 + i] = sum;
-      }
+    for (int j = 0; j < KC; ++j) {
+      if (j >= k) break;
+      const float sum = warp_sum(dot[j]);
+      if (lane == 0) s_dot[r][warp][j] = sum;
     }
   }
   __syncthreads();
@@ -546,8 +604,9 @@ __global__ void __launch_bounds__(kThreads) combine_bwd_kernel(const uint16_t* _
   }
 }
 
-static dim3 exchange_block(int vecs) {
-  int x = (vecs + 31) / 32 * 32;
+// Threads of a token, each with `pieces` pieces of its row, and tokens of a block.
+static dim3 exchange_block(int vecs, int pieces) {
+  int x = ((vecs + pieces - 1) / pieces + 31) / 32 * 32;
   if (x > kThreads) x = kThreads;
   int y = kThreads / x;
   return dim3(x, y > 8 ? 8 : y);
@@ -681,7 +740,7 @@ TDB_API int tdb_moe_dispatch(const void* x, int64_t ldx, int tokens, int k, int 
   if (int rc = check_exchange("moe dispatch", tokens, k, H)) return rc;
   if (tokens == 0) return 0;
   if (!slots || bad_rows(x, ldx, H) || bad_rows(out, ldo, H)) return bad_alignment("moe dispatch");
-  const dim3 block = exchange_block(H / 8);
+  const dim3 block = exchange_block(H / 8, kDispatchPieces);
   const int turns = exchange_turns(tokens, block);
   dispatch_kernel<<<exchange_grid(tokens, block, turns), block, 0, static_cast<cudaStream_t>(stream)>>>(
       static_cast<const uint16_t*>(x), ldx, tokens, k, H / 8, turns, slots, static_cast<uint16_t*>(out), ldo,
@@ -697,11 +756,21 @@ TDB_API int tdb_moe_combine(const void* y, int64_t ldy, int tokens, int k, int H
   if (tokens == 0) return 0;
   if (!slots || bad_rows(y, ldy, H) || bad_rows(out, ldo, H) || (residual && bad_rows(residual, ldr, H)))
     return bad_alignment("moe combine");
-  const dim3 block = exchange_block(H / 8);
-  const int turns = exchange_turns(tokens, block);
-  combine_kernel<<<exchange_grid(tokens, block, turns), block, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(y), ldy, tokens, k, H / 8, turns, slots, weights, static_cast<const uint16_t*>(residual), ldr,
-      static_cast<uint16_t*>(out), ldo, tdb_host::status_ptr());
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+#define TDB_COMBINE(KC)                                                                                              \
+  {                                                                                                                  \
+    const dim3 block = exchange_block(H / 8, kCombinePieces<KC>);                                                    \
+    const int turns = exchange_turns(tokens, block);                                                                 \
+    combine_kernel<KC><<<exchange_grid(tokens, block, turns), block, 0, s>>>(                                        \
+        static_cast<const uint16_t*>(y), ldy, tokens, k, H / 8, turns, slots, weights,                               \
+        static_cast<const uint16_t*>(residual), ldr, static_cast<uint16_t*>(out), ldo, tdb_host::status_ptr());      \
+  }
+  if (k == 1) TDB_COMBINE(1)
+  else if (k == 2) TDB_COMBINE(2)
+  else if (k <= 4) TDB_COMBINE(4)
+  else if (k <= 8) TDB_COMBINE(8)
+  else TDB_COMBINE(16)
+#undef TDB_COMBINE
   tdb_host::launched(1);
   return int(cudaGetLastError());
 }
@@ -714,11 +783,21 @@ TDB_API int tdb_moe_combine_bwd(const void* dout, int64_t ldd, const void* y, in
   if (tokens == 0) return 0;
   if (!slots || !weights || !dweights || bad_rows(dout, ldd, H) || bad_rows(y, ldy, H) || bad_rows(dy, lddy, H))
     return bad_alignment("moe combine backward");
-  const dim3 block = exchange_block(H / 8);
-  const int turns = exchange_turns(tokens, block);
-  combine_bwd_kernel<<<exchange_grid(tokens, block, turns), block, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(dout), ldd, static_cast<const uint16_t*>(y), ldy, tokens, k, H / 8, turns, slots, weights,
-      static_cast<uint16_t*>(dy), lddy, dweights, tdb_host::status_ptr());
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+#define TDB_COMBINE_BWD(KC)                                                                                          \
+  {                                                                                                                  \
+    const dim3 block = exchange_block(H / 8, kCombinePieces<KC>);                                                    \
+    const int turns = exchange_turns(tokens, block);                                                                 \
+    combine_bwd_kernel<KC><<<exchange_grid(tokens, block, turns), block, 0, s>>>(                                    \
+        static_cast<const uint16_t*>(dout), ldd, static_cast<const uint16_t*>(y), ldy, tokens, k, H / 8, turns,      \
+        slots, weights, static_cast<uint16_t*>(dy), lddy, dweights, tdb_host::status_ptr());                         \
+  }
+  if (k == 1) TDB_COMBINE_BWD(1)
+  else if (k == 2) TDB_COMBINE_BWD(2)
+  else if (k <= 4) TDB_COMBINE_BWD(4)
+  else if (k <= 8) TDB_COMBINE_BWD(8)
+  else TDB_COMBINE_BWD(16)
+#undef TDB_COMBINE_BWD
   tdb_host::launched(1);
   return int(cudaGetLastError());
 }

@@ -127,18 +127,24 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __re
                                                             const int* offsets, int groups, int rows, int mat_blocks,
                                                             int* status) {
   extern __shared__ int sh[];
-  Layout l;
-  if (!make_layout(l, offsets, groups, rows, mat_blocks, sh, status)) return;
   const int lane = threadIdx.x & 31;
   const int pieces = (K + 255) / 256;
   const int first = blockIdx.y * kBatch;
-  for (int r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < total_rows; r += gridDim.x * kWarps) {
-    const int k0 = first * 256 + lane * 8;
+  const int k0 = first * 256 + lane * 8;
+  auto load = [&](int r, uint4 (&in)[kBatch]) {
     const uint16_t* src = x + int64_t(r) * ldx + k0;
-    uint4 in[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b)
-      in[b] = k0 + b * 256 < K ? __ldg(reinterpret_cast<const uint4*>(src + b * 256)) : make_uint4(0, 0, 0, 0);
+      in[b] = r < total_rows && k0 + b * 256 < K ? __ldg(reinterpret_cast<const uint4*>(src + b * 256))
+                                                 : make_uint4(0, 0, 0, 0);
+  };
+  const int step = gridDim.x * kWarps;
+  int r = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  uint4 in[kBatch];
+  load(r, in);  // before the groups' table is built
+  Layout l;
+  if (!make_layout(l, offsets, groups, rows, mat_blocks, sh, status)) return;
+  for (; r < total_rows; r += step, load(r, in)) {
     int64_t blk;
     int row;
     if (!l.find(r, blk, row)) continue;
