@@ -30,12 +30,19 @@ static int launch_rows_tile(int tile, const RowsParams& p, cudaStream_t s) {
   return launch_rows<1, 32, OP, MODE, false>(p, s);
 }
 
-// Tile of a call.  Forward with few rows: the streaming kernel (16).  Forward
-// and data gradient: up to 256 rows x 256 columns on SM pairs (512), 128 x 128
-// (128) or 32 x 128 (32), the smallest whose rows hold an average group.
+// Tile of a call.  Forward with few rows: the streaming kernel (16) while the
+// 128-column tiles of the groups that can have rows would leave SMs idle (two
+// experts of 4096 x 16384 and one token: 52 us against 76; 16384 x 4096, 256
+// tiles: 53 against 50).  Otherwise up to 256 rows x 256 columns on SM pairs
+// (512), 128 x 128 (128) or 32 x 128 (32), the smallest whose rows hold an
+// average group (8 groups of 16384 x 4096 with 64 rows each: 272 us with 32,
+// 195 with 128, 197 with 512; with 512 rows each 596 with 128, 375 with 512).
 static int pick_tile(int op, int64_t rows, int groups, int M, int N) {
   if (op == kWeightGrad) return M >= 256 && N >= 256 ? 512 : 128;
-  if (op == kForward && rows <= kFewRows) return 16;
+  if (op == kForward && rows <= kFewRows) {
+    const int64_t tiles = (rows < groups ? rows : groups) * ((N + 127) / 128);
+    if (tiles * 5 < int64_t(tdb_host::sm_count()) * 4) return 16;
+  }
   if (rows <= int64_t(groups) * 32) return 32;
   return rows >= int64_t(groups) * 192 && N >= 256 ? 512 : 128;
 }
@@ -45,9 +52,17 @@ static int launch_few(const RowsParams& p, const void* A, int64_t lda, const voi
   const int64_t units = int64_t((p.N + 15) / 16) * (p.rows < p.groups ? p.rows : p.groups);
   const int64_t most = int64_t(tdb_host::sm_count()) * 2;
   const unsigned grid = unsigned(units < most ? units : most);
-  few_rows_kernel<MODE><<<grid, kFewThreads, 0, s>>>(static_cast<const uint16_t*>(A), lda, static_cast<const uint16_t*>(W),
-                                                     p.offsets, p.groups, p.rows, p.N, p.K, p.bias, p.C, p.ldc, p.aux_out,
-                                                     p.ld_aux, p.status);
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr_set[dev & 63]) {
+    cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewRing);
+    if (e != cudaSuccess) return tdb_host::fail(int(e), "cudaFuncSetAttribute(grouped few rows) failed");
+    attr_set[dev & 63] = true;
+  }
+  few_rows_kernel<MODE><<<grid, kFewThreads, kFewRing, s>>>(
+      static_cast<const uint16_t*>(A), lda, static_cast<const uint16_t*>(W), p.offsets, p.groups, p.rows, p.N, p.K, p.bias,
+      p.C, p.ldc, p.aux_out, p.ld_aux, p.status);
   tdb_host::launched(1);
   return int(cudaGetLastError());
 }

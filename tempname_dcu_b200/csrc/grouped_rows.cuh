@@ -47,10 +47,11 @@ struct RowsConfig {
   static constexpr int kBox = CG == 2 ? 64 : 32;       // token rows per TMA copy: only boxes with rows are loaded
   static constexpr int kABytes = 128 * 128;            // 128 rows of 64 bf16 or 256 e2m1
   static constexpr int kBBytes = kBRows * 128;
-  static constexpr int kBlocksB = (BT + 127) / 128;    // scale atom rows of the token operand
+  static constexpr int kBlockRows = BT == 32 ? 32 : 128;  // token rows that a scale block holds (see mx4.cu)
+  static constexpr int kBlocksB = BT / kBlockRows;        // scale blocks of a tile's token rows
   static constexpr int kSfBytes = MX4 ? 1024 * (1 + kBlocksB) : 0;
   static constexpr int kStageBytes = kABytes + kBBytes + kSfBytes;
-  static constexpr int kStages = BT == 32 ? 9 : (MX4 ? 5 : 6);
+  static constexpr int kStages = BT == 32 ? (MX4 ? 8 : 9) : (MX4 ? 5 : 6);
   static constexpr int kAccums = MX4 && BT == 256 ? 1 : 2;  // beside two of 256 columns no scale would fit
   static constexpr int kSfCols = MX4 ? 8 * (1 + kBlocksB) : 0;
   static constexpr int kUsedCols = kAccums * BT + kStages * kSfCols;
@@ -99,20 +100,20 @@ struct RowsTile {
   int g;
   int n0;            // first output column of the tile (the pair's)
   int r0, count;     // first row and number of rows
-  int block;         // MX4: first 128-row scale block of the rows
+  int block;         // MX4: first scale block of the rows
   int mma_n;         // count rounded up to 16
 };
 
 // The groups' table in shared memory: row offsets, first tile and (MX4) first
-// 128-row scale block of each group.
+// scale block of each group.
 struct RowsTable {
   const int* off;
   const int* first;
   const int* block;
 };
 
-// Tiles of a group: ceil(n / BT) of them, of equal size up to 16 rows (MX4:
-// multiples of 128 rows, where scale atoms start).
+// Tiles of a group: ceil(n / BT) of them, of equal size up to 16 rows (MX4: of
+// BT rows, since tiles start where scale blocks do).
 template <int BT, bool MX4>
 __device__ __forceinline__ int rows_per_tile(int n, int tiles) {
   if (MX4) return BT;
@@ -140,16 +141,19 @@ __device__ __forceinline__ bool load_offsets(const int* offsets, int groups, int
   return __any_sync(0xffffffffu, bad);
 }
 
-// First tile (and 128-row block) of each group, by one warp.
-template <int BT, bool BLOCKS>
+// First tile of BT rows (and first scale block of BR rows, BR > 0) of each
+// group, by one warp.
+template <int BT, int BR>
 __device__ __forceinline__ void scan_tiles(const int* off, int groups, int* first, int* block) {
+  constexpr bool BLOCKS = BR > 0;
+  constexpr int kRows = BLOCKS ? BR : 1;
   const int lane = threadIdx.x & 31;
   const int per = (groups + 31) / 32;
   int sum = 0, bsum = 0;
   for (int g = lane * per; g < min(lane * per + per, groups); ++g) {
     const int n = off[g + 1] - off[g];
     sum += (n + BT - 1) / BT;
-    bsum += (n + 127) / 128;
+    bsum += (n + kRows - 1) / kRows;
   }
   int inc = sum, binc = bsum;
 #pragma unroll
@@ -168,7 +172,7 @@ __device__ __forceinline__ void scan_tiles(const int* off, int groups, int* firs
     run += (n + BT - 1) / BT;
     if (BLOCKS) {
       block[g] = brun;
-      brun += (n + 127) / 128;
+      brun += (n + kRows - 1) / kRows;
     }
   }
   if (lane == 31) first[groups] = inc;
@@ -199,7 +203,7 @@ __device__ __forceinline__ RowsTile rows_locate(const RowsParams& p, const RowsT
   const int step = rows_per_tile<BT, MX4>(n, mt);
   r.r0 = t.off[lo] + mi * step;
   r.count = min(step, n - mi * step);  // > 0: (mt - 1) * step <= (mt - 1) * BT < n
-  r.block = MX4 ? t.block[lo] + mi * step / 128 : 0;
+  r.block = MX4 ? t.block[lo] + mi * RowsConfig<CG, BT, MX4>::kBlocksB : 0;
   r.mma_n = (r.count + 15) & ~15;
   return r;
 }
@@ -531,7 +535,7 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
     const bool bad = load_offsets(p.offsets, p.groups, p.rows, off, status);
     if (lane == 0) bars->bad_offsets = bad;
     __syncwarp();
-    if (!bad) scan_tiles<BT, MX4>(off, p.groups, first, block);
+    if (!bad) scan_tiles<BT, MX4 ? Cfg::kBlockRows : 0>(off, p.groups, first, block);
   }
   tc_fence_before();
   if (CG == 2)
@@ -574,7 +578,7 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
             load_2d<CG>(sf, &p.tmSfa, bar, 0, (t.g * p.a_blocks + ab) * p.kpairs + kb);
 #pragma unroll
             for (int j = 0; j < Cfg::kBlocksB; ++j)
-              load_2d<CG>(sf + 1024 * (1 + j), &p.tmSfb, bar, 0, (t.block + (128 * j < t.count ? j : 0)) * p.kpairs + kb);
+              load_2d<CG>(sf + 1024 * (1 + j), &p.tmSfb, bar, 0, (t.block + (Cfg::kBlockRows * j < t.count ? j : 0)) * p.kpairs + kb);
           } else {
             const int k0 = kb * BK;
             if (!kAMn) {

@@ -13,8 +13,10 @@
 // order in which tcgen05.cp 32x128b.warpx4 brings them to TMEM.  Atoms of one
 // 128-row block are consecutive along K, rounded up to an even number (a K
 // step of the product is 256 values); blocks past K hold byte 0.  With
-// offsets the rows of each group start a new 128-row block, so that a tile of
-// the grouped product starts at a block wherever its group starts.
+// offsets the rows of each group start a new block, so that a tile of the
+// grouped product starts at a block wherever its group starts; when the groups
+// hold at most 32 rows on average (block_rows) every 32 rows do, for tiles of
+// 32 rows, and the other three quarters of their atoms stay unused.
 #include <cuda_fp16.h>
 
 #include "grouped_launch.cuh"
@@ -69,8 +71,9 @@ __device__ __forceinline__ void e2m1x8_values(uint32_t q, float (&v)[8]) {
 
 struct Layout {
   const int* off;    // shared: group offsets, or null
-  const int* block;  // shared: first 128-row block of each group
+  const int* block;  // shared: first block of each group
   int groups;
+  int block_rows;        // 128, or 32 (with offsets)
   int rows, mat_blocks;  // without offsets: rows and blocks of one matrix
   // Scale block and row in it of row `r`; false for a row outside every group.
   __device__ __forceinline__ bool find(int r, int64_t& blk, int& in) const {
@@ -88,18 +91,19 @@ struct Layout {
       if (off[mid] <= r) lo = mid; else hi = mid - 1;
     }
     const int local = r - off[lo];
-    blk = block[lo] + local / 128;
-    in = local % 128;
+    blk = block[lo] + local / block_rows;
+    in = local % block_rows;
     return true;
   }
 };
 
 // Builds the layout's tables; returns false (status recorded) for bad offsets.
-__device__ __forceinline__ bool make_layout(Layout& l, const int* offsets, int groups, int rows, int mat_blocks, int* sh,
-                                            int* status) {
+__device__ __forceinline__ bool make_layout(Layout& l, const int* offsets, int groups, int rows, int mat_blocks,
+                                            int block_rows, int* sh, int* status) {
   l.off = nullptr;
   l.block = nullptr;
   l.groups = groups;
+  l.block_rows = block_rows;
   l.rows = rows;
   l.mat_blocks = mat_blocks;
   if (!offsets) return true;
@@ -110,7 +114,12 @@ __device__ __forceinline__ bool make_layout(Layout& l, const int* offsets, int g
   if (threadIdx.x < 32) {
     const bool bad = grouped::load_offsets(offsets, groups, rows, off, status);
     __syncwarp();
-    if (!bad) grouped::scan_tiles<128, true>(off, groups, first, block);
+    if (!bad) {
+      if (block_rows == 32)
+        grouped::scan_tiles<32, 32>(off, groups, first, block);
+      else
+        grouped::scan_tiles<128, 128>(off, groups, first, block);
+    }
     if (threadIdx.x == 0) bad_offsets = bad;
   }
   __syncthreads();
@@ -124,7 +133,7 @@ __device__ __forceinline__ bool make_layout(Layout& l, const int* offsets, int g
 // no division on the way (the row comes from the block, the pieces from its y).
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, int total_rows,
                                                             int K, uint8_t* __restrict__ q, uint8_t* __restrict__ sf,
-                                                            const int* offsets, int groups, int rows, int mat_blocks,
+                                                            const int* offsets, int groups, int rows, int mat_blocks, int block_rows,
                                                             int* status) {
   extern __shared__ int sh[];
   const int lane = threadIdx.x & 31;
@@ -143,7 +152,7 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __re
   uint4 in[kBatch];
   load(r, in);  // before the groups' table is built
   Layout l;
-  if (!make_layout(l, offsets, groups, rows, mat_blocks, sh, status)) return;
+  if (!make_layout(l, offsets, groups, rows, mat_blocks, block_rows, sh, status)) return;
   for (; r < total_rows; r += step, load(r, in)) {
     int64_t blk;
     int row;
@@ -181,10 +190,10 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __re
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf,
                                                               int total_rows, int K, uint16_t* __restrict__ out,
                                                               int64_t ldo, const int* offsets, int groups, int rows,
-                                                              int mat_blocks, int* status) {
+                                                              int mat_blocks, int block_rows, int* status) {
   extern __shared__ int sh[];
   Layout l;
-  if (!make_layout(l, offsets, groups, rows, mat_blocks, sh, status)) return;
+  if (!make_layout(l, offsets, groups, rows, mat_blocks, block_rows, sh, status)) return;
   const int lane = threadIdx.x & 31;
   const int pieces = (K + 255) / 256;
   const int first = blockIdx.y * kBatch;
@@ -219,10 +228,13 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __r
 
 static int64_t pairs_of(int64_t K) { return (K + 255) / 256; }
 
-// 128-row scale blocks of an operand: matrices x ceil(rows / 128), or with
-// groups the most that any offsets can need.
+// Rows per scale block of an operand with offsets.
+static int block_rows(int64_t rows, int64_t groups) { return groups > 0 && rows <= groups * 32 ? 32 : 128; }
+
+// Scale blocks of an operand: matrices x ceil(rows / 128), or with groups the
+// most that any offsets can need.
 static int64_t blocks_of(int64_t matrices, int64_t rows, int64_t groups) {
-  if (groups > 0) return rows / 128 + (rows < groups ? rows : groups);
+  if (groups > 0) return rows / block_rows(rows, groups) + (rows < groups ? rows : groups);
   return matrices * ((rows + 127) / 128);
 }
 
@@ -267,7 +279,8 @@ TDB_API int tdb_mx4_quantize(const void* x, int64_t ldx, int64_t matrices, int64
   mx4::quantize_kernel<<<mx4::grid_for(matrices * rows, K, offsets != nullptr), mx4::kThreads,
                          offsets ? size_t(3 * (groups + 1)) * 4 : 0, static_cast<cudaStream_t>(stream)>>>(
       static_cast<const uint16_t*>(x), ldx, int(matrices * rows), int(K), static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf),
-      offsets, groups, int(rows), int((rows + 127) / 128), tdb_host::status_ptr());
+      offsets, groups, int(rows), int((rows + 127) / 128), mx4::block_rows(rows, offsets ? groups : 0),
+      tdb_host::status_ptr());
   tdb_host::launched(1);
   return int(cudaGetLastError());
 }
@@ -284,14 +297,18 @@ TDB_API int tdb_mx4_dequantize(const void* q, const void* sf, int64_t matrices, 
   mx4::dequantize_kernel<<<mx4::grid_for(matrices * rows, K, offsets != nullptr), mx4::kThreads,
                            offsets ? size_t(3 * (groups + 1)) * 4 : 0, static_cast<cudaStream_t>(stream)>>>(
       static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(sf), int(matrices * rows), int(K), static_cast<uint16_t*>(out),
-      ldo, offsets, groups, int(rows), int((rows + 127) / 128), tdb_host::status_ptr());
+      ldo, offsets, groups, int(rows), int((rows + 127) / 128), mx4::block_rows(rows, offsets ? groups : 0),
+      tdb_host::status_ptr());
   tdb_host::launched(1);
   return int(cudaGetLastError());
 }
 
-// Tile code that a 4-bit product takes: 512 = up to 256 rows x 256 columns on
-// SM pairs, 128 = 128 x 128.
+// Tile code that a 4-bit product takes (groups 0: without offsets): 512 = up to
+// 256 rows x 256 columns on SM pairs, 128 = 128 x 128, 32 = 32 x 128 where the
+// scale blocks hold 32 rows.
 TDB_API int tdb_mx4_pick_tile(long long rows, int groups, int N) {
+  if (rows <= int64_t(groups > 1 ? groups : 1) * 32) return 32;
+  if (groups < 1) groups = 1;
   return rows >= int64_t(groups) * 192 && N >= 256 ? 512 : 128;
 }
 
@@ -308,9 +325,12 @@ TDB_API int tdb_mx4_gemm(const void* qx, const void* sfx, const void* qw, const 
       (reinterpret_cast<uintptr_t>(qx) | reinterpret_cast<uintptr_t>(sfx) | reinterpret_cast<uintptr_t>(qw) |
        reinterpret_cast<uintptr_t>(sfw) | reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(bias)) % 16)
     return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 product: operands must be 16-byte aligned, output rows too");
-  if (tile == 0) tile = tdb_mx4_pick_tile(rows, groups, N);
-  if (tile != 128 && tile != 512)
-    return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 product: tile must be 0, 128 or 512");
+  if (tile == 0) tile = tdb_mx4_pick_tile(rows, offsets ? groups : 0, N);
+  // tiles of 32 rows and scale blocks of 32 rows go together; up to 32 rows without offsets are one block either way
+  const bool fits = offsets ? (tile == 32) == (mx4::block_rows(rows, groups) == 32) : tile != 32 || rows <= 32;
+  if ((tile != 32 && tile != 128 && tile != 512) || !fits)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 product: tile must be 0, or one that fits the scale blocks: 32 "
+                          "for at most 32 rows per group on average, else 128 or 512");
   const int64_t pairs = mx4::pairs_of(K);
   const int64_t x_blocks = offsets ? mx4::blocks_of(1, rows, groups) : mx4::blocks_of(1, rows, 0);
   const int64_t w_blocks = (N + 127) / 128;
@@ -345,6 +365,7 @@ TDB_API int tdb_mx4_gemm(const void* qx, const void* sfx, const void* qw, const 
   p.bias = static_cast<const uint16_t*>(bias);
   p.status = tdb_host::status_ptr();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return tile == 512 ? launch_rows<2, 256, kForward, gemm::kBias, true>(p, s)
-                     : launch_rows<1, 128, kForward, gemm::kBias, true>(p, s);
+  if (tile == 512) return launch_rows<2, 256, kForward, gemm::kBias, true>(p, s);
+  if (tile == 128) return launch_rows<1, 128, kForward, gemm::kBias, true>(p, s);
+  return launch_rows<1, 32, kForward, gemm::kBias, true>(p, s);
 }

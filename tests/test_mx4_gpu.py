@@ -129,7 +129,7 @@ def test_linear(cuda, M, N, K, tile):
 
 
 @pytest.mark.parametrize("tile", [0, 128, 512])
-@pytest.mark.parametrize("counts", [[1], [0, 3, 0], [130, 0, 257, 64, 1, 0, 77], [256, 128, 384], [31, 33, 513, 127]])
+@pytest.mark.parametrize("counts", [[130], [0, 103, 0], [130, 0, 257, 64, 1, 0, 77], [256, 128, 384], [31, 33, 513, 127]])
 @pytest.mark.parametrize("N,K", [(64, 64), (264, 320), (520, 1056)])
 def test_grouped_linear(cuda, counts, N, K, tile):
     import torch
@@ -155,6 +155,36 @@ def test_grouped_linear(cuda, counts, N, K, tile):
         exact = xv[lo:hi] @ wv[g].t() + b[g].double()
         assert _within(out[lo:hi], exact, xv[lo:hi].abs() @ wv[g].abs().t() + b[g].double().abs(), K)
     assert (out[:lead] == 7).all() and (out[bounds[-1]:] == 7).all()
+    _status_ok()
+
+
+@pytest.mark.parametrize("counts", [[1], [0, 3, 0], [40, 0, 1, 70, 0, 9], [0] * 60 + [200] + [1] * 9, [32, 33, 31, 0]])
+@pytest.mark.parametrize("N,K", [(8, 32), (264, 320), (520, 1056)])
+def test_grouped_linear_with_small_groups(cuda, counts, N, K):
+    """At most 32 rows per group on average: scale blocks and tiles of 32 rows."""
+    import torch
+    from tempname_dcu_b200.ops import mx4, native
+    torch.manual_seed(N + K)
+    lead, G = 2, len(counts)
+    R = sum(counts) + lead
+    bounds = [lead]
+    for n in counts:
+        bounds.append(bounds[-1] + n)
+    assert native.lib().tdb_mx4_pick_tile(R, G, N) == (32 if R <= 32 * G else 128)
+    off = torch.tensor(bounds, dtype=torch.int32, device=cuda)
+    x = torch.randn(R, K, device=cuda).to(torch.bfloat16)
+    x[:lead] = float("nan")
+    w = (torch.randn(G, N, K, device=cuda) * 0.02).to(torch.bfloat16)
+    xv, wv = _values(x), _values(w)
+    qx, sfx = mx4.quantize(x, offsets=off)
+    assert _same(mx4.dequantize(qx, sfx, offsets=off)[lead:], xv[lead:])
+    qw, sfw = mx4.quantize(w)
+    out = torch.full((R, N), 7.0, device=cuda, dtype=torch.bfloat16)
+    mx4.grouped_linear(qx, sfx, qw, sfw, off, out=out)
+    for g in range(G):
+        lo, hi = bounds[g], bounds[g + 1]
+        assert _within(out[lo:hi], xv[lo:hi] @ wv[g].t(), xv[lo:hi].abs() @ wv[g].abs().t(), K)
+    assert (out[:lead] == 7).all()
     _status_ok()
 
 
@@ -214,6 +244,10 @@ def test_refusals(cuda):
                  lambda: mx4.linear(q, sf, qw[0], sfw, out=x)):
         with pytest.raises((ValueError, TypeError)):
             call()
+    with pytest.raises(native.NativeError):  # scale blocks of 32 rows go with tiles of 32 rows
+        mx4.grouped_linear(*mx4.quantize(x, offsets=off), qw, sfw, off, tile=128)
+    with pytest.raises(native.NativeError):
+        mx4.linear(*mx4.quantize(torch.cat([x] * 5)), qw[0].contiguous(), sfw, tile=32)
     native.clear_status()
     mx4.quantize(x, offsets=torch.tensor([0, 9, 8], dtype=torch.int32, device=cuda))
     with pytest.raises(native.NativeError):
