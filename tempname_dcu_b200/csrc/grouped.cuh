@@ -192,6 +192,8 @@ __device__ __forceinline__ void mainloop(const Params& p) {
       tmem_relinquish();
     }
   }
+  // everything above needs no memory of the kernels before this one
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (warp == 3) {
     const bool bad = load_offsets(p.offsets, p.groups, p.rows, off, status);
     if (lane == 0) bars->bad_offsets = bad;

@@ -23,7 +23,7 @@ static int launch_units(void (*kern)(P), const P& p, int threads, int64_t tiles,
   cudaGetDevice(&dev);
   LaunchState& state = states[dev & 63];
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = CG;
   attr[0].val.clusterDim.y = 1;
@@ -32,7 +32,10 @@ static int launch_units(void (*kern)(P), const P& p, int threads, int64_t tiles,
   cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
+  // the setup of the kernel may run while the kernel before it on the stream ends
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
   if (!state.ready) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, max_smem);
     if (e != cudaSuccess) return tdb_host::fail(int(e), "cudaFuncSetAttribute(grouped) failed");

@@ -531,6 +531,8 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
       tmem_relinquish();
     }
   }
+  // everything above needs no memory of the kernels before this one
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (warp == 2) {
     const bool bad = load_offsets(p.offsets, p.groups, p.rows, off, status);
     if (lane == 0) bars->bad_offsets = bad;
