@@ -8,6 +8,8 @@ namespace grouped {
 
 constexpr int kBand = 8;  // token tiles per raster band
 
+constexpr int kTwoPerSm = 113 * 1024;  // shared memory of a CTA when two share an SM
+
 struct LaunchState {
   bool ready = false;
   int pairs = 0;  // SM pairs that can be resident at once (CG = 2)
@@ -48,7 +50,8 @@ static int launch_units(void (*kern)(P), const P& p, int threads, int64_t tiles,
     }
     state.ready = true;
   }
-  int64_t units = tdb_host::grid_sms() / CG;
+  // two CTAs of the small tiles share an SM while the groups' table leaves them room
+  int64_t units = int64_t(tdb_host::grid_sms()) * (smem <= kTwoPerSm ? 2 : 1) / CG;
   if (CG == 2 && units > state.pairs) units = state.pairs;
   if (units < 1) units = 1;
   if (tiles < units) units = tiles;
@@ -60,7 +63,7 @@ static int launch_units(void (*kern)(P), const P& p, int threads, int64_t tiles,
 }
 
 template <int CG, int BT, int OP, int MODE, bool MX4>
-__global__ void __launch_bounds__(kThreads, 1) rows_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(kThreads, BT == 32 ? 2 : 1) rows_kernel(const __grid_constant__ RowsParams p) {
   rows_mainloop<CG, BT, OP, MODE, MX4>(p);
 }
 

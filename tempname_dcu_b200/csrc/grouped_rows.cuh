@@ -51,7 +51,7 @@ struct RowsConfig {
   static constexpr int kBlocksB = BT / kBlockRows;        // scale blocks of a tile's token rows
   static constexpr int kSfBytes = MX4 ? 1024 * (1 + kBlocksB) : 0;
   static constexpr int kStageBytes = kABytes + kBBytes + kSfBytes;
-  static constexpr int kStages = BT == 32 ? (MX4 ? 8 : 9) : (MX4 ? 5 : 6);
+  static constexpr int kStages = BT == 32 ? 4 : (MX4 ? 5 : 6);
   static constexpr int kAccums = MX4 && BT == 256 ? 1 : 2;  // beside two of 256 columns no scale would fit
   static constexpr int kSfCols = MX4 ? 8 * (1 + kBlocksB) : 0;
   static constexpr int kUsedCols = kAccums * BT + kStages * kSfCols;
