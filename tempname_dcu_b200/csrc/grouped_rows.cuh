@@ -398,13 +398,21 @@ struct RowsEpilogue {
     }
   }
 
-  __device__ __forceinline__ void stage(uint32_t buf, const float (&v)[32]) {
+  // bf16 fragments of a block: w[4i + m] holds rows 8i + 2(lane%4) + {0, 1} of column 8m + lane/4.
+  __device__ __forceinline__ static void pack(const float (&v)[32], uint32_t (&w)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[4 * i] = pack_bf16x2(v[4 * i], v[4 * i + 1]);
+      w[4 * i + 1] = pack_bf16x2(v[4 * i + 2], v[4 * i + 3]);
+      w[4 * i + 2] = pack_bf16x2(v[16 + 4 * i], v[16 + 4 * i + 1]);
+      w[4 * i + 3] = pack_bf16x2(v[16 + 4 * i + 2], v[16 + 4 * i + 3]);
+    }
+  }
+  __device__ __forceinline__ static void stage(uint32_t buf, const uint32_t (&w)[16]) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int i = 0; i < 4; ++i)  // rows 8i .. 8i+7
-      stmatrix_x4_trans(piece(buf, 8 * i + (lane & 7), lane >> 3), pack_bf16x2(v[4 * i], v[4 * i + 1]),
-                        pack_bf16x2(v[4 * i + 2], v[4 * i + 3]), pack_bf16x2(v[16 + 4 * i], v[16 + 4 * i + 1]),
-                        pack_bf16x2(v[16 + 4 * i + 2], v[16 + 4 * i + 3]));
+      stmatrix_x4_trans(piece(buf, 8 * i + (lane & 7), lane >> 3), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
 
   __device__ __forceinline__ void copy_rows(uint32_t buf, uint16_t* dst, int64_t ld, int rows, int col0) {
@@ -419,13 +427,10 @@ struct RowsEpilogue {
     }
   }
 
-  // v[16h' + 4i + 2h + e]: column 16h' + 8h + lane/4, row 8i + 2(lane%4) + e of
-  // the block of `valid` (<= 32 used) rows at row0.
-  __device__ __forceinline__ void block(float (&v)[32], const uint4 (&a)[4], int row0, int valid, int col0) {
-    const int lane = threadIdx.x & 31;
-    const uint32_t buf = base + uint32_t((kTwo ? 0 : (blocks & 1)) * kBuf);
-    if (blocks >= (kTwo ? 1 : 2)) {  // the bulk store that last read the buffer is done with it
-      if (lane == 0) {
+  // The bulk store that last read the buffer about to be written is done with it.
+  __device__ __forceinline__ uint32_t claim() {
+    if (blocks >= (kTwo ? 1 : 2)) {
+      if ((threadIdx.x & 31) == 0) {
         if (kTwo)
           asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         else
@@ -433,13 +438,49 @@ struct RowsEpilogue {
       }
       __syncwarp();
     }
+    return base + uint32_t((kTwo ? 0 : (blocks & 1)) * kBuf);
+  }
+
+  // Writes the staged block (kTwo: and the pre-activations staged behind it),
+  // `valid` (<= 32 used) rows from row0.
+  __device__ __forceinline__ void release(uint32_t buf, int row0, int valid, int col0) {
+    const int lane = threadIdx.x & 31;
+    if (valid >= 32) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        gemm::TmaBf16Epi<gemm::kStore>::store(&p.tmC, buf, col0, row0);
+        if (kTwo) gemm::TmaBf16Epi<gemm::kStore>::store(&p.tmAux, base + uint32_t(kBuf), col0, row0);
+      }
+    } else {  // the group's last rows: those after them belong to another group
+      __syncwarp();
+      copy_rows(buf, p.C + int64_t(row0) * p.ldc, p.ldc, valid, col0);
+      if (kTwo) copy_rows(base + uint32_t(kBuf), p.aux_out + int64_t(row0) * p.ld_aux, p.ld_aux, valid, col0);
+      __syncwarp();
+    }
+    // one bulk group per block, also where it is empty, so that claim() counts blocks
+    if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    ++blocks;
+  }
+
+  __device__ __forceinline__ void add_bias(float (&v)[32]) const {
     if (MODE == gemm::kBias || MODE == gemm::kBiasGelu) {
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] += bias[2 * (j >> 4) + ((j >> 1) & 1)];
     }
+  }
+
+  // v[16h' + 4i + 2h + e]: column 16h' + 8h + lane/4, row 8i + 2(lane%4) + e of
+  // the block of `valid` (<= 32 used) rows at row0.
+  __device__ __forceinline__ void block(float (&v)[32], const uint4 (&a)[4], int row0, int valid, int col0) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t buf = claim();
+    uint32_t w[16];
+    add_bias(v);
     if (MODE == gemm::kBiasGelu) {
       // the activation is taken of the fp32 pre-activation; only its saved copy is rounded
-      stage(base + uint32_t(kBuf), v);
+      pack(v, w);
+      stage(base + uint32_t(kBuf), w);
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = gelu(v[j]);
     }
@@ -463,23 +504,9 @@ struct RowsEpilogue {
       }
       __syncwarp();
     }
-    stage(buf, v);
-    if (valid >= 32) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) {
-        gemm::TmaBf16Epi<gemm::kStore>::store(&p.tmC, buf, col0, row0);
-        if (kTwo) gemm::TmaBf16Epi<gemm::kStore>::store(&p.tmAux, base + uint32_t(kBuf), col0, row0);
-      }
-    } else {  // the group's last rows: those after them belong to another group
-      __syncwarp();
-      copy_rows(buf, p.C + int64_t(row0) * p.ldc, p.ldc, valid, col0);
-      if (kTwo) copy_rows(base + uint32_t(kBuf), p.aux_out + int64_t(row0) * p.ld_aux, p.ld_aux, valid, col0);
-      __syncwarp();
-    }
-    // one bulk group per block, also where it is empty, so that the wait above counts blocks
-    if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-    ++blocks;
+    pack(v, w);
+    stage(buf, w);
+    release(buf, row0, valid, col0);
   }
 };
 
@@ -679,33 +706,67 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
       tc_fence_after();
       const uint32_t acc = tmem_base + (uint32_t(quarter * 32) << 16) + b * BT;
       const int chunks = (t.count + 31) / 32;
+      if constexpr (Cfg::kAccums == 1) {
+        // The only accumulator: it is read whole (rounded to bf16, half the
+        // registers) and given back to the MMAs before anything is stored.
+        uint32_t w[BT / 32][16];
+#pragma unroll
+        for (int c = 0; c < BT / 32; ++c) {
+          if (c < chunks && on) {
+            uint32_t lo[16], hi[16];
+            tmem_ld_16x256b_x4(acc + c * 32, lo);
+            tmem_ld_16x256b_x4(acc + (16u << 16) + c * 32, hi);
+            tmem_wait_ld();
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              v[j] = __uint_as_float(lo[j]);
+              v[16 + j] = __uint_as_float(hi[j]);
+            }
+            epi.add_bias(v);
+            epi.pack(v, w[c]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_leader<CG>(&bars->tmem_empty[b]);
+#pragma unroll
+        for (int c = 0; c < BT / 32; ++c) {
+          if (c < chunks && on) {
+            const uint32_t buf = epi.claim();
+            epi.stage(buf, w[c]);
+            epi.release(buf, t.r0 + 32 * c, t.count - 32 * c, col0);
+          }
+        }
+      } else {
 #pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
-        uint32_t lo[16], hi[16];
-        if (on) {
-          tmem_ld_16x256b_x4(acc + c * 32, lo);
-          tmem_ld_16x256b_x4(acc + (16u << 16) + c * 32, hi);
-          tmem_wait_ld();
-        }
-        if (c == chunks - 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_leader<CG>(&bars->tmem_empty[b]);
-        }
-        if (!on) continue;
-        float v[32];
+        for (int c = 0; c < chunks; ++c) {
+          uint32_t lo[16], hi[16];
+          if (on) {
+            tmem_ld_16x256b_x4(acc + c * 32, lo);
+            tmem_ld_16x256b_x4(acc + (16u << 16) + c * 32, hi);
+            tmem_wait_ld();
+          }
+          if (c == chunks - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_leader<CG>(&bars->tmem_empty[b]);
+          }
+          if (!on) continue;
+          float v[32];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          v[j] = __uint_as_float(lo[j]);
-          v[16 + j] = __uint_as_float(hi[j]);
-        }
-        uint4 cur[4];
-        if (MODE == gemm::kGeluBwd) {
+          for (int j = 0; j < 16; ++j) {
+            v[j] = __uint_as_float(lo[j]);
+            v[16 + j] = __uint_as_float(hi[j]);
+          }
+          uint4 cur[4];
+          if (MODE == gemm::kGeluBwd) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) cur[j] = aux[j];
-          if (c + 1 < chunks) epi.load_aux(t.r0 + 32 * (c + 1), t.count - 32 * (c + 1), col0, aux);
+            for (int j = 0; j < 4; ++j) cur[j] = aux[j];
+            if (c + 1 < chunks) epi.load_aux(t.r0 + 32 * (c + 1), t.count - 32 * (c + 1), col0, aux);
+          }
+          epi.block(v, cur, t.r0 + 32 * c, t.count - 32 * c, col0);
         }
-        epi.block(v, cur, t.r0 + 32 * c, t.count - 32 * c, col0);
       }
       ++tc;
     }

@@ -38,6 +38,12 @@ __host__ __device__ __forceinline__ int block_exponent(uint32_t abs_bits) {
   return e < -127 ? -127 : e;  // at most 126
 }
 
+__device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
   uint32_t r;
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
@@ -158,19 +164,20 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __re
     int row;
     if (!l.find(r, blk, row)) continue;
     uint8_t* dst = q + int64_t(r) * (K / 2) + k0 / 2;
-    uint8_t* scale = sf + (blk * pieces + first) * 1024 + (lane >> 4) * 512 + (row & 31) * 16 + (row >> 5) * 4;
+    uint8_t* scale =
+        sf + (blk * pieces + first) * 1024 + (lane >> 4) * 512 + (row & 31) * 16 + (row >> 5) * 4 + ((lane >> 2) & 3);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       if (first + b >= pieces) break;
       const uint32_t w[4] = {in[b].x, in[b].y, in[b].z, in[b].w};
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) top = max(top, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // largest |value| of the 32: as 16-bit integers the bits of |bf16| are ordered
+      uint32_t pair = max16x2(max16x2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                              max16x2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+      pair = max16x2(pair, __shfl_xor_sync(0xffffffffu, pair, 1));
+      pair = max16x2(pair, __shfl_xor_sync(0xffffffffu, pair, 2));
+      const uint32_t top = max(pair & 0xffffu, pair >> 16);
       const bool finite = top < 0x7f80u;
       const int e = finite ? block_exponent(top) : 128;
-      uint32_t byte = uint32_t(e + 127);
       const float inv = __uint_as_float(uint32_t(127 - e) << 23);  // 2^-e, normal for e in [-127, 126]
       float v[8];
 #pragma unroll
@@ -179,10 +186,7 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __re
         v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u) * inv;
       }
       if (k0 + b * 256 < K) *reinterpret_cast<uint32_t*>(dst + b * 128) = finite ? e2m1x8(v) : 0u;
-      // four blocks' bytes -> one word of the atom (0 past K)
-      byte |= __shfl_down_sync(0xffffffffu, byte, 4) << 8;
-      byte |= __shfl_down_sync(0xffffffffu, byte, 8) << 16;
-      if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scale + b * 1024) = byte;
+      if ((lane & 3) == 0) scale[b * 1024] = uint8_t(e + 127);  // 0 past K
     }
   }
 }
