@@ -8,6 +8,9 @@ validate_config, parameter_counts).  Additions for B200 workloads:
   (64: every shard stays a multiple of 8 columns for the GEMM/CE kernels at
   TP <= 8).  Padded logits are masked out of the softmax.
 * world_size 1 is allowed (no tensor parallelism).
+* ``experts`` / ``experts_per_token`` (default 2) -- the feed-forward block of
+  every layer becomes a mixture of that many experts (each with ``ffn`` hidden
+  units); on one rank.
 """
 from __future__ import annotations
 
@@ -21,6 +24,7 @@ SMALL_CONFIG = dict(layers=2, hidden=256, ffn=1024, heads=2, sequence=256, micro
                     vocab=1024, chunk_rows=128)
 
 HEAD_DIM = 128
+MAX_EXPERTS, MAX_EXPERTS_PER_TOKEN = 512, 16  # limits of the router (ops.moe)
 _INT_KEYS = tuple(DEFAULT_CONFIG)
 _FLOAT_DEFAULTS = (("learning_rate", 1e-4), ("weight_decay", 0.01), ("max_grad_norm", 1.0),
                    ("layer_norm_epsilon", 1e-5))
@@ -49,6 +53,14 @@ def validate_config(config, world_size=8):
         raise ValueError("world_size must be a positive integer")
     if type(c.get("pad_vocab", False)) is not bool:
         raise ValueError("pad_vocab must be a bool")
+    if "experts" in c or "experts_per_token" in c:
+        experts, chosen = c.get("experts"), c.setdefault("experts_per_token", 2)
+        if type(experts) is not int or experts <= 0 or experts % 8 or experts > MAX_EXPERTS:
+            raise ValueError(f"experts must be a multiple of 8, at most {MAX_EXPERTS}")
+        if type(chosen) is not int or not 1 <= chosen <= min(experts, MAX_EXPERTS_PER_TOKEN):
+            raise ValueError(f"experts_per_token must be 1..{MAX_EXPERTS_PER_TOKEN} and at most the number of experts")
+        if world_size != 1:
+            raise ValueError("a mixture of experts trains on one rank")
     c["padded_vocab"] = padded_vocab(c, world_size)
     for key in ("hidden", "ffn", "heads"):
         if c[key] % world_size:
@@ -90,6 +102,10 @@ def parameter_counts(config, world_size=8):
     h, f, v, s, layers = c["hidden"], c["ffn"], c["padded_vocab"], c["sequence"], c["layers"]
     logical = v * h + s * h + layers * (4 * h * h + 2 * h * f + 9 * h + f) + 2 * h
     replicated = s * h + layers * 6 * h + 2 * h
+    if "experts" in c:  # router, and per expert both weights and biases, in place of one dense block
+        e = c["experts"]
+        logical += layers * (e * h + (e - 1) * (2 * h * f + f + h))
+        replicated -= layers * h  # the second bias is the experts' own
     sharded = logical - replicated
     return dict(logical_parameters=logical, replicated_parameters=replicated, sharded_parameters=sharded,
                 parameters_per_rank=sharded // world_size + replicated, tied_embedding_head=True)
@@ -103,5 +119,7 @@ def train_flops_per_step(config, world_size=1) -> float:
     h, f, v, s, layers = c["hidden"], c["ffn"], c["padded_vocab"], c["sequence"], c["layers"]
     tokens = s * c["micro_batch"] * c["accumulation_steps"]
     matmul = layers * (4 * h * h + 2 * h * f) + v * h
+    if "experts" in c:
+        matmul += layers * ((c["experts_per_token"] - 1) * 2 * h * f + c["experts"] * h)
     attention = layers * 2 * 2 * s * h / 2  # QK^T and PV per token, causal half
     return 6.0 * tokens * matmul + 3.0 * tokens * attention

@@ -11,6 +11,12 @@ forward, per layer (x: SP rows [m/W, h])::
     ln2 = LN(x1); ln2f = AG(ln2); z = ln2f W1^T + b1; h = gelu(z)
     x2 = x1 + RS(h W2^T) + b2                                 (row-parallel, operator)
 
+with ``experts`` in the configuration (one rank) the feed-forward block is::
+
+    logits = ln2 Wr^T; r = top-k(logits); xs = dispatch(ln2, r)
+    z = xs W1_e^T + b1_e; h = gelu(z); ys = h W2_e^T + b2_e   (products grouped by expert)
+    x2 = x1 + combine(ys, r)
+
 backward mirrors it: data gradients through the transposed GEMMs (the
 collective order reversed), weight gradients accumulated directly into the
 fp32 gradient buffer by the GEMM epilogue, bias gradients by deterministic
@@ -266,6 +272,9 @@ class GPT:
             self.codec_observer.observe("attn", attn, self.P(p + "attn_weight"))
         x1 = self.operators[2 * i].forward(attn, self.P(p + "attn_weight"), self.P(p + "attn_bias"), x)
         ln2, mean2, rstd2 = K.layernorm_fwd(x1, self.P(p + "ln2_weight"), self.P(p + "ln2_bias"), eps)
+        if "experts" in c:
+            x2, routed = self._experts_fwd(p, ln2, x1)
+            return x2, (x, mean1, rstd1, ln1f, qkv, attn, lse, x1, mean2, rstd2, ln2, *routed)
         if self.agg is not None:
             h1, ln2f, z = self.agg(ln2, self.P(p + "fc1_weight"), mode=self.agg.BIAS_GELU,
                                    bias=self.P(p + "fc1_bias"))
@@ -276,6 +285,38 @@ class GPT:
             self.codec_observer.observe("mlp", h1, self.P(p + "fc2_weight"))
         x2 = self.operators[2 * i + 1].forward(h1, self.P(p + "fc2_weight"), self.P(p + "fc2_bias"), x1)
         return x2, (x, mean1, rstd1, ln1f, qkv, attn, lse, x1, mean2, rstd2, ln2f, z, h1)
+
+    def _experts_fwd(self, p, ln2, x1):
+        """x1 + the experts' weighted sum; also what the backward needs (in the
+        places of a dense block's z and h1)."""
+        from ..ops import gemm as G
+        from ..ops import grouped, moe
+        logits = G.gemm(ln2, self.P(p + "router_weight"), mode=G.ACC_F32)  # fp32: near ties decide the routing
+        r = moe.route(logits, self.config["experts_per_token"])
+        xs = moe.dispatch(ln2, r)
+        h1, z = grouped.linear_gelu(xs, self.P(p + "fc1_weight"), r.offsets, self.P(p + "fc1_bias"))
+        ys = grouped.linear(h1, self.P(p + "fc2_weight"), r.offsets, self.P(p + "fc2_bias"))
+        return moe.combine(ys, r, residual=x1), (z, (logits, r, xs, h1, ys))
+
+    def _experts_bwd(self, p, dx2, ln2, z, routed, acc):
+        """Gradient of the block with respect to ln2; parameter gradients are
+        written or added (``acc``)."""
+        import torch
+        from ..ops import gemm as G
+        from ..ops import grouped, moe
+        logits, r, xs, h1, ys = routed
+        off = r.offsets
+        dys, dweights = moe.combine_bwd(dx2, ys, r)
+        grouped.bias_grad(dys, off, self.Gr(p + "fc2_bias"), accumulate=acc)
+        grouped.weight_grad(dys, h1, off, self.Gr(p + "fc2_weight"), accumulate=acc)
+        dz = grouped.matmul_nt(dys, self.P(p + "fc2_weight"), off, gelu_pre=z)
+        grouped.bias_grad(dz, off, self.Gr(p + "fc1_bias"), accumulate=acc)
+        grouped.weight_grad(dz, xs, off, self.Gr(p + "fc1_weight"), accumulate=acc)
+        dxs = grouped.matmul_nt(dz, self.P(p + "fc1_weight"), off)
+        dlogits = moe.route_bwd(logits, r, dweights,
+                                out=torch.empty(logits.shape, dtype=torch.bfloat16, device=logits.device))
+        G.weight_grad(dlogits, ln2, self.Gr(p + "router_weight"), accumulate=acc)
+        return moe.dispatch_bwd(dxs, r, residual=G.matmul_nt(dlogits, self.P(p + "router_weight")))
 
     def forward_backward(self, tokens, targets, loss_acc=None, *, grad_scale=None, loss_scale=None,
                          overwrite_grads=False):
@@ -385,19 +426,22 @@ class GPT:
         c, p = self.config, f"layers.{i}."
         x, mean1, rstd1, ln1f, qkv, attn, lse, x1, mean2, rstd2, ln2f, z, h1 = saved
         keep = []  # operands of weight / bias gradients still running on the overlap stream
-        # FC2 (row-parallel): x2 = x1 + RS(h1 W2^T) + b2
-        self._colsum(dx2, p + "fc2_bias", acc, keep)
-        if self.agg is not None:
-            with self._fused_share():
-                dz, dyf = self.agg(dx2, self.P(p + "fc2_weight"), b_mn=True, mode=self.agg.GELU_BWD, aux=z)
+        if "experts" in c:
+            dln2 = self._experts_bwd(p, dx2, ln2f, z, h1, acc)
         else:
-            dyf = self.tp.gather(dx2)
-            dz = G.matmul_nt(dyf, self.P(p + "fc2_weight"), gelu_pre=z)
-        self._wgrad(dyf, h1, p + "fc2_weight", keep, acc)
-        # FC1 (column-parallel)
-        self._colsum(dz, p + "fc1_bias", acc, keep)
-        self._wgrad(dz, ln2f, p + "fc1_weight", keep, acc)
-        dln2 = self._dgrad_rs(dz, self.P(p + "fc1_weight"))
+            # FC2 (row-parallel): x2 = x1 + RS(h1 W2^T) + b2
+            self._colsum(dx2, p + "fc2_bias", acc, keep)
+            if self.agg is not None:
+                with self._fused_share():
+                    dz, dyf = self.agg(dx2, self.P(p + "fc2_weight"), b_mn=True, mode=self.agg.GELU_BWD, aux=z)
+            else:
+                dyf = self.tp.gather(dx2)
+                dz = G.matmul_nt(dyf, self.P(p + "fc2_weight"), gelu_pre=z)
+            self._wgrad(dyf, h1, p + "fc2_weight", keep, acc)
+            # FC1 (column-parallel)
+            self._colsum(dz, p + "fc1_bias", acc, keep)
+            self._wgrad(dz, ln2f, p + "fc1_weight", keep, acc)
+            dln2 = self._dgrad_rs(dz, self.P(p + "fc1_weight"))
         dx1 = K.layernorm_bwd(x1, self.P(p + "ln2_weight"), mean2, rstd2, dln2, self.Gr(p + "ln2_weight"),
                               self.Gr(p + "ln2_bias"), ln_scratch, dres=dx2, accumulate=acc)
         # attention out (row-parallel)

@@ -57,6 +57,18 @@ def gpt_param_specs(c, world):
             ParamSpec(p + "qkv_bias", (3 * h // world,), False, False, "zeros"),
             ParamSpec(p + "attn_weight", (h, h // world), False, True, "normal", out_std),
             ParamSpec(p + "attn_bias", (h,), True, False, "zeros"),
+        ]
+        if "experts" in c:  # one rank (validate_config): the experts' matrices stacked
+            e = c["experts"]
+            specs += [
+                ParamSpec(p + "router_weight", (e, h), False, True, "normal"),
+                ParamSpec(p + "fc1_weight", (e, f, h), False, True, "normal"),
+                ParamSpec(p + "fc1_bias", (e, f), False, False, "zeros"),
+                ParamSpec(p + "fc2_weight", (e, h, f), False, True, "normal", out_std),
+                ParamSpec(p + "fc2_bias", (e, h), False, False, "zeros"),
+            ]
+            continue
+        specs += [
             ParamSpec(p + "fc1_weight", (f // world, h), False, True, "normal"),
             ParamSpec(p + "fc1_bias", (f // world,), False, False, "zeros"),
             ParamSpec(p + "fc2_weight", (h, f // world), False, True, "normal", out_std),

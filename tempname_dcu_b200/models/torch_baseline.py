@@ -99,6 +99,8 @@ class BaselineTrainer:
         self.world = dist.get_world_size(group) if dist.is_initialized() else 1
         self.rank = dist.get_rank(group) if dist.is_initialized() else 0
         c = self.config = validate_config(config, self.world)
+        if "experts" in c:
+            raise ValueError("the PyTorch baseline has a dense feed-forward block")
         self.device = torch.device("cpu") if device == "cpu" else torch.device(device, torch.cuda.current_device())
         h, f, L, W = c["hidden"], c["ffn"], c["layers"], self.world
         gen = torch.Generator(device=self.device).manual_seed(seed + 1000003 * self.rank)
