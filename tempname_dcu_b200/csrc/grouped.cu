@@ -50,7 +50,8 @@ static int pick_tile(int op, int64_t rows, int groups, int M, int N) {
 template <int MODE>
 static int launch_few(const RowsParams& p, const void* A, int64_t lda, const void* W, cudaStream_t s) {
   const int64_t units = int64_t((p.N + 15) / 16) * (p.rows < p.groups ? p.rows : p.groups);
-  const int64_t most = int64_t(tdb_host::sm_count()) * 2;
+  const int sms = tdb_host::grid_sms();
+  const int64_t most = sms == tdb_host::sm_count() ? int64_t(sms) * 2 : sms;
   const unsigned grid = unsigned(units < most ? units : most);
   static bool attr_set[64] = {false};
   int dev = 0;

@@ -50,8 +50,9 @@ static int launch_units(void (*kern)(P), const P& p, int threads, int64_t tiles,
     }
     state.ready = true;
   }
-  // two CTAs of the small tiles share an SM while the groups' table leaves them room
-  int64_t units = int64_t(tdb_host::grid_sms()) * (smem <= kTwoPerSm ? 2 : 1) / CG;
+  int64_t units = tdb_host::grid_sms() / CG;
+  // two CTAs of the small tiles share an SM while the groups' table leaves them room and the caller has the whole GPU
+  if (smem <= kTwoPerSm && tdb_host::grid_sms() == tdb_host::sm_count()) units *= 2;
   if (CG == 2 && units > state.pairs) units = state.pairs;
   if (units < 1) units = 1;
   if (tiles < units) units = tiles;

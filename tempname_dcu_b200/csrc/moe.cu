@@ -341,20 +341,12 @@ __global__ void __launch_bounds__(kThreads) route_bwd_kernel(const T* __restrict
   const float dot = warp_sum(w * dw);
   O* o = out + t * ld_out;
   if (normalize) {
-    const float g = w * (dw - dot);
-    float r[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) r[i] = 0.f;
-    for (int j = 0; j < k; ++j) {
-      const int at = __shfl_sync(0xffffffffu, id, j);
-      const float gj = __shfl_sync(0xffffffffu, g, j);
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        if (at == i * 32 + lane) r[i] = gj;
-    }
+    // zeros, then the chosen ones over them (__syncwarp orders the two stores)
 #pragma unroll
     for (int i = 0; i < NP; ++i)
-      if (i * 32 + lane < E) store_logit(o + i * 32 + lane, r[i]);
+      if (i * 32 + lane < E) store_logit(o + i * 32 + lane, 0.f);
+    __syncwarp();
+    if (uint32_t(id) < uint32_t(E)) store_logit(o + id, w * (dw - dot));
     return;
   }
   float z[NP], d[NP], top = -INFINITY;

@@ -48,6 +48,7 @@ def _rows(t, rows, cols, device, what):
     ld, step = t.stride() if t.dim() == 2 else (0, 0)
     if rows <= 1:
         ld = cols
+    _need(rows < 2 ** 31 and cols < 2 ** 31, f"{what} must have fewer than 2^31 rows and columns")
     _need(t.shape == (rows, cols) and step == 1 and ld >= cols and t.get_device() == device,
           f"{what} must be [{rows}, {cols}] with contiguous rows that do not overlap, on the operands' device")
     return ld

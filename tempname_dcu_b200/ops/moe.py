@@ -81,6 +81,8 @@ class Routing:
                   "offsets, order and slots must be contiguous int32 vectors")
             _need(t.get_device() == index, "the tensors must be on one device")
         _need(weights.get_device() == index, "the tensors must be on one device")
+        _need(ids.shape[1] >= 1 and ids.shape[1] <= MAX_TOP_K and ids.numel() < 2 ** 31,
+              f"1..{MAX_TOP_K} choices per token, fewer than 2^31 in all")
         _need(self.slots.numel() == ids.numel() and self.order.numel() == ids.numel() and self.offsets.numel() > 1,
               "order and slots must have tokens * k entries, offsets experts + 1")
 
@@ -126,7 +128,8 @@ def _columns(t, what):
     """(rows, columns, device) of a row operand."""
     _need(t.dim() == 2 and t.is_cuda, f"{what} must be a matrix on a CUDA device")
     rows, cols = t.shape
-    _need(cols > 0 and cols % 8 == 0, f"{what} needs a multiple of 8 columns")
+    _need(cols > 0 and cols % 8 == 0 and cols < 2 ** 31 and rows < 2 ** 31,
+          f"{what} needs a multiple of 8 columns, and fewer than 2^31 rows and columns")
     return rows, cols, t.get_device()
 
 
@@ -137,6 +140,7 @@ def _logits(logits, what="logits"):
     _need(bf16 or logits.dtype is torch.float32, f"{what} must be fp32 or bf16")
     tokens, experts = logits.shape
     _need(1 <= experts <= MAX_EXPERTS, f"the number of experts must be 1..{MAX_EXPERTS}")
+    _need(tokens < 2 ** 31 // MAX_TOP_K, "at most 2^27 tokens")
     ld, step = logits.stride()
     if tokens <= 1:
         ld = experts

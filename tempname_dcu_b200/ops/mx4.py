@@ -65,7 +65,8 @@ def _operand(q, sf, groups, device, what):
     shape = q.shape
     matrices = shape[0] if len(shape) == 3 else 1
     rows, K = shape[-2], 2 * shape[-1]
-    _need(K > 0 and K % 32 == 0, f"{what}: K must be a positive multiple of 32")
+    _need(K > 0 and K % 32 == 0 and K < 2 ** 26 and rows < 2 ** 31,
+          f"{what}: K must be a positive multiple of 32 below 2^26, and rows fewer than 2^31")
     _need(sf.dtype is torch.uint8 and sf.is_contiguous() and sf.get_device() == device and
           sf.numel() >= scale_bytes(rows, K, groups, matrices),
           f"the scales of {what} must be the uint8 buffer that quantize wrote for these rows (and offsets)")
