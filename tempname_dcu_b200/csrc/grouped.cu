@@ -32,19 +32,22 @@ static int launch_rows_tile(int tile, const RowsParams& p, cudaStream_t s) {
 
 // Tile of a call.  Forward with few rows: the streaming kernel (16) while the
 // 128-column tiles of the groups that can have rows would leave SMs idle (two
-// experts of 4096 x 16384 and one token: 52 us against 76; 16384 x 4096, 256
-// tiles: 53 against 50).  Otherwise up to 256 rows x 256 columns on SM pairs
-// (512), 128 x 128 (128) or 32 x 128 (32), the smallest whose rows hold an
-// average group (8 groups of 16384 x 4096 with 64 rows each: 272 us with 32,
-// 195 with 128, 197 with 512; with 512 rows each 596 with 128, 375 with 512).
+// experts of 4096 x 16384 and one token: 52 us against 80; 16384 x 4096, 256
+// tiles: 53 against 47).  Weight gradient: SM pairs (512) when the sums are long
+// enough to hide their larger tiles' output (8 groups of 4096 x 4096 with 256
+// rows each 126 us with 128, 137 with 512; 384: 168 and 140; 1024: 374 and 249)
+// and the tiles fill half of the pairs (8 of 512 x 512 with 1024 rows each: 11.5
+// and 14.0).
 static int pick_tile(int op, int64_t rows, int groups, int M, int N) {
-  if (op == kWeightGrad) return M >= 256 && N >= 256 ? 512 : 128;
+  if (op == kWeightGrad) {
+    const int64_t tiles = int64_t(groups) * ((M + 255) / 256) * ((N + 255) / 256);
+    return M >= 256 && N >= 256 && rows >= int64_t(groups) * 320 && fills(tiles, tdb_host::sm_count() / 2) ? 512 : 128;
+  }
   if (op == kForward && rows <= kFewRows) {
     const int64_t tiles = (rows < groups ? rows : groups) * ((N + 127) / 128);
     if (tiles * 5 < int64_t(tdb_host::sm_count()) * 4) return 16;
   }
-  if (rows <= int64_t(groups) * 32) return 32;
-  return rows >= int64_t(groups) * 192 && N >= 256 ? 512 : 128;
+  return pick_rows_tile(rows, groups, N);
 }
 
 template <int MODE>

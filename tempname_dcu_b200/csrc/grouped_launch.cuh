@@ -80,6 +80,25 @@ static int launch_rows(const RowsParams& p, cudaStream_t stream) {
                           Cfg::smem_bytes(kMaxGroups), state, stream);
 }
 
+// Whether `tiles` CTAs' or pairs' worth of work fills at least half of `slots`.
+static bool fills(int64_t tiles, int64_t slots) { return 2 * tiles >= slots; }
+
+// Tile of a product of `rows` rows in `groups` groups with N output columns:
+// 512 = up to 256 rows x 256 columns on SM pairs, 128 = 128 x 128, 32 = 32 x
+// 128; the largest that an average group's rows nearly fill and that has tiles
+// enough.  Measured with 8 groups, microseconds with 32 / 128 / 512: 4096 x 4096
+// with 32 rows each 47 / 50 / 51, 96: 70 / 53 / 55, 128: 86 / 56 / 55, 160:
+// 103 / 87 / 58, 384: 213 / 154 / 102; 512 x 2048, where large tiles leave SMs
+// idle, with 64 rows each 13.1 / 14.3 / 14.8, 160: 13.8 / 15.4 / 17.0.
+static int pick_rows_tile(int64_t rows, int64_t groups, int N) {
+  const int64_t used = rows < groups ? rows : groups;
+  const int64_t average = used > 0 ? (rows + used - 1) / used : 0;
+  const int sms = tdb_host::sm_count();
+  if (average >= 128 && N >= 256 && fills(used * ((average + 255) / 256) * ((N + 255) / 256), sms / 2)) return 512;
+  if (average > 32 && fills(used * ((average + 127) / 128) * ((N + 127) / 128), sms)) return 128;
+  return 32;
+}
+
 // bf16 output rows in blocks of 32 rows x 32 columns.
 static int make_output_map(CUtensorMap* map, const void* C, int rows, int N, int64_t ldc) {
   return tdb_host::make_tmap_2d(map, C, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(N), uint64_t(rows), uint64_t(ldc),

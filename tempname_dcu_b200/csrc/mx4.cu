@@ -307,13 +307,15 @@ TDB_API int tdb_mx4_dequantize(const void* q, const void* sf, int64_t matrices, 
   return int(cudaGetLastError());
 }
 
-// Tile code that a 4-bit product takes (groups 0: without offsets): 512 = up to
-// 256 rows x 256 columns on SM pairs, 128 = 128 x 128, 32 = 32 x 128 where the
-// scale blocks hold 32 rows.
+// Tile code that a 4-bit product takes (groups 0: without offsets).  32 where
+// the scale blocks hold 32 rows, else as pick_rows_tile says, but not below 128
+// (4096 rows x 16384 x 4096: 229 us with 128, 148 with 512; 512 x 4096 x 4096:
+// 12.5 and 16.0).
 TDB_API int tdb_mx4_pick_tile(long long rows, int groups, int N) {
-  if (rows <= int64_t(groups > 1 ? groups : 1) * 32) return 32;
   if (groups < 1) groups = 1;
-  return rows >= int64_t(groups) * 192 && N >= 256 ? 512 : 128;
+  if (rows <= int64_t(groups) * 32) return 32;
+  const int tile = tdb::grouped::pick_rows_tile(rows, groups, N);
+  return tile < 128 ? 128 : tile;
 }
 
 // C[r, :] = x[r] w_g^T (+ bias[g]) for the rows r of group g, x and w as
