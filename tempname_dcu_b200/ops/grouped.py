@@ -36,11 +36,6 @@ native.register("tdb_grouped_bias_grad", [V, I64, V, I, V, I, I, I, V])
 MAX_GROUPS = 1024
 
 
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
-
-
 def _rows(t, rows, cols, device, what):
     """Row stride of a bf16 [rows, cols] matrix with contiguous rows."""
     if t.dtype is not torch.bfloat16:
@@ -48,43 +43,51 @@ def _rows(t, rows, cols, device, what):
     ld, step = t.stride() if t.dim() == 2 else (0, 0)
     if rows <= 1:
         ld = cols
-    _need(rows < 2 ** 31 and cols < 2 ** 31, f"{what} must have fewer than 2^31 rows and columns")
-    _need(t.shape == (rows, cols) and step == 1 and ld >= cols and t.get_device() == device,
-          f"{what} must be [{rows}, {cols}] with contiguous rows that do not overlap, on the operands' device")
+    if not (rows < 2 ** 31 and cols < 2 ** 31):
+        raise ValueError(f"{what} must have fewer than 2^31 rows and columns")
+    if not (t.shape == (rows, cols) and step == 1 and ld >= cols and t.get_device() == device):
+        raise ValueError(f"{what} must be [{rows}, {cols}] with contiguous rows that do not overlap, on the "
+                         f"operands' device")
     return ld
 
 
 def _offsets(offsets, groups, device):
-    _need(offsets.dtype is torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and
-          offsets.get_device() == device, "offsets must be a contiguous int32 vector on the operands' device")
-    _need(offsets.numel() == groups + 1, f"offsets must have groups + 1 = {groups + 1} entries")
-    _need(1 <= groups <= MAX_GROUPS, f"the number of groups must be 1..{MAX_GROUPS}")
+    if not (offsets.dtype is torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and
+            offsets.get_device() == device):
+        raise ValueError("offsets must be a contiguous int32 vector on the operands' device")
+    if not (offsets.numel() == groups + 1):
+        raise ValueError(f"offsets must have groups + 1 = {groups + 1} entries")
+    if not (1 <= groups <= MAX_GROUPS):
+        raise ValueError(f"the number of groups must be 1..{MAX_GROUPS}")
 
 
 def _fp32(out, shape, device, what):
     if out.dtype is not torch.float32:
         raise TypeError(f"{what} is fp32")
-    _need(out.shape == shape and out.is_contiguous() and out.get_device() == device,
-          f"out_f32 must be contiguous {list(shape)} on the operands' device")
+    if not (out.shape == shape and out.is_contiguous() and out.get_device() == device):
+        raise ValueError(f"out_f32 must be contiguous {list(shape)} on the operands' device")
 
 
 def _gemm(a, w, offsets, data_grad, mode, out, bias, aux, aux_out, tile):
-    _need(a.dim() == 2 and a.is_cuda, "the row operand must be a matrix on a CUDA device")
+    if not (a.dim() == 2 and a.is_cuda):
+        raise ValueError("the row operand must be a matrix on a CUDA device")
     index = a.get_device()
     if w.dtype is not torch.bfloat16:
         raise TypeError("w must be bf16")
-    _need(w.dim() == 3 and w.is_contiguous() and w.get_device() == index,
-          "w must be a contiguous [groups, N, K] tensor on the operands' device")
+    if not (w.dim() == 3 and w.is_contiguous() and w.get_device() == index):
+        raise ValueError("w must be a contiguous [groups, N, K] tensor on the operands' device")
     groups, N, K = w.shape
     if data_grad:
         N, K = K, N
     rows = a.shape[0]
-    _need(N > 0 and K > 0 and N % 8 == 0 and K % 8 == 0, "N and K must be positive multiples of 8")
+    if not (N > 0 and K > 0 and N % 8 == 0 and K % 8 == 0):
+        raise ValueError("N and K must be positive multiples of 8")
     lda = _rows(a, rows, K, index, "dy" if data_grad else "x")
     _offsets(offsets, groups, index)
     if bias is not None:
-        _need(bias.dtype is torch.bfloat16 and bias.shape == (groups, N) and bias.is_contiguous() and
-              bias.get_device() == index, f"bias must be contiguous bf16 [{groups}, {N}] on the operands' device")
+        if not (bias.dtype is torch.bfloat16 and bias.shape == (groups, N) and bias.is_contiguous() and
+                bias.get_device() == index):
+            raise ValueError(f"bias must be contiguous bf16 [{groups}, {N}] on the operands' device")
     if out is None:
         out = a.new_empty((rows, N))
     ldc = _rows(out, rows, N, index, "out")
@@ -108,7 +111,8 @@ def linear(x, w, offsets, bias=None, out=None, tile=0):
 def linear_gelu(x, w, offsets, bias=None, pre_out=None, out=None, tile=0):
     """Returns (gelu(z), z) with z = x[r] @ w[g]^T (+ bias[g]) from one kernel.
     The activation is taken of the fp32 sum; z is its bf16 rounding."""
-    _need(x.dim() == 2 and w.dim() == 3, "x must be [R, K] and w [groups, N, K]")
+    if not (x.dim() == 2 and w.dim() == 3):
+        raise ValueError("x must be [R, K] and w [groups, N, K]")
     if pre_out is None:
         pre_out = x.new_empty((x.shape[0], w.shape[1]))
     if out is None:
@@ -127,13 +131,15 @@ def matmul_nt(dy, w, offsets, out=None, gelu_pre=None, tile=0):
 def weight_grad(dy, x, offsets, out_f32=None, accumulate=True, tile=0):
     """``out_f32[g] (+)= dy_g^T @ x_g`` in fp32, [groups, N, K]; an empty group
     adds nothing (or gets zeros without ``accumulate``)."""
-    _need(dy.dim() == 2 and x.dim() == 2 and dy.is_cuda, "dy and x must be matrices on a CUDA device")
+    if not (dy.dim() == 2 and x.dim() == 2 and dy.is_cuda):
+        raise ValueError("dy and x must be matrices on a CUDA device")
     index = dy.get_device()
     rows, N = dy.shape
     K = x.shape[1]
     groups = offsets.numel() - 1
     _offsets(offsets, groups, index)
-    _need(N > 0 and K > 0 and N % 8 == 0 and K % 8 == 0, "N and K must be positive multiples of 8")
+    if not (N > 0 and K > 0 and N % 8 == 0 and K % 8 == 0):
+        raise ValueError("N and K must be positive multiples of 8")
     ldy = _rows(dy, rows, N, index, "dy")
     ldx = _rows(x, rows, K, index, "x")
     if out_f32 is None:
@@ -149,12 +155,14 @@ def weight_grad(dy, x, offsets, out_f32=None, accumulate=True, tile=0):
 @native.on_tensor_device
 def bias_grad(dy, offsets, out_f32=None, accumulate=True):
     """``out_f32[g] (+)= `` the sum of dy's rows of group g, fp32 [groups, N]."""
-    _need(dy.dim() == 2 and dy.is_cuda, "dy must be a matrix on a CUDA device")
+    if not (dy.dim() == 2 and dy.is_cuda):
+        raise ValueError("dy must be a matrix on a CUDA device")
     index = dy.get_device()
     rows, N = dy.shape
     groups = offsets.numel() - 1
     _offsets(offsets, groups, index)
-    _need(N > 0 and N % 8 == 0, "N must be a positive multiple of 8")
+    if not (N > 0 and N % 8 == 0):
+        raise ValueError("N must be a positive multiple of 8")
     ldy = _rows(dy, rows, N, index, "dy")
     if out_f32 is None:
         out_f32 = torch.empty((groups, N), dtype=torch.float32, device=dy.device)

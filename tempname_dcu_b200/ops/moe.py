@@ -45,11 +45,6 @@ MAX_EXPERTS = 512
 MAX_TOP_K = 16
 
 
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
-
-
 @dataclass(frozen=True)
 class Routing:
     """A batch's choices of experts, grouped.
@@ -72,19 +67,21 @@ class Routing:
 
     def __post_init__(self):
         ids, weights, index = self.ids, self.weights, self.ids.get_device()
-        _need(ids.dim() == 2 and ids.dtype is torch.int32 and ids.is_contiguous(),
-              "ids must be contiguous int32 [tokens, k]")
-        _need(weights.shape == ids.shape and weights.dtype is torch.float32 and weights.is_contiguous(),
-              "weights must be contiguous fp32 [tokens, k]")
+        if not (ids.dim() == 2 and ids.dtype is torch.int32 and ids.is_contiguous()):
+            raise ValueError("ids must be contiguous int32 [tokens, k]")
+        if not (weights.shape == ids.shape and weights.dtype is torch.float32 and weights.is_contiguous()):
+            raise ValueError("weights must be contiguous fp32 [tokens, k]")
         for t in (self.offsets, self.order, self.slots):
-            _need(t.dtype is torch.int32 and t.dim() == 1 and t.is_contiguous(),
-                  "offsets, order and slots must be contiguous int32 vectors")
-            _need(t.get_device() == index, "the tensors must be on one device")
-        _need(weights.get_device() == index, "the tensors must be on one device")
-        _need(ids.shape[1] >= 1 and ids.shape[1] <= MAX_TOP_K and ids.numel() < 2 ** 31,
-              f"1..{MAX_TOP_K} choices per token, fewer than 2^31 in all")
-        _need(self.slots.numel() == ids.numel() and self.order.numel() == ids.numel() and self.offsets.numel() > 1,
-              "order and slots must have tokens * k entries, offsets experts + 1")
+            if not (t.dtype is torch.int32 and t.dim() == 1 and t.is_contiguous()):
+                raise ValueError("offsets, order and slots must be contiguous int32 vectors")
+            if not (t.get_device() == index):
+                raise ValueError("the tensors must be on one device")
+        if not (weights.get_device() == index):
+            raise ValueError("the tensors must be on one device")
+        if not (ids.shape[1] >= 1 and ids.shape[1] <= MAX_TOP_K and ids.numel() < 2 ** 31):
+            raise ValueError(f"1..{MAX_TOP_K} choices per token, fewer than 2^31 in all")
+        if not (self.slots.numel() == ids.numel() and self.order.numel() == ids.numel() and self.offsets.numel() > 1):
+            raise ValueError("order and slots must have tokens * k entries, offsets experts + 1")
 
     @property
     def tokens(self):
@@ -109,7 +106,8 @@ def _routing(ids, weights, offsets, order, slots, normalize):
 def _check_routing(r, device):
     """(tokens, k) of a routing on the device of a call's tensors."""
     ids = r.ids
-    _need(ids.get_device() == device, "the routing must be on the tensors' device")
+    if not (ids.get_device() == device):
+        raise ValueError("the routing must be on the tensors' device")
     return ids.shape
 
 
@@ -118,33 +116,40 @@ def _rows(t, rows, cols, device, what):
     ld, step = t.stride() if t.dim() == 2 else (0, 0)
     if rows <= 1:
         ld = cols
-    _need(t.dtype is torch.bfloat16 and t.shape == (rows, cols) and step == 1 and ld >= cols and
-          t.get_device() == device,
-          f"{what} must be bf16 [{rows}, {cols}] with contiguous rows that do not overlap, on the tensors' device")
+    if not (t.dtype is torch.bfloat16 and t.shape == (rows, cols) and step == 1 and ld >= cols and
+            t.get_device() == device):
+        raise ValueError(f"{what} must be bf16 [{rows}, {cols}] with contiguous rows that do not overlap, on the "
+                         f"tensors' device")
     return ld
 
 
 def _columns(t, what):
     """(rows, columns, device) of a row operand."""
-    _need(t.dim() == 2 and t.is_cuda, f"{what} must be a matrix on a CUDA device")
+    if not (t.dim() == 2 and t.is_cuda):
+        raise ValueError(f"{what} must be a matrix on a CUDA device")
     rows, cols = t.shape
-    _need(cols > 0 and cols % 8 == 0 and cols < 2 ** 31 and rows < 2 ** 31,
-          f"{what} needs a multiple of 8 columns, and fewer than 2^31 rows and columns")
+    if not (cols > 0 and cols % 8 == 0 and cols < 2 ** 31 and rows < 2 ** 31):
+        raise ValueError(f"{what} needs a multiple of 8 columns, and fewer than 2^31 rows and columns")
     return rows, cols, t.get_device()
 
 
 def _logits(logits, what="logits"):
     """(tokens, experts, row stride, is bf16, device)."""
-    _need(logits.dim() == 2 and logits.is_cuda, f"{what} must be a [tokens, experts] matrix on a CUDA device")
+    if not (logits.dim() == 2 and logits.is_cuda):
+        raise ValueError(f"{what} must be a [tokens, experts] matrix on a CUDA device")
     bf16 = logits.dtype is torch.bfloat16
-    _need(bf16 or logits.dtype is torch.float32, f"{what} must be fp32 or bf16")
+    if not (bf16 or logits.dtype is torch.float32):
+        raise ValueError(f"{what} must be fp32 or bf16")
     tokens, experts = logits.shape
-    _need(1 <= experts <= MAX_EXPERTS, f"the number of experts must be 1..{MAX_EXPERTS}")
-    _need(tokens < 2 ** 31 // MAX_TOP_K, "at most 2^27 tokens")
+    if not (1 <= experts <= MAX_EXPERTS):
+        raise ValueError(f"the number of experts must be 1..{MAX_EXPERTS}")
+    if not (tokens < 2 ** 31 // MAX_TOP_K):
+        raise ValueError("at most 2^27 tokens")
     ld, step = logits.stride()
     if tokens <= 1:
         ld = experts
-    _need((step == 1 or experts == 1) and ld >= experts, f"{what} needs contiguous rows that do not overlap")
+    if not ((step == 1 or experts == 1) and ld >= experts):
+        raise ValueError(f"{what} needs contiguous rows that do not overlap")
     return tokens, experts, ld, int(bf16), logits.get_device()
 
 
@@ -156,8 +161,8 @@ def route(logits, top_k, normalize=True):
     index first; NaN counts as the largest) with softmax weights over the
     chosen ones (``normalize``) or over all experts."""
     tokens, experts, ld, bf16, index = _logits(logits)
-    _need(type(top_k) is int and 1 <= top_k <= min(experts, MAX_TOP_K),
-          f"top_k must be 1..{MAX_TOP_K} and at most the number of experts")
+    if not (type(top_k) is int and 1 <= top_k <= min(experts, MAX_TOP_K)):
+        raise ValueError(f"top_k must be 1..{MAX_TOP_K} and at most the number of experts")
     normalize = bool(normalize)
     dev = logits.device
     weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
@@ -183,14 +188,18 @@ def route_bwd(logits, routing, dweights, out=None):
     normalised."""
     tokens, experts, ld, bf16, index = _logits(logits)
     shape = _check_routing(routing, index)
-    _need(shape[0] == tokens and routing.experts == experts, "routing and logits have different sizes")
-    _need(dweights.shape == shape and dweights.dtype is torch.float32 and dweights.is_contiguous() and
-          dweights.get_device() == index, "dweights must be contiguous fp32 [tokens, k] on the logits' device")
+    if not (shape[0] == tokens and routing.experts == experts):
+        raise ValueError("routing and logits have different sizes")
+    if not (dweights.shape == shape and dweights.dtype is torch.float32 and dweights.is_contiguous() and
+            dweights.get_device() == index):
+        raise ValueError("dweights must be contiguous fp32 [tokens, k] on the logits' device")
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
-    _need(out.shape == (tokens, experts), "out must be [tokens, experts]")
+    if not (out.shape == (tokens, experts)):
+        raise ValueError("out must be [tokens, experts]")
     _, _, ld_out, out_bf16, out_index = _logits(out, "out")
-    _need(out_index == index, "out must be on the logits' device")
+    if not (out_index == index):
+        raise ValueError("out must be on the logits' device")
     native.check(native.lib().tdb_moe_route_bwd(logits.data_ptr(), bf16, ld, tokens, experts, shape[1],
                                                 bool(routing.normalize), routing.ids.data_ptr(),
                                                 routing.weights.data_ptr(), dweights.data_ptr(), out.data_ptr(),
@@ -203,7 +212,8 @@ def dispatch(x, routing, out=None):
     """Rows grouped by expert: ``out[slots[t*k + j]] = x[t]``, [tokens*k, H]."""
     tokens, H, index = _columns(x, "x")
     shape = _check_routing(routing, index)
-    _need(shape[0] == tokens, "routing and x have different numbers of tokens")
+    if not (shape[0] == tokens):
+        raise ValueError("routing and x have different numbers of tokens")
     k = shape[1]
     ldx = _rows(x, tokens, H, index, "x")
     if out is None:
@@ -247,7 +257,8 @@ def combine_bwd(dout, ys, routing, out=None):
     fp32).  The residual's gradient is ``dout`` itself."""
     tokens, H, index = _columns(dout, "dout")
     shape = _check_routing(routing, index)
-    _need(shape[0] == tokens, "routing and dout have different numbers of tokens")
+    if not (shape[0] == tokens):
+        raise ValueError("routing and dout have different numbers of tokens")
     k = shape[1]
     ldd = _rows(dout, tokens, H, index, "dout")
     ldy = _rows(ys, tokens * k, H, index, "ys")

@@ -37,18 +37,15 @@ E2M1_MAX = 6.0
 MAX_GROUPS = 1024
 
 
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
-
-
 def _groups(offsets, device):
     if offsets is None:
         return 0
-    _need(offsets.dtype is torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and
-          offsets.get_device() == device, "offsets must be a contiguous int32 vector on the operands' device")
+    if not (offsets.dtype is torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and
+            offsets.get_device() == device):
+        raise ValueError("offsets must be a contiguous int32 vector on the operands' device")
     groups = offsets.numel() - 1
-    _need(1 <= groups <= MAX_GROUPS, f"the number of groups must be 1..{MAX_GROUPS}")
+    if not (1 <= groups <= MAX_GROUPS):
+        raise ValueError(f"the number of groups must be 1..{MAX_GROUPS}")
     return groups
 
 
@@ -60,16 +57,18 @@ def scale_bytes(rows: int, k: int, groups: int = 0, matrices: int = 1) -> int:
 
 def _operand(q, sf, groups, device, what):
     """(matrices, rows, K) of a quantized operand."""
-    _need(q.dtype is torch.uint8 and q.dim() in (2, 3) and q.is_contiguous() and q.get_device() == device,
-          f"{what} must be contiguous uint8 [..., K/2] as written by quantize, on the operands' device")
+    if not (q.dtype is torch.uint8 and q.dim() in (2, 3) and q.is_contiguous() and q.get_device() == device):
+        raise ValueError(f"{what} must be contiguous uint8 [..., K/2] as written by quantize, on the operands' "
+                         f"device")
     shape = q.shape
     matrices = shape[0] if len(shape) == 3 else 1
     rows, K = shape[-2], 2 * shape[-1]
-    _need(K > 0 and K % 32 == 0 and K < 2 ** 26 and rows < 2 ** 31,
-          f"{what}: K must be a positive multiple of 32 below 2^26, and rows fewer than 2^31")
-    _need(sf.dtype is torch.uint8 and sf.is_contiguous() and sf.get_device() == device and
-          sf.numel() >= scale_bytes(rows, K, groups, matrices),
-          f"the scales of {what} must be the uint8 buffer that quantize wrote for these rows (and offsets)")
+    if not (K > 0 and K % 32 == 0 and K < 2 ** 26 and rows < 2 ** 31):
+        raise ValueError(f"{what}: K must be a positive multiple of 32 below 2^26, and rows fewer than 2^31")
+    if not (sf.dtype is torch.uint8 and sf.is_contiguous() and sf.get_device() == device and
+            sf.numel() >= scale_bytes(rows, K, groups, matrices)):
+        raise ValueError(f"the scales of {what} must be the uint8 buffer that quantize wrote for these rows (and "
+                         f"offsets)")
     return matrices, rows, K
 
 
@@ -80,31 +79,34 @@ def quantize(x, offsets=None, q=None, sf=None):
     if x.dtype is not torch.bfloat16:
         raise TypeError("quantize expects bf16")
     dims = x.dim()
-    _need(x.is_cuda and dims in (2, 3), "x must be [rows, K] or [matrices, rows, K] on a CUDA device")
+    if not (x.is_cuda and dims in (2, 3)):
+        raise ValueError("x must be [rows, K] or [matrices, rows, K] on a CUDA device")
     shape, stride = x.shape, x.stride()
     rows, K = shape[-2:]
-    _need(K > 0 and K % 32 == 0 and stride[-1] == 1, "K must be a positive multiple of 32, the last dimension contiguous")
+    if not (K > 0 and K % 32 == 0 and stride[-1] == 1):
+        raise ValueError("K must be a positive multiple of 32, the last dimension contiguous")
     index = x.get_device()
     groups = _groups(offsets, index)
     matrices, ld = 1, stride[0] if rows > 1 else K
     if dims == 3:
-        _need(x.is_contiguous() and offsets is None and shape[0] > 0,
-              "a [matrices, rows, K] operand must be contiguous and takes no offsets")
+        if not (x.is_contiguous() and offsets is None and shape[0] > 0):
+            raise ValueError("a [matrices, rows, K] operand must be contiguous and takes no offsets")
         matrices, ld = shape[0], K
-    _need(ld >= K, "x: rows must not overlap")
+    if not (ld >= K):
+        raise ValueError("x: rows must not overlap")
     lib = native.lib()
     need = lib.tdb_mx4_scale_bytes(matrices, rows, K, groups)
     packed = shape[:-1] + (K // 2,)
     if q is None:
         q = torch.empty(packed, dtype=torch.uint8, device=x.device)
     else:
-        _need(q.dtype is torch.uint8 and q.shape == packed and q.is_contiguous() and q.get_device() == index,
-              "q must be contiguous uint8 [..., K/2] on x's device")
+        if not (q.dtype is torch.uint8 and q.shape == packed and q.is_contiguous() and q.get_device() == index):
+            raise ValueError("q must be contiguous uint8 [..., K/2] on x's device")
     if sf is None:
         sf = torch.empty(need, dtype=torch.uint8, device=x.device)
     else:
-        _need(sf.dtype is torch.uint8 and sf.numel() >= need and sf.is_contiguous() and sf.get_device() == index,
-              f"sf must be a contiguous uint8 buffer of at least {need} bytes on x's device")
+        if not (sf.dtype is torch.uint8 and sf.numel() >= need and sf.is_contiguous() and sf.get_device() == index):
+            raise ValueError(f"sf must be a contiguous uint8 buffer of at least {need} bytes on x's device")
     native.check(lib.tdb_mx4_quantize(x.data_ptr(), ld, matrices, rows, K, None if offsets is None else offsets.data_ptr(),
                                       groups, q.data_ptr(), sf.data_ptr(), native.current_stream(index)), "mx4 quantize")
     return q, sf
@@ -114,17 +116,19 @@ def quantize(x, offsets=None, q=None, sf=None):
 def dequantize(q, sf, offsets=None, out=None):
     """The bf16 values of an operand produced by ``quantize`` with the same
     ``offsets``: exact, but for a value of 2^128, which reads as an infinity."""
-    _need(q.is_cuda, "q must be on a CUDA device")
+    if not (q.is_cuda):
+        raise ValueError("q must be on a CUDA device")
     index = q.get_device()
     groups = _groups(offsets, index)
     matrices, rows, K = _operand(q, sf, groups, index, "q")
-    _need(offsets is None or q.dim() == 2, "a [matrices, rows, K] operand takes no offsets")
+    if not (offsets is None or q.dim() == 2):
+        raise ValueError("a [matrices, rows, K] operand takes no offsets")
     shape = q.shape[:-1] + (K,)
     if out is None:
         out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
-    _need(out.dtype is torch.bfloat16 and out.shape == shape and out.get_device() == index and out.stride(-1) == 1 and
-          (out.is_contiguous() or (out.dim() == 2 and out.stride(0) >= K)),
-          "out must be bf16 [..., K] with contiguous rows that do not overlap, on q's device")
+    if not (out.dtype is torch.bfloat16 and out.shape == shape and out.get_device() == index and
+            out.stride(-1) == 1 and (out.is_contiguous() or (out.dim() == 2 and out.stride(0) >= K))):
+        raise ValueError("out must be bf16 [..., K] with contiguous rows that do not overlap, on q's device")
     ld = out.stride(0) if out.dim() == 2 and rows > 1 else K
     native.check(native.lib().tdb_mx4_dequantize(q.data_ptr(), sf.data_ptr(), matrices, rows, K,
                                                  None if offsets is None else offsets.data_ptr(), groups,
@@ -133,25 +137,31 @@ def dequantize(q, sf, offsets=None, out=None):
 
 
 def _product(qx, sfx, qw, sfw, offsets, bias, out, tile):
-    _need(qx.is_cuda and qx.dim() == 2, "qx must be a quantized [rows, K] operand on a CUDA device")
+    if not (qx.is_cuda and qx.dim() == 2):
+        raise ValueError("qx must be a quantized [rows, K] operand on a CUDA device")
     index = qx.get_device()
     groups = _groups(offsets, index)
     _, rows, K = _operand(qx, sfx, groups, index, "qx")
     matrices, N, Kw = _operand(qw, sfw, 0, index, "qw")
-    _need(K == Kw, f"the K extents differ: {K} and {Kw}")
-    _need(matrices == max(groups, 1), "qw must hold one matrix per group")
-    _need(N > 0 and N % 8 == 0, "N must be a positive multiple of 8")
+    if not (K == Kw):
+        raise ValueError(f"the K extents differ: {K} and {Kw}")
+    if not (matrices == max(groups, 1)):
+        raise ValueError("qw must hold one matrix per group")
+    if not (N > 0 and N % 8 == 0):
+        raise ValueError("N must be a positive multiple of 8")
     if bias is not None:
-        _need(bias.dtype is torch.bfloat16 and bias.numel() == matrices * N and bias.shape[-1] == N and
-              bias.is_contiguous() and bias.get_device() == index, "bias must be contiguous bf16 [N] or [groups, N]")
+        if not (bias.dtype is torch.bfloat16 and bias.numel() == matrices * N and bias.shape[-1] == N and
+                bias.is_contiguous() and bias.get_device() == index):
+            raise ValueError("bias must be contiguous bf16 [N] or [groups, N]")
     if out is None:
         out = torch.empty((rows, N), dtype=torch.bfloat16, device=qx.device)
     ld, step = out.stride() if out.dim() == 2 else (0, 0)
     if rows <= 1:
         ld = N
-    _need(out.dtype is torch.bfloat16 and out.shape == (rows, N) and step == 1 and ld >= N and
-          out.get_device() == index,
-          f"out must be bf16 [{rows}, {N}] with contiguous rows that do not overlap, on the operands' device")
+    if not (out.dtype is torch.bfloat16 and out.shape == (rows, N) and step == 1 and ld >= N and
+            out.get_device() == index):
+        raise ValueError(f"out must be bf16 [{rows}, {N}] with contiguous rows that do not overlap, on the "
+                         f"operands' device")
     native.check(native.lib().tdb_mx4_gemm(
         qx.data_ptr(), sfx.data_ptr(), qw.data_ptr(), sfw.data_ptr(), None if offsets is None else offsets.data_ptr(),
         matrices, out.data_ptr(), ld, rows, N, K, None if bias is None else bias.data_ptr(), tile,
@@ -163,7 +173,8 @@ def _product(qx, sfx, qw, sfw, offsets, bias, out, tile):
 def linear(qx, sfx, qw, sfw, bias=None, out=None, tile=0):
     """``values(qx) @ values(qw)^T (+ bias)`` in bf16 with fp32 accumulation;
     qx [M, K], qw [N, K] from ``quantize``."""
-    _need(qw.dim() == 2, "qw must be a quantized [N, K] matrix")
+    if not (qw.dim() == 2):
+        raise ValueError("qw must be a quantized [N, K] matrix")
     return _product(qx, sfx, qw, sfw, None, bias, out, tile)
 
 
@@ -172,5 +183,6 @@ def grouped_linear(qx, sfx, qw, sfw, offsets, bias=None, out=None, tile=0):
     """``values(qx)[r] @ values(qw)[g]^T (+ bias[g])`` for the rows r of group
     g; qx [R, K] quantized with these ``offsets``, qw [groups, N, K], bias
     [groups, N].  Rows outside every group keep their contents."""
-    _need(offsets is not None and qw.dim() == 3, "grouped_linear needs offsets and a quantized [groups, N, K] operand")
+    if not (offsets is not None and qw.dim() == 3):
+        raise ValueError("grouped_linear needs offsets and a quantized [groups, N, K] operand")
     return _product(qx, sfx, qw, sfw, offsets, bias, out, tile)
