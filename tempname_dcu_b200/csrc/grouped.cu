@@ -167,7 +167,7 @@ TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (tile == 16)
     return mode == gemm::kBiasGelu ? launch_few<gemm::kBiasGelu>(p, A, lda, W, s) : launch_few<gemm::kBias>(p, A, lda, W, s);
-  const uint32_t box_rows = tile == 512 ? 64 : 32;
+  const uint32_t box_rows = tile == 512 ? 128 : 32;
   int rc = tdb_host::make_tmap_2d(&p.tmB, A, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, uint64_t(K), uint64_t(rows),
                                   uint64_t(lda), gemm::BK, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;

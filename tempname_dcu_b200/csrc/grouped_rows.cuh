@@ -44,7 +44,7 @@ template <int CG, int BT, bool MX4>
 struct RowsConfig {
   static constexpr int kTileN = 128 * CG;              // output columns per tile
   static constexpr int kBRows = BT / CG;               // token rows staged per CTA
-  static constexpr int kBox = CG == 2 ? 64 : 32;       // token rows per TMA copy: only boxes with rows are loaded
+  static constexpr int kBox = CG == 2 ? 128 : 32;      // token rows per TMA copy: only boxes with rows are loaded
   static constexpr int kABytes = 128 * 128;            // 128 rows of 64 bf16 or 256 e2m1
   static constexpr int kBBytes = kBRows * 128;
   static constexpr int kBlockRows = BT == 32 ? 32 : 128;  // token rows that a scale block holds (see mx4.cu)

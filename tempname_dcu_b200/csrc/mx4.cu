@@ -347,7 +347,7 @@ TDB_API int tdb_mx4_gemm(const void* qx, const void* sfx, const void* qw, const 
   int rc = tdb_host::make_tmap_3d(&p.tmA, qw, u8, 1, uint64_t(K / 2), uint64_t(N), uint64_t(groups), uint64_t(K / 2),
                                   uint64_t(K / 2) * uint64_t(N), 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  rc = tdb_host::make_tmap_2d(&p.tmB, qx, u8, 1, uint64_t(K / 2), uint64_t(rows), uint64_t(K / 2), 128, tile == 512 ? 64 : 32,
+  rc = tdb_host::make_tmap_2d(&p.tmB, qx, u8, 1, uint64_t(K / 2), uint64_t(rows), uint64_t(K / 2), 128, tile == 512 ? 128 : 32,
                               CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   rc = tdb_host::make_tmap_2d(&p.tmSfa, sfw, u32, 4, 256, uint64_t(int64_t(groups) * w_blocks * pairs), 256, 256, 1,
