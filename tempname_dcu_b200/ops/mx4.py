@@ -51,8 +51,12 @@ def _groups(offsets, device):
 
 def scale_bytes(rows: int, k: int, groups: int = 0, matrices: int = 1) -> int:
     """Bytes of the scales of ``matrices`` [rows, k] operands, or of one whose
-    rows lie in ``groups`` groups."""
-    return native.lib().tdb_mx4_scale_bytes(matrices, rows, k, groups)
+    rows lie in ``groups`` groups (as ``tdb_mx4_scale_bytes``, without the call)."""
+    if groups > 0:
+        blocks = rows // (32 if rows <= groups * 32 else 128) + min(rows, groups)
+    else:
+        blocks = matrices * -(-rows // 128)
+    return blocks * -(-k // 256) * 1024
 
 
 def _operand(q, sf, groups, device, what):
@@ -94,21 +98,21 @@ def quantize(x, offsets=None, q=None, sf=None):
         matrices, ld = shape[0], K
     if not (ld >= K):
         raise ValueError("x: rows must not overlap")
-    lib = native.lib()
-    need = lib.tdb_mx4_scale_bytes(matrices, rows, K, groups)
+    need = scale_bytes(rows, K, groups, matrices)
     packed = shape[:-1] + (K // 2,)
     if q is None:
-        q = torch.empty(packed, dtype=torch.uint8, device=x.device)
+        q = x.new_empty(packed, dtype=torch.uint8)
     else:
         if not (q.dtype is torch.uint8 and q.shape == packed and q.is_contiguous() and q.get_device() == index):
             raise ValueError("q must be contiguous uint8 [..., K/2] on x's device")
     if sf is None:
-        sf = torch.empty(need, dtype=torch.uint8, device=x.device)
+        sf = x.new_empty(need, dtype=torch.uint8)
     else:
         if not (sf.dtype is torch.uint8 and sf.numel() >= need and sf.is_contiguous() and sf.get_device() == index):
             raise ValueError(f"sf must be a contiguous uint8 buffer of at least {need} bytes on x's device")
-    native.check(lib.tdb_mx4_quantize(x.data_ptr(), ld, matrices, rows, K, None if offsets is None else offsets.data_ptr(),
-                                      groups, q.data_ptr(), sf.data_ptr(), native.current_stream(index)), "mx4 quantize")
+    native.check(native.lib().tdb_mx4_quantize(x.data_ptr(), ld, matrices, rows, K,
+                                               None if offsets is None else offsets.data_ptr(), groups, q.data_ptr(),
+                                               sf.data_ptr(), native.current_stream(index)), "mx4 quantize")
     return q, sf
 
 
@@ -125,7 +129,7 @@ def dequantize(q, sf, offsets=None, out=None):
         raise ValueError("a [matrices, rows, K] operand takes no offsets")
     shape = q.shape[:-1] + (K,)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty(shape, dtype=torch.bfloat16)
     if not (out.dtype is torch.bfloat16 and out.shape == shape and out.get_device() == index and
             out.stride(-1) == 1 and (out.is_contiguous() or (out.dim() == 2 and out.stride(0) >= K))):
         raise ValueError("out must be bf16 [..., K] with contiguous rows that do not overlap, on q's device")
@@ -154,7 +158,7 @@ def _product(qx, sfx, qw, sfw, offsets, bias, out, tile):
                 bias.is_contiguous() and bias.get_device() == index):
             raise ValueError("bias must be contiguous bf16 [N] or [groups, N]")
     if out is None:
-        out = torch.empty((rows, N), dtype=torch.bfloat16, device=qx.device)
+        out = qx.new_empty((rows, N), dtype=torch.bfloat16)
     ld, step = out.stride() if out.dim() == 2 else (0, 0)
     if rows <= 1:
         ld = N

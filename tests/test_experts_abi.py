@@ -102,6 +102,11 @@ def test_mx4_refusals():
     assert lib.tdb_mx4_scale_bytes(1, 64, 256, 2) == (2 + 2) * 1024
     assert lib.tdb_mx4_scale_bytes(1, 65, 256, 2) == (0 + 2) * 1024
     assert lib.tdb_mx4_scale_bytes(3, 130, 300, 0) == 3 * 2 * 2 * 1024
+    from tempname_dcu_b200.ops import mx4
+    for rows in (0, 1, 31, 32, 33, 64, 65, 127, 128, 129, 5000):
+        for k in (32, 256, 288):
+            for groups, matrices in ((0, 1), (0, 3), (1, 1), (2, 1), (7, 1), (200, 1)):
+                assert mx4.scale_bytes(rows, k, groups, matrices) == lib.tdb_mx4_scale_bytes(matrices, rows, k, groups)
 
 
 def test_python_refusals_without_a_gpu():
