@@ -16,10 +16,16 @@
 //
 // Sums.  The tensor core truncates when it adds to its fp32 accumulator, an
 // error that grows with the number of additions and has one sign: 1170 rows
-// were 2.2e-6 off (relative 2-norm), the output being fp32.  So a chain of
-// MMAs stops after kChain steps (512 rows) and the epilogue warps, which hold
-// the output tile in registers, add the chain's result rounding to nearest;
-// two TMEM accumulators alternate, so the MMAs do not wait.
+// were 2.2e-6 off (relative 2-norm), 8192 rows 4.4e-6, the output being fp32.
+// So a chain of MMAs stops after kChain steps (512 rows) and the epilogue
+// warps, which hold the output tile in registers, add the chain's result
+// rounding to nearest: 4.8e-7 for any size.  Two TMEM accumulators alternate,
+// so the MMAs do not wait; chains of 256 rows cost 7 % more time.
+//
+// Bounds: short sums the fp32 output (8 groups of 128 rows, 4096 x 4096: 108 us,
+// 5 TB/s), long ones the tensor cores and the output's share of the same path
+// to memory (7 groups of 1170 rows: 287 us from a cool start, 316 us back to
+// back at the power limit, 0.87 PFLOP/s).
 //
 // The output leaves by TMA stores or, when adding, TMA reduce-adds (one writer
 // per element: deterministic); an empty group's tiles are zeros, or skipped
