@@ -136,8 +136,10 @@ TDB_API int tdb_grouped_pick_tile(int op, long long rows, int groups, int M, int
 TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data_grad, const int* offsets, int groups,
                              void* C, int64_t ldc, int rows, int N, int K, int mode, const void* bias, const void* aux,
                              int64_t ld_aux, void* aux_out, int tile, void* stream) {
-  if (groups < 1 || groups > kMaxGroups || rows < 0 || N <= 0 || K <= 0 || N % 8 || K % 8)
-    return tdb_host::fail(int(cudaErrorInvalidValue), "grouped: 1..%d groups, N and K multiples of 8", kMaxGroups);
+  if (groups < 1 || groups > kMaxGroups || rows < 0 || N <= 0 || K <= 0 || N % 8 || K % 8 || rows > kMaxExtent ||
+      N > kMaxExtent || K > kMaxExtent)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "grouped: 1..%d groups, N and K multiples of 8, extents below 2^31 - 1024",
+                          kMaxGroups);
   if (rows == 0) return 0;
   if (!A || !W || !C || !offsets || lda % 8 || lda < K || ldc % 8 || ldc < N || misaligned(A) || misaligned(W) ||
       misaligned(C) || (bias && misaligned(bias)))
@@ -149,8 +151,8 @@ TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data
       (mode == gemm::kGeluBwd && (!aux || misaligned(aux) || ld_aux % 8 || ld_aux < N)))
     return bad("grouped: the pre-activation must be 16-byte aligned with 16-byte row strides");
   if (tile == 0) tile = tdb::grouped::pick_tile(data_grad ? kDataGrad : kForward, rows, groups, 0, N);
-  if (tile != 32 && tile != 128 && tile != 512 && (tile != 16 || data_grad || rows > kFewRows))
-    return bad("grouped: tile must be 0, 32, 128 or 512 (16: forward with at most 16 rows)");
+  if (tile != 32 && tile != 128 && tile != 512 && (tile != 16 || data_grad || rows > kFewRows || N > (1 << 26)))
+    return bad("grouped: tile must be 0, 32, 128 or 512 (16: forward with at most 16 rows and 2^26 columns)");
   RowsParams p = {};
   p.offsets = offsets;
   p.groups = groups;
@@ -200,8 +202,10 @@ TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data
 TDB_API int tdb_grouped_weight_grad(const void* dY, int64_t ldy, const void* X, int64_t ldx, const int* offsets,
                                     int groups, float* C, int rows, int N, int K, int accumulate, int tile,
                                     void* stream) {
-  if (groups < 1 || groups > kMaxGroups || rows < 0 || N <= 0 || K <= 0 || N % 8 || K % 8)
-    return tdb_host::fail(int(cudaErrorInvalidValue), "grouped weight gradient: 1..%d groups, N and K multiples of 8",
+  if (groups < 1 || groups > kMaxGroups || rows < 0 || N <= 0 || K <= 0 || N % 8 || K % 8 || rows > kMaxExtent ||
+      N > kMaxExtent || K > kMaxExtent)
+    return tdb_host::fail(int(cudaErrorInvalidValue),
+                          "grouped weight gradient: 1..%d groups, N and K multiples of 8, extents below 2^31 - 1024",
                           kMaxGroups);
   if (!C || misaligned(C)) return bad("grouped weight gradient: the output must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -237,7 +241,7 @@ TDB_API int tdb_grouped_weight_grad(const void* dY, int64_t ldy, const void* X, 
 // out[g] (fp32 [groups, N]) (+)= the sum of dY's rows of group g.
 TDB_API int tdb_grouped_bias_grad(const void* dY, int64_t ldy, const int* offsets, int groups, float* out, int rows,
                                   int N, int accumulate, void* stream) {
-  if (groups < 1 || groups > kMaxGroups || rows < 0 || N <= 0 || N % 8)
+  if (groups < 1 || groups > kMaxGroups || rows < 0 || N <= 0 || N % 8 || rows > kMaxExtent || N > kMaxExtent)
     return tdb_host::fail(int(cudaErrorInvalidValue), "grouped bias gradient: 1..%d groups, N a multiple of 8", kMaxGroups);
   if (!out || !offsets || (rows > 0 && (!dY || ldy % 8 || ldy < N || misaligned(dY))))
     return bad("grouped bias gradient: rows must be 16-byte aligned");

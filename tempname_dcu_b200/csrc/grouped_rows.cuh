@@ -49,6 +49,7 @@ namespace grouped {
 using gemm::BK;
 constexpr int kThreads = 192;
 constexpr int kMaxGroups = 1024;
+constexpr int kMaxExtent = 0x7fffffff - 1024;  // rows and columns: tile coordinates past the end stay 32-bit
 
 enum Op : int { kForward = 0, kDataGrad = 1, kWeightGrad = 2 };
 

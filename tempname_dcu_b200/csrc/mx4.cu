@@ -148,15 +148,15 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __re
   const int pieces = (K + 255) / 256;
   const int first = blockIdx.y * kBatch;
   const int k0 = first * 256 + lane * 8;
-  auto load = [&](int r, uint4 (&in)[kBatch]) {
-    const uint16_t* src = x + int64_t(r) * ldx + k0;
+  auto load = [&](int64_t r, uint4 (&in)[kBatch]) {
+    const uint16_t* src = x + r * ldx + k0;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b)
       in[b] = r < total_rows && k0 + b * 256 < K ? __ldg(reinterpret_cast<const uint4*>(src + b * 256))
                                                  : make_uint4(0, 0, 0, 0);
   };
-  const int step = gridDim.x * kWarps;
-  int r = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int64_t step = int64_t(gridDim.x) * kWarps;
+  int64_t r = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   uint4 in[kBatch];
   load(r, in);  // before the groups' table is built
   Layout l;
@@ -164,8 +164,8 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const uint16_t* __re
   for (; r < total_rows; r += step, load(r, in)) {
     int64_t blk;
     int row;
-    if (!l.find(r, blk, row)) continue;
-    uint8_t* dst = q + int64_t(r) * (K / 2) + k0 / 2;
+    if (!l.find(int(r), blk, row)) continue;
+    uint8_t* dst = q + r * (K / 2) + k0 / 2;
     uint8_t* scale =
         sf + (blk * pieces + first) * 1024 + (lane >> 4) * 512 + (row & 31) * 16 + (row >> 5) * 4 + ((lane >> 2) & 3);
 #pragma unroll
@@ -204,12 +204,12 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __r
   const int lane = threadIdx.x & 31;
   const int pieces = (K + 255) / 256;
   const int first = blockIdx.y * kBatch;
-  for (int r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < total_rows; r += gridDim.x * kWarps) {
+  for (int64_t r = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); r < total_rows; r += int64_t(gridDim.x) * kWarps) {
     int64_t blk;
     int row;
-    if (!l.find(r, blk, row)) continue;
+    if (!l.find(int(r), blk, row)) continue;
     const int k0 = first * 256 + lane * 8;
-    const uint8_t* src = q + int64_t(r) * (K / 2) + k0 / 2;
+    const uint8_t* src = q + r * (K / 2) + k0 / 2;
     const uint8_t* scale = sf + (blk * pieces + first) * 1024 + (lane >> 4) * 512 + (row & 31) * 16 + (row >> 5) * 4 +
                            ((lane >> 2) & 3);
     uint32_t in[kBatch], byte[kBatch];
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __r
       uint32_t o[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(v[2 * j] * s, v[2 * j + 1] * s);
-      *reinterpret_cast<uint4*>(out + int64_t(r) * ldo + k0 + b * 256) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4*>(out + r * ldo + k0 + b * 256) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
 }
@@ -327,7 +327,8 @@ TDB_API int tdb_mx4_pick_tile(long long rows, int groups, int N) {
 TDB_API int tdb_mx4_gemm(const void* qx, const void* sfx, const void* qw, const void* sfw, const int* offsets, int groups,
                          void* C, int64_t ldc, int rows, int N, int K, const void* bias, int tile, void* stream) {
   using namespace tdb::grouped;
-  if (groups < 1 || groups > kMaxGroups || (!offsets && groups != 1) || rows < 0 || N <= 0 || N % 8 || K < 32 || K % 32)
+  if (groups < 1 || groups > kMaxGroups || (!offsets && groups != 1) || rows < 0 || N <= 0 || N % 8 || K < 32 ||
+      K % 32 || K >= (1 << 26) || rows > kMaxExtent || N > kMaxExtent)
     return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 product: 1..%d groups, N a multiple of 8, K of 32", kMaxGroups);
   if (rows == 0) return 0;
   if (!qx || !sfx || !qw || !sfw || !C || ldc % 8 || ldc < N ||

@@ -45,7 +45,7 @@ MAX_EXPERTS = 512
 MAX_TOP_K = 16
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Routing:
     """A batch's choices of experts, grouped.
 

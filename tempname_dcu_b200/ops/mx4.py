@@ -14,6 +14,8 @@ Rows may be any number, K a multiple of 32, N of the products a multiple of 8.
 an operand quantized with offsets goes into ``grouped_linear`` with the same
 offsets.  Weights are quantized once, [N, K] or [groups, N, K].
 
+``tile`` asks for a tile shape (0: by the sizes), for measurements.
+
 Against ``ops.mx`` (8-bit values): half the bytes and twice the tensor-core
 rate, at 2 significant bits per value.
 """

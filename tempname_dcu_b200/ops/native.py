@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import inspect
 import threading
 
 from . import _build
@@ -121,14 +122,17 @@ def on_tensor_device(fn):
     """Run ``fn(tensor, ...)`` with the tensor's CUDA device current, so that its
     allocations and launches go there.  A tensor that is not on a CUDA device
     is left to the function's own checks."""
+    first = next(iter(inspect.signature(fn).parameters))
+
     @functools.wraps(fn)
-    def call(tensor, *args, **kwargs):
+    def call(*args, **kwargs):
         import torch
+        tensor = args[0] if args else kwargs.get(first)
         index = tensor.get_device() if isinstance(tensor, torch.Tensor) else -1
         if index < 0 or index == torch.cuda.current_device():
-            return fn(tensor, *args, **kwargs)
+            return fn(*args, **kwargs)
         with torch.cuda.device(index):
-            return fn(tensor, *args, **kwargs)
+            return fn(*args, **kwargs)
     return call
 
 

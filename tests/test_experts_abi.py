@@ -62,7 +62,8 @@ def test_grouped_refusals():
              a=A, dg=0):
         return lib.tdb_grouped_gemm(a, lda, A, dg, A, groups, A, ldc, rows, N, K, mode, bias, aux, ld_aux, aux_out, tile,
                                     None)
-    for bad in (dict(groups=0), dict(groups=1025), dict(N=36, ldc=40), dict(K=60), dict(rows=-1), dict(N=0)):
+    for bad in (dict(groups=0), dict(groups=1025), dict(N=36, ldc=40), dict(K=60), dict(rows=-1), dict(N=0),
+                dict(rows=2 ** 31 - 8), dict(N=2 ** 31 - 8, ldc=2 ** 31)):
         _refused(gemm(**bad), b"groups")
     for bad in (dict(lda=60), dict(lda=56), dict(ldc=28), dict(a=ODD), dict(mode=1, bias=ODD)):
         _refused(gemm(**bad), b"aligned")
@@ -73,6 +74,7 @@ def test_grouped_refusals():
     _refused(gemm(tile=64), b"tile")
     _refused(gemm(tile=16, dg=1), b"tile")
     _refused(gemm(tile=16, rows=17), b"tile")
+    _refused(gemm(tile=16, N=2 ** 27, ldc=2 ** 27), b"tile")
     assert gemm(rows=0, a=None) == 0
     _refused(lib.tdb_grouped_weight_grad(A, 32, A, 64, A, 2, ODD, 8, 32, 64, 0, 0, None), b"aligned")
     _refused(lib.tdb_grouped_weight_grad(A, 28, A, 64, A, 2, A, 8, 32, 64, 0, 0, None), b"aligned")
@@ -91,7 +93,7 @@ def test_mx4_refusals():
 
     def gemm(offsets=None, groups=1, ldc=32, rows=8, N=32, K=64, bias=None, tile=0, q=A):
         return lib.tdb_mx4_gemm(q, A, A, A, offsets, groups, A, ldc, rows, N, K, bias, tile, None)
-    for bad in (dict(groups=2), dict(N=36), dict(K=48), dict(offsets=A, groups=1025), dict(rows=-1)):
+    for bad in (dict(groups=2), dict(N=36), dict(K=48), dict(offsets=A, groups=1025), dict(rows=-1), dict(rows=2 ** 31 - 8)):
         _refused(gemm(**bad), b"groups")
     for bad in (dict(ldc=28), dict(q=ODD), dict(bias=ODD)):
         _refused(gemm(**bad), b"aligned")
@@ -130,5 +132,9 @@ def test_python_refusals_without_a_gpu():
                 dict(offsets=torch.zeros(1, dtype=torch.int32)), dict(ids=ids.t())):
         with pytest.raises(ValueError):
             moe.Routing(**dict(dict(ids=ids, weights=torch.zeros(4, 2), offsets=off, order=flat, slots=flat), **bad))
+    for call in (lambda: moe.route(logits=z, top_k=2), lambda: mx4.quantize(x=x)):  # by keyword: the same refusals
+        with pytest.raises(ValueError):
+            call()
+    assert r == r and r != moe.Routing(ids=ids, weights=torch.zeros(4, 2), offsets=off, order=flat, slots=flat)
     with pytest.raises(Exception):
         r.ids = None  # frozen: the checks hold for its life

@@ -124,6 +124,16 @@ def test_rows_beyond_32_bit_offsets(cuda):
     native.raise_on_status()
 
 
+def test_tensors_by_keyword(cuda):
+    import torch
+    from tempname_dcu_b200.ops import grouped, moe
+    z, x = torch.randn(9, 8, device=cuda), torch.randn(9, 64, device=cuda).to(torch.bfloat16)
+    r = moe.route(logits=z, top_k=2)
+    w = torch.randn(8, 32, 64, device=cuda).to(torch.bfloat16)
+    y = grouped.linear(x=moe.dispatch(x=x, routing=r), w=w, offsets=r.offsets)
+    assert torch.equal(y, grouped.linear(moe.dispatch(x, r), w, r.offsets))
+
+
 def test_layer_against_64_bits(cuda):
     """Router, exchange and both products as a layer uses them, with the
     gradients, for a ragged batch with a closed expert."""
