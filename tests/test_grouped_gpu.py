@@ -205,6 +205,19 @@ def test_few_rows(cuda, counts, N, K):
     _status_ok()
 
 
+@pytest.mark.parametrize("tile", [16, 32, 128, 512])
+def test_gelu_of_infinities_and_nan(cuda, tile):
+    import torch
+    from tempname_dcu_b200.ops import grouped
+    off = _offsets([5, 7], cuda)
+    x, w, b = _bf(12, 64, device=cuda), _bf(2, 32, 64, device=cuda), torch.zeros(2, 32, device=cuda, dtype=torch.bfloat16)
+    b[1, 0], b[1, 1], b[1, 2], b[1, 3], b[1, 4] = float("inf"), -float("inf"), float("nan"), 1e20, -1e20
+    h, z = grouped.linear_gelu(x, w, off, b, tile=tile)
+    assert torch.isfinite(h[:5]).all() and torch.isfinite(h[5:, 3:]).all()
+    assert (h[5:, 0] == float("inf")).all() and (h[5:, 1] == 0).all() and h[5:, 2].isnan().all()
+    assert torch.equal(h[5:, 3], z[5:, 3]) and (h[5:, 4] == 0).all()
+
+
 def test_many_groups_and_repeat_bitwise(cuda):
     import torch
     from tempname_dcu_b200.ops import grouped
