@@ -90,8 +90,9 @@ def _gemm(a, w, offsets, data_grad, mode, out, bias, aux, aux_out, tile):
                 bias.get_device() == index):
             raise ValueError(f"bias must be contiguous bf16 [{groups}, {N}] on the operands' device")
     if out is None:
-        out = a.new_empty((rows, N))
-    ldc = _rows(out, rows, N, index, "out")
+        out, ldc = a.new_empty((rows, N)), N
+    else:
+        ldc = _rows(out, rows, N, index, "out")
     pre = aux_out if aux_out is not None else aux
     ld_aux = 0 if pre is None else _rows(pre, rows, N, index, "the pre-activation")
     native.check(native.lib().tdb_grouped_gemm(
@@ -116,8 +117,6 @@ def linear_gelu(x, w, offsets, bias=None, pre_out=None, out=None, tile=0):
         raise ValueError("x must be [R, K] and w [groups, N, K]")
     if pre_out is None:
         pre_out = x.new_empty((x.shape[0], w.shape[1]))
-    if out is None:
-        out = torch.empty_like(pre_out, memory_format=torch.contiguous_format)
     return _gemm(x, w, offsets, 0, BIAS_GELU, out, bias, None, pre_out, tile), pre_out
 
 
@@ -146,7 +145,8 @@ def weight_grad(dy, x, offsets, out_f32=None, accumulate=True, tile=0):
     if out_f32 is None:
         out_f32 = torch.empty((groups, N, K), dtype=torch.float32, device=dy.device)
         accumulate = False
-    _fp32(out_f32, (groups, N, K), index, "the weight gradient")
+    else:
+        _fp32(out_f32, (groups, N, K), index, "the weight gradient")
     native.check(native.lib().tdb_grouped_weight_grad(
         dy.data_ptr(), ldy, x.data_ptr(), ldx, offsets.data_ptr(), groups, out_f32.data_ptr(), rows, N, K,
         bool(accumulate), tile, native.current_stream(index)), "grouped weight gradient")
@@ -168,7 +168,8 @@ def bias_grad(dy, offsets, out_f32=None, accumulate=True):
     if out_f32 is None:
         out_f32 = torch.empty((groups, N), dtype=torch.float32, device=dy.device)
         accumulate = False
-    _fp32(out_f32, (groups, N), index, "the bias gradient")
+    else:
+        _fp32(out_f32, (groups, N), index, "the bias gradient")
     native.check(native.lib().tdb_grouped_bias_grad(dy.data_ptr(), ldy, offsets.data_ptr(), groups, out_f32.data_ptr(),
                                                     rows, N, bool(accumulate), native.current_stream(index)),
                  "grouped bias gradient")

@@ -194,12 +194,13 @@ def route_bwd(logits, routing, dweights, out=None):
             dweights.get_device() == index):
         raise ValueError("dweights must be contiguous fp32 [tokens, k] on the logits' device")
     if out is None:
-        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
-    if not (out.shape == (tokens, experts)):
-        raise ValueError("out must be [tokens, experts]")
-    _, _, ld_out, out_bf16, out_index = _logits(out, "out")
-    if not (out_index == index):
-        raise ValueError("out must be on the logits' device")
+        out, ld_out, out_bf16 = torch.empty_like(logits, memory_format=torch.contiguous_format), experts, bf16
+    else:
+        if not (out.shape == (tokens, experts)):
+            raise ValueError("out must be [tokens, experts]")
+        _, _, ld_out, out_bf16, out_index = _logits(out, "out")
+        if not (out_index == index):
+            raise ValueError("out must be on the logits' device")
     native.check(native.lib().tdb_moe_route_bwd(logits.data_ptr(), bf16, ld, tokens, experts, shape[1],
                                                 bool(routing.normalize), routing.ids.data_ptr(),
                                                 routing.weights.data_ptr(), dweights.data_ptr(), out.data_ptr(),
@@ -217,8 +218,9 @@ def dispatch(x, routing, out=None):
     k = shape[1]
     ldx = _rows(x, tokens, H, index, "x")
     if out is None:
-        out = x.new_empty((tokens * k, H))
-    ldo = _rows(out, tokens * k, H, index, "out")
+        out, ldo = x.new_empty((tokens * k, H)), H
+    else:
+        ldo = _rows(out, tokens * k, H, index, "out")
     native.check(native.lib().tdb_moe_dispatch(x.data_ptr(), ldx, tokens, k, H, routing.slots.data_ptr(),
                                                out.data_ptr(), ldo, native.current_stream(index)), "moe dispatch")
     return out
@@ -230,8 +232,9 @@ def _combine(y, routing, weighted, residual, out, what):
     ldy = _rows(y, tokens * k, H, index, "the grouped rows")
     ldr = 0 if residual is None else _rows(residual, tokens, H, index, "residual")
     if out is None:
-        out = y.new_empty((tokens, H))
-    ldo = _rows(out, tokens, H, index, "out")
+        out, ldo = y.new_empty((tokens, H)), H
+    else:
+        ldo = _rows(out, tokens, H, index, "out")
     native.check(native.lib().tdb_moe_combine(y.data_ptr(), ldy, tokens, k, H, routing.slots.data_ptr(),
                                               routing.weights.data_ptr() if weighted else None,
                                               None if residual is None else residual.data_ptr(), ldr, out.data_ptr(),
@@ -263,8 +266,9 @@ def combine_bwd(dout, ys, routing, out=None):
     ldd = _rows(dout, tokens, H, index, "dout")
     ldy = _rows(ys, tokens * k, H, index, "ys")
     if out is None:
-        out = dout.new_empty((tokens * k, H))
-    ldo = _rows(out, tokens * k, H, index, "out")
+        out, ldo = dout.new_empty((tokens * k, H)), H
+    else:
+        ldo = _rows(out, tokens * k, H, index, "out")
     dweights = torch.empty_like(routing.weights)
     native.check(native.lib().tdb_moe_combine_bwd(dout.data_ptr(), ldd, ys.data_ptr(), ldy, tokens, k, H,
                                                   routing.slots.data_ptr(), routing.weights.data_ptr(),

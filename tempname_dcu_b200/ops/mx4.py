@@ -160,14 +160,15 @@ def _product(qx, sfx, qw, sfw, offsets, bias, out, tile):
                 bias.is_contiguous() and bias.get_device() == index):
             raise ValueError("bias must be contiguous bf16 [N] or [groups, N]")
     if out is None:
-        out = qx.new_empty((rows, N), dtype=torch.bfloat16)
-    ld, step = out.stride() if out.dim() == 2 else (0, 0)
-    if rows <= 1:
-        ld = N
-    if not (out.dtype is torch.bfloat16 and out.shape == (rows, N) and step == 1 and ld >= N and
-            out.get_device() == index):
-        raise ValueError(f"out must be bf16 [{rows}, {N}] with contiguous rows that do not overlap, on the "
-                         f"operands' device")
+        out, ld = qx.new_empty((rows, N), dtype=torch.bfloat16), N
+    else:
+        ld, step = out.stride() if out.dim() == 2 else (0, 0)
+        if rows <= 1:
+            ld = N
+        if not (out.dtype is torch.bfloat16 and out.shape == (rows, N) and step == 1 and ld >= N and
+                out.get_device() == index):
+            raise ValueError(f"out must be bf16 [{rows}, {N}] with contiguous rows that do not overlap, on the "
+                             f"operands' device")
     native.check(native.lib().tdb_mx4_gemm(
         qx.data_ptr(), sfx.data_ptr(), qw.data_ptr(), sfw.data_ptr(), None if offsets is None else offsets.data_ptr(),
         matrices, out.data_ptr(), ld, rows, N, K, None if bias is None else bias.data_ptr(), tile,
