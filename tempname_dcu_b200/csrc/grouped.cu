@@ -71,19 +71,30 @@ static int launch_few(const RowsParams& p, const void* A, int64_t lda, const voi
   return int(cudaGetLastError());
 }
 
-// Sums of dy's rows per group and column.  One block per group and 64
-// columns: 8 threads x 8 columns by 32 row lanes, joined in a fixed order.
-// Bound by reading dy: 8192 x 4096 in 9.5 us (7 TB/s, partly from L2).
+// Sums of dy's rows per group and column.  A block takes 64 columns of a group,
+// 8 threads x 8 columns by 32 row lanes, joined in a fixed order.  PARTS > 1: a
+// cluster of that many blocks shares a group's rows (each a contiguous part)
+// and the first adds the others' sums, read from their shared memory; for
+// outputs whose blocks would not fill the SMs.  Bound by reading dy: 8 groups,
+// 8192 x 4096 in 9.5 us (7 TB/s, partly from L2).
+template <int PARTS>
 __global__ void __launch_bounds__(256) bias_grad_kernel(const uint16_t* __restrict__ dy, int64_t ld, int rows, int N,
                                                         const int* __restrict__ offsets, float* __restrict__ out,
                                                         int accumulate, int* status) {
   __shared__ float sh[32][65];
-  const int g = blockIdx.y, cx = threadIdx.x & 7, lane_row = threadIdx.x >> 3;
-  const int col = blockIdx.x * 64 + cx * 8;
-  const int lo = offsets[g], hi = offsets[g + 1];
-  if (lo < 0 || hi < lo || hi > rows) {
-    if (threadIdx.x == 0) record_status(status, kBadArgument, 301, g, hi);
+  __shared__ float sums[64];
+  const int g = blockIdx.z, cx = threadIdx.x & 7, lane_row = threadIdx.x >> 3;
+  const int col = blockIdx.y * 64 + cx * 8;
+  const int first = offsets[g], last = offsets[g + 1];
+  if (first < 0 || last < first || last > rows) {  // the same for every block of the cluster
+    if (threadIdx.x == 0) record_status(status, kBadArgument, 301, g, last);
     return;
+  }
+  int lo = first, hi = last;
+  if (PARTS > 1) {
+    const int part = (last - first + PARTS - 1) / PARTS;
+    lo = min(first + int(blockIdx.x) * part, last);
+    hi = min(lo + part, last);
   }
   float acc[8] = {};
   if (col < N) {
@@ -101,14 +112,55 @@ __global__ void __launch_bounds__(256) bias_grad_kernel(const uint16_t* __restri
 #pragma unroll
   for (int j = 0; j < 8; ++j) sh[lane_row][cx * 8 + j] = acc[j];
   __syncthreads();
-  const int c = blockIdx.x * 64 + int(threadIdx.x);
-  if (threadIdx.x < 64 && c < N) {
-    float s = 0.f;
+  float s = 0.f;
+  if (threadIdx.x < 64) {
 #pragma unroll
     for (int r = 0; r < 32; ++r) s += sh[r][threadIdx.x];
+    if (PARTS > 1) sums[threadIdx.x] = s;
+  }
+  if (PARTS > 1) {
+    gemm2::cluster_sync();
+    if (blockIdx.x == 0 && threadIdx.x < 64) {
+      s = 0.f;
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) {
+        float v;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                     : "=f"(v)
+                     : "r"(gemm2::mapa(smem_u32(&sums[threadIdx.x]), uint32_t(i)))
+                     : "memory");
+        s += v;
+      }
+    }
+    gemm2::cluster_sync();  // no block leaves while its sums are read
+    if (blockIdx.x != 0) return;
+  }
+  const int c = blockIdx.y * 64 + int(threadIdx.x);
+  if (threadIdx.x < 64 && c < N) {
     float* o = out + int64_t(g) * N + c;
     *o = accumulate ? *o + s : s;
   }
+}
+
+template <int PARTS>
+static int launch_bias_grad(const uint16_t* dY, int64_t ldy, int rows, int N, const int* offsets, int groups, float* out,
+                            int accumulate, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PARTS;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(PARTS, (N + 63) / 64, groups);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = PARTS > 1 ? 1 : 0;
+  int* status = tdb_host::status_ptr();
+  cudaError_t e = cudaLaunchKernelEx(&cfg, bias_grad_kernel<PARTS>, dY, ldy, rows, N, offsets, out, accumulate, status);
+  tdb_host::launched(1);
+  if (e != cudaSuccess) return tdb_host::fail(int(e), "grouped bias gradient: launch failed");
+  return 0;
 }
 
 static bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
@@ -245,8 +297,11 @@ TDB_API int tdb_grouped_bias_grad(const void* dY, int64_t ldy, const int* offset
     return tdb_host::fail(int(cudaErrorInvalidValue), "grouped bias gradient: 1..%d groups, N a multiple of 8", kMaxGroups);
   if (!out || !offsets || (rows > 0 && (!dY || ldy % 8 || ldy < N || misaligned(dY))))
     return bad("grouped bias gradient: rows must be 16-byte aligned");
-  bias_grad_kernel<<<dim3((N + 63) / 64, groups), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(dY), ldy, rows, N, offsets, out, accumulate, tdb_host::status_ptr());
-  tdb_host::launched(1);
-  return int(cudaGetLastError());
+  if ((N + 63) / 64 > 65535) return bad("grouped bias gradient: at most 65535 x 64 columns");
+  const uint16_t* dy = static_cast<const uint16_t*>(dY);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // eight blocks per group and 64 columns unless the groups' own blocks fill the SMs (8 of 256 threads each)
+  if (int64_t(groups) * ((N + 63) / 64) >= int64_t(tdb_host::sm_count()) * 2)
+    return launch_bias_grad<1>(dy, ldy, rows, N, offsets, groups, out, accumulate, s);
+  return launch_bias_grad<8>(dy, ldy, rows, N, offsets, groups, out, accumulate, s);
 }

@@ -205,6 +205,28 @@ def test_few_rows(cuda, counts, N, K):
     _status_ok()
 
 
+@pytest.mark.parametrize("counts", [[5000, 3, 0, 1], [0, 0], [9, 4000], [130] * 40])
+@pytest.mark.parametrize("N", [8, 72, 1000, 4096])
+def test_bias_gradient_of_long_groups(cuda, counts, N):
+    """Groups whose rows several blocks share, and outputs that need no sharing."""
+    import torch
+    from tempname_dcu_b200.ops import grouped
+    torch.manual_seed(N)
+    off = _offsets(counts, cuda, start=2)
+    dy = _bf(sum(counts) + 5, N + 8, device=cuda)[:, :N]
+    dy[:2] = float("nan")
+    dy[-3:] = float("inf")
+    spans = list(zip(off.tolist(), off.tolist()[1:]))
+    exact = torch.stack([dy[a:c].double().sum(0) for a, c in spans])
+    size = torch.stack([dy[a:c].double().abs().sum(0) for a, c in spans])
+    got = grouped.bias_grad(dy, off)
+    assert _within(got, exact, size, max(max(counts), 1), 2.0 ** -24)
+    again = got.clone()
+    grouped.bias_grad(dy, off, again)
+    assert torch.equal(again, got + got) and torch.equal(got, grouped.bias_grad(dy, off))
+    _status_ok()
+
+
 @pytest.mark.parametrize("tile", [16, 32, 128, 512])
 def test_gelu_of_infinities_and_nan(cuda, tile):
     import torch
