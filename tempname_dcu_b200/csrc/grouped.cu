@@ -47,7 +47,7 @@ static int pick_tile(int op, int64_t rows, int groups, int M, int N) {
     const int64_t tiles = (rows < groups ? rows : groups) * ((N + 127) / 128);
     if (tiles * 5 < int64_t(tdb_host::sm_count()) * 4) return 16;
   }
-  return pick_rows_tile(rows, groups, N);
+  return pick_rows_tile(rows, groups, N, (M + gemm::BK - 1) / gemm::BK);
 }
 
 template <int MODE>
@@ -173,8 +173,8 @@ static int bad(const char* what) { return tdb_host::fail(int(cudaErrorInvalidVal
 using namespace tdb;
 using namespace tdb::grouped;
 
-// Tile code that a grouped call takes (op 0 forward, 1 data gradient, 2 weight
-// gradient); see pick_tile.
+// Tile code that a grouped call takes (op 0 forward, 1 data gradient: M summed
+// values; 2 weight gradient: M x N outputs); see pick_tile.
 TDB_API int tdb_grouped_pick_tile(int op, long long rows, int groups, int M, int N) {
   return tdb::grouped::pick_tile(op, rows, groups, M, N);
 }
@@ -202,7 +202,7 @@ TDB_API int tdb_grouped_gemm(const void* A, int64_t lda, const void* W, int data
   if ((mode == gemm::kBiasGelu && (!aux_out || misaligned(aux_out) || ld_aux % 8 || ld_aux < N)) ||
       (mode == gemm::kGeluBwd && (!aux || misaligned(aux) || ld_aux % 8 || ld_aux < N)))
     return bad("grouped: the pre-activation must be 16-byte aligned with 16-byte row strides");
-  if (tile == 0) tile = tdb::grouped::pick_tile(data_grad ? kDataGrad : kForward, rows, groups, 0, N);
+  if (tile == 0) tile = tdb::grouped::pick_tile(data_grad ? kDataGrad : kForward, rows, groups, K, N);
   if (tile != 32 && tile != 128 && tile != 512 && (tile != 16 || data_grad || rows > kFewRows || N > (1 << 26)))
     return bad("grouped: tile must be 0, 32, 128 or 512 (16: forward with at most 16 rows and 2^26 columns)");
   RowsParams p = {};

@@ -85,6 +85,7 @@ struct alignas(64) RowsParams {
   const int* offsets;        // [groups + 1], or null: one group of all rows
   int groups, rows;
   int N, K;                  // output columns, summed values
+  int parts;                 // SPLIT: CTAs per tile
   int band;                  // token tiles per raster band
   int a_blocks, kpairs;      // MX4: 128-row blocks of a weight matrix, atom pairs along K
   uint16_t* C;
@@ -524,9 +525,25 @@ struct RowsEpilogue {
   }
 };
 
-template <int CG, int BT, int OP, int MODE, bool MX4>
+// A barrier over the cluster's threads, for warps whose lanes took different ways.
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ float load_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// SPLIT (CG = 1): a cluster of CTAs computes one tile, each a part of the summed
+// steps.  They leave their accumulators in shared memory; chunk c (32 rows) is
+// then added up, always in the same order, and stored by CTA c % parts.  For
+// long sums whose tiles are few.
+template <int CG, int BT, int OP, int MODE, bool MX4, bool SPLIT = false>
 __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
   using Cfg = RowsConfig<CG, BT, MX4>;
+  static_assert(!SPLIT || (CG == 1 && Cfg::kAccums == 2 && BT * 512 <= Cfg::kStages * Cfg::kStageBytes), "split sums");
   constexpr int S = Cfg::kStages;
   constexpr bool kAMn = OP == kDataGrad;
   constexpr int kStep = MX4 ? 256 : BK;  // summed values per stage
@@ -543,9 +560,13 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? gemm2::cluster_ctarank() : 0u;
-  const int unit = CG == 2 ? blockIdx.x >> 1 : blockIdx.x;
-  const int units = CG == 2 ? gridDim.x >> 1 : gridDim.x;
-  const int num_kb = (p.K + kStep - 1) / kStep;
+  // SPLIT: a unit is a cluster of `parts` CTAs, and there are as many units as tiles
+  const int part = SPLIT ? int(gemm2::cluster_ctarank()) : 0, parts = SPLIT ? p.parts : 1;
+  const int unit = CG == 2 ? blockIdx.x >> 1 : SPLIT ? blockIdx.x / parts : blockIdx.x;
+  const int units = CG == 2 ? gridDim.x >> 1 : SPLIT ? gridDim.x / parts : gridDim.x;
+  const int all_kb = (p.K + kStep - 1) / kStep;
+  const int first_kb = SPLIT ? all_kb * part / parts : 0;  // this CTA's steps (at least one: parts <= all_kb)
+  const int num_kb = SPLIT ? all_kb * (part + 1) / parts - first_kb : all_kb;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -605,7 +626,7 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
         const int share = t.mma_n / CG;
         const int b0 = t.r0 + int(rank) * share;  // and its share of the token rows
         const int boxes = (share + Cfg::kBox - 1) / Cfg::kBox;
-        for (int kb = 0; kb < num_kb; ++kb, ++it, ring.next()) {
+        for (int kb = first_kb; kb < first_kb + num_kb; ++kb, ++it, ring.next()) {
           const int s = ring.s;
           if (!mbar_wait(&bars->empty[s], ring.phase ^ 1, status, 310)) { ok = false; *abort_flag = 1; break; }
           uint8_t* sa = smem + s * Cfg::kStageBytes;
@@ -702,8 +723,61 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
     // ---------------- Epilogue (warps 2..5) ----------------
     const int quarter = warp & 3;  // TMEM lanes [32*quarter, 32*quarter+32)
     RowsEpilogue<MODE> epi{p, smem_u32(epi_smem) + uint32_t(quarter * 2 * Cfg::kBuf)};
+    if constexpr (SPLIT) {
+      // fp32 of chunk c, this warp, fragment element j: 4 bytes per lane (the ring is free: its steps are summed)
+      const uint32_t mine = smem_u32(smem) + uint32_t(quarter * 4096 + lane * 4);
+      RowsTile t;
+      bool ok = unit < tiles;
+      if (ok) {
+        t = rows_locate<CG, BT, MX4>(p, table, unit);
+        ok = __all_sync(~0u, mbar_wait(&bars->tmem_full[0], 0, status, 330) && !*abort_flag);
+        tc_fence_after();
+      }
+      const int col0 = ok ? t.n0 + quarter * 32 : p.N, chunks = ok ? (t.count + 31) / 32 : 0;
+      const bool on = col0 < p.N;
+      auto read = [&](int c, float (&v)[32]) {
+        uint32_t lo[16], hi[16];
+        const uint32_t acc = tmem_base + (uint32_t(quarter * 32) << 16) + c * 32;
+        tmem_ld_16x256b_x4(acc, lo);
+        tmem_ld_16x256b_x4(acc + (16u << 16), hi);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          v[j] = __uint_as_float(lo[j]);
+          v[16 + j] = __uint_as_float(hi[j]);
+        }
+      };
+      if (on) {
+        for (int c = 0; c < chunks; ++c) {
+          if (c % parts == part) continue;
+          float v[32];
+          read(c, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + uint32_t(c * 16384 + j * 128)), "f"(v[j]) : "memory");
+        }
+      }
+      cluster_barrier();
+      if (on) {
+        epi.tile_begin(t, col0);
+        for (int c = part; c < chunks; c += parts) {
+          uint4 aux[4];
+          if (MODE == gemm::kGeluBwd) epi.load_aux(t.r0 + 32 * c, t.count - 32 * c, col0, aux);
+          float v[32];
+          read(c, v);
+          for (int i = 0; i < parts; ++i) {
+            if (i == part) continue;
+            const uint32_t from = gemm2::mapa(mine + uint32_t(c * 16384), uint32_t(i));
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += load_cluster(from + uint32_t(j * 128));
+          }
+          epi.block(v, aux, t.r0 + 32 * c, t.count - 32 * c, col0);
+        }
+      }
+      cluster_barrier();  // no CTA leaves while its sums are read
+    }
     int tc = 0;
-    for (int i = unit; i < tiles; i += units) {
+    for (int i = unit; !SPLIT && i < tiles; i += units) {
       const RowsTile t = rows_locate<CG, BT, MX4>(p, table, i);
       const int b = Cfg::kAccums == 2 ? (tc & 1) : 0;
       const int use = Cfg::kAccums == 2 ? (tc >> 1) : tc;
@@ -787,6 +861,10 @@ __device__ __forceinline__ void rows_mainloop(const RowsParams& p) {
     epi.finish();
   }
 
+  if (SPLIT && warp < 2) {  // the epilogue's two barriers
+    cluster_barrier();
+    cluster_barrier();
+  }
   tc_fence_before();
   __syncthreads();
   if (CG == 2) {

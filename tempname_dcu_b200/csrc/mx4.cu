@@ -317,7 +317,7 @@ TDB_API int tdb_mx4_dequantize(const void* q, const void* sf, int64_t matrices, 
 TDB_API int tdb_mx4_pick_tile(long long rows, int groups, int N) {
   if (groups < 1) groups = 1;
   if (rows <= int64_t(groups) * 32) return 32;
-  const int tile = tdb::grouped::pick_rows_tile(rows, groups, N);
+  const int tile = tdb::grouped::pick_rows_tile(rows, groups, N, 0);
   return tile < 128 ? 128 : tile;
 }
 

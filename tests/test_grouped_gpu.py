@@ -205,6 +205,51 @@ def test_few_rows(cuda, counts, N, K):
     _status_ok()
 
 
+@pytest.mark.parametrize("tile", [0, 32, 128])
+@pytest.mark.parametrize("counts", [[17], [40, 0, 3, 129], [100, 260], [1] * 20])
+@pytest.mark.parametrize("terms", [512, 1000, 4104, 8192])
+def test_long_sums_of_few_tiles(cuda, terms, counts, tile):
+    """Tiles whose summed values several blocks share."""
+    import torch
+    from tempname_dcu_b200.ops import grouped
+    torch.manual_seed(terms)
+    G, width = len(counts), 72
+    off = _offsets(counts, cuda, start=2)
+    R = sum(counts) + 5
+    spans = list(zip(off.tolist(), off.tolist()[1:]))
+    x = _bf(R, terms, device=cuda)
+    x[:2] = float("nan")
+    x[-3:] = float("inf")
+    rows = slice(2, R - 3)
+    w, b, pre = _bf(G, width, terms, device=cuda, scale=0.1), _bf(G, width, device=cuda), _bf(R, width, device=cuda)
+    group = torch.repeat_interleave(torch.arange(G, device=cuda), torch.tensor(counts, device=cuda))
+    exact = torch.cat([x[a:c].double() @ w[g].double().t() for g, (a, c) in enumerate(spans)])
+    size = torch.cat([x[a:c].double().abs() @ w[g].double().abs().t() for g, (a, c) in enumerate(spans)])
+    out = torch.full((R, width + 8), 7.0, device=cuda, dtype=torch.bfloat16)
+    grouped.linear(x, w, off, out=out[:, :width], tile=tile)
+    assert _within(out[rows, :width], exact, size, terms)
+    assert (out[:2] == 7).all() and (out[-3:] == 7).all() and (out[:, width:] == 7).all()
+    assert torch.equal(grouped.linear(x, w, off, tile=tile)[rows], out[rows, :width])
+    z, zs = exact + b.double()[group], size + b.double().abs()[group]
+    h, got = grouped.linear_gelu(x, w, off, b, tile=tile)
+    assert _within(got[rows], z, zs, terms)
+    gelu = 0.5 * z * torch.erfc(-z / 2 ** 0.5)
+    # |gelu'| < 1.13; the distribution function is off by less than 1.5e-7 / 2 (its approximation) + 2^-22, times z
+    assert ((h[rows].double() - gelu).abs() <= gelu.abs() * 2.0 ** -8 + 1.2 * zs * terms * 2.0 ** -22 + z.abs() * 4e-7).all()
+    wt = w.transpose(1, 2).contiguous()  # [G, terms, width]: the gradient of x sums over its rows
+    dx = torch.full((R, width), 7.0, device=cuda, dtype=torch.bfloat16)
+    grouped.matmul_nt(x, wt, off, out=dx, tile=tile)
+    assert _within(dx[rows], exact, size, terms)
+    p = pre[rows].double()
+    slope = 0.5 * torch.erfc(-p / 2 ** 0.5) + p * torch.exp(-p * p / 2) / (2 * torch.pi) ** 0.5
+    grouped.matmul_nt(x, wt, off, gelu_pre=pre, out=dx, tile=tile)
+    # the slope in fp32: its terms are below 1.2, each within 2^-20
+    assert ((dx[rows].double() - exact * slope).abs() <=
+            (exact * slope).abs() * 2.0 ** -8 + 1.2 * size * terms * 2.0 ** -22 + exact.abs() * 2.0 ** -19).all()
+    assert (dx[:2] == 7).all() and (dx[-3:] == 7).all()
+    _status_ok()
+
+
 @pytest.mark.parametrize("counts", [[5000, 3, 0, 1], [0, 0], [9, 4000], [130] * 40])
 @pytest.mark.parametrize("N", [8, 72, 1000, 4096])
 def test_bias_gradient_of_long_groups(cuda, counts, N):

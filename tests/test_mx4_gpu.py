@@ -188,6 +188,32 @@ def test_grouped_linear_with_small_groups(cuda, counts, N, K):
     _status_ok()
 
 
+@pytest.mark.parametrize("counts", [[1], [0, 140, 0], [40, 0, 1, 70], [9] * 12])
+@pytest.mark.parametrize("K", [2048, 2592, 8192])
+def test_long_sums_of_few_tiles(cuda, counts, K):
+    """Tiles whose summed values several blocks share."""
+    import torch
+    from tempname_dcu_b200.ops import mx4
+    torch.manual_seed(K)
+    G, N, R = len(counts), 136, sum(counts)
+    bounds = [sum(counts[:g]) for g in range(G + 1)]
+    off = torch.tensor(bounds, dtype=torch.int32, device=cuda)
+    x = torch.randn(R, K, device=cuda).to(torch.bfloat16)
+    w = (torch.randn(G, N, K, device=cuda) * 0.02).to(torch.bfloat16)
+    b = torch.randn(G, N, device=cuda).to(torch.bfloat16)
+    xv, wv = _values(x), _values(w)
+    qw, sfw = mx4.quantize(w)
+    out = mx4.grouped_linear(*mx4.quantize(x, offsets=off), qw, sfw, off, bias=b)
+    for g in range(G):
+        lo, hi = bounds[g], bounds[g + 1]
+        assert _within(out[lo:hi], xv[lo:hi] @ wv[g].t() + b[g].double(),
+                       xv[lo:hi].abs() @ wv[g].abs().t() + b[g].double().abs(), K)
+    y = mx4.linear(*mx4.quantize(x), *mx4.quantize(w[0]))
+    assert _within(y, xv @ wv[0].t(), xv.abs() @ wv[0].abs().t(), K)
+    assert torch.equal(y, mx4.linear(*mx4.quantize(x), *mx4.quantize(w[0])))
+    _status_ok()
+
+
 def test_nan_stays_in_its_row(cuda):
     import torch
     from tempname_dcu_b200.ops import mx4
