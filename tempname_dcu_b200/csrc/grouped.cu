@@ -8,9 +8,9 @@
 namespace tdb {
 namespace grouped {
 
-template <int CG, int BN>
+template <int CG, int BN, bool SPLIT>
 __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid_constant__ Params p) {
-  mainloop<CG, BN>(p);
+  mainloop<CG, BN, SPLIT>(p);
 }
 
 template <int CG, int BN>
@@ -18,8 +18,15 @@ static int launch_weight_grad(const Params& p, cudaStream_t stream) {
   using Cfg = Config<CG, BN>;
   static_assert(Cfg::smem_bytes(kMaxGroups) <= 227 * 1024, "shared memory budget");
   const int64_t tiles = int64_t(p.groups) * ((p.M + Cfg::kTileM - 1) / Cfg::kTileM) * ((p.N + BN - 1) / BN);
+  if constexpr (CG == 1) {
+    static SplitState state[64];
+    const int steps = p.rows / p.groups / gemm::BK;  // of an average group
+    const int rc = launch_split(weight_grad_kernel<CG, BN, true>, p, kWgThreads, tiles, steps, Cfg::smem_bytes(p.groups),
+                                Cfg::smem_bytes(kMaxGroups), state, stream);
+    if (rc >= 0) return rc;
+  }
   static LaunchState state[64];
-  return launch_units<CG>(weight_grad_kernel<CG, BN>, p, kWgThreads, tiles, Cfg::smem_bytes(p.groups),
+  return launch_units<CG>(weight_grad_kernel<CG, BN, false>, p, kWgThreads, tiles, Cfg::smem_bytes(p.groups),
                           Cfg::smem_bytes(kMaxGroups), state, stream);
 }
 

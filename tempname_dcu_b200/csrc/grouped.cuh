@@ -27,6 +27,13 @@
 // to memory (7 groups of 1170 rows: 287 us from a cool start, 316 us back to
 // back at the power limit, 0.87 PFLOP/s).
 //
+// Few tiles with long sums (SPLIT, CG = 1): a cluster of CTAs computes one tile,
+// each a part of the group's steps.  The tile's 16 boxes of 32 x 32 values go to
+// the CTAs in turn; each leaves the boxes of the others in its shared memory and
+// adds up its own, always in the same order: 2 groups of 4096 rows, 64 x 64,
+// 26.2 us with one CTA each, 12.7 with eight; 2 of 8192, 512 x 512, 50 and 22;
+// 4 of 1024, 256 x 1024 (two CTAs of 8 steps each), 10.4 and 10.5.
+//
 // The output leaves by TMA stores or, when adding, TMA reduce-adds (one writer
 // per element: deterministic); an empty group's tiles are zeros, or skipped
 // when adding.
@@ -73,6 +80,7 @@ struct alignas(64) Params {
   int groups, rows;
   int M, N;              // output [groups][M][N]
   int band;              // m tiles per raster band
+  int parts;             // SPLIT: CTAs per tile
   int accumulate;
   int* status;
 };
@@ -95,13 +103,14 @@ static_assert(sizeof(Barriers) <= 512, "barrier slot");
 struct Tile {
   int g;
   int m0, n0;   // first output row and column
-  int k0, kb;   // first summed row and number of BK steps
+  int k0, kb;   // first summed row and number of BK steps (SPLIT: of this CTA's part)
+  int rows;     // of the group
   int last;     // rows of the last step, 1..64
   __device__ __forceinline__ bool patched() const { return (last & 15) != 0; }
 };
 
-template <int CG, int BN>
-__device__ __forceinline__ Tile locate(const Params& p, const int* off, int i) {
+template <int CG, int BN, bool SPLIT>
+__device__ __forceinline__ Tile locate(const Params& p, const int* off, int i, int share) {
   using Cfg = Config<CG, BN>;
   const int nt = (p.N + BN - 1) / BN, mt = (p.M + Cfg::kTileM - 1) / Cfg::kTileM;
   Tile r;
@@ -117,6 +126,13 @@ __device__ __forceinline__ Tile locate(const Params& p, const int* off, int i) {
   r.k0 = off[r.g];
   r.kb = (count + BK - 1) / BK;
   r.last = count - (r.kb - 1) * BK;
+  r.rows = count;
+  if (SPLIT) {
+    const int lo = int(int64_t(r.kb) * share / p.parts), hi = int(int64_t(r.kb) * (share + 1) / p.parts);
+    if (hi != r.kb || lo == hi) r.last = BK;
+    r.k0 += lo * BK;
+    r.kb = hi - lo;
+  }
   return r;
 }
 
@@ -153,9 +169,10 @@ __device__ __forceinline__ void bulk_store_3d(const CUtensorMap* map, uint32_t b
                  : "memory");
 }
 
-template <int CG, int BN>
+template <int CG, int BN, bool SPLIT = false>
 __device__ __forceinline__ void mainloop(const Params& p) {
   using Cfg = Config<CG, BN>;
+  static_assert(!SPLIT || (CG == 1 && 16 * 4096 <= Cfg::kStages * Cfg::kStageBytes), "split sums");
   static_assert(CG == 1 || BN == 256, "SM pairs compute 256 x 256 tiles");
   constexpr int S = Cfg::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -168,8 +185,10 @@ __device__ __forceinline__ void mainloop(const Params& p) {
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? gemm2::cluster_ctarank() : 0u;
-  const int unit = CG == 2 ? blockIdx.x >> 1 : blockIdx.x;
-  const int units = CG == 2 ? gridDim.x >> 1 : gridDim.x;
+  // SPLIT: a unit is a cluster of p.parts CTAs, and there are as many units as tiles
+  const int share = SPLIT ? int(gemm2::cluster_ctarank()) : 0;
+  const int unit = CG == 2 ? blockIdx.x >> 1 : SPLIT ? blockIdx.x / p.parts : blockIdx.x;
+  const int units = CG == 2 ? gridDim.x >> 1 : SPLIT ? gridDim.x / p.parts : gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -224,7 +243,7 @@ __device__ __forceinline__ void mainloop(const Params& p) {
       uint32_t issued = 0, part = 0, partial = 0;  // per stage: phase bit of part_full, last use was partial
       bool ok = true;
       for (int i = unit; i < tiles && ok; i += units) {
-        const Tile t = locate<CG, BN>(p, off, i);
+        const Tile t = locate<CG, BN, SPLIT>(p, off, i, share);
         const int m0 = t.m0 + int(rank) * 128, n0 = t.n0 + int(rank) * Cfg::kBRows;
         int k0 = t.k0;
         for (int kb = 0; kb < t.kb; ++kb, k0 += BK, ring.next(), ++issued) {
@@ -275,7 +294,7 @@ __device__ __forceinline__ void mainloop(const Params& p) {
       const uint64_t a_desc = gemm::desc_mnmajor(smem_u32(smem));
       const uint64_t b_desc = gemm::desc_mnmajor(smem_u32(smem) + Cfg::kABytes);
       for (int i = unit; i < tiles && ok; i += units) {
-        const Tile t = locate<CG, BN>(p, off, i);
+        const Tile t = locate<CG, BN, SPLIT>(p, off, i, share);
         for (int c0 = 0; c0 < t.kb && ok; c0 += kChain, ++tc) {
           const int b = tc & 1, c1 = min(c0 + kChain, t.kb);
           if (!mbar_wait(&bars->tmem_empty[b], ((tc >> 1) & 1) ^ 1, status, 320)) { ok = false; break; }
@@ -318,7 +337,7 @@ __device__ __forceinline__ void mainloop(const Params& p) {
       // ---------------- Foreign rows ----------------
       uint32_t it = 0, part = 0;  // steps before and in this tile; phase bit of each stage's part_full
       for (int i = unit; i < tiles; i += units) {
-        const Tile t = locate<CG, BN>(p, off, i);
+        const Tile t = locate<CG, BN, SPLIT>(p, off, i, share);
         it += t.kb;
         if (t.kb == 0 || !t.patched()) continue;
         const int s = (it - 1) % S;
@@ -346,10 +365,10 @@ __device__ __forceinline__ void mainloop(const Params& p) {
     const int half = (warp - 4) >> 2;
     const uint32_t buf = smem_u32(epi_smem) + uint32_t((warp - 4) * Cfg::kBuf);
     int tc = 0;
-    bool ok = true;
+    bool ok = true, joined = false;
     for (int i = unit; i < tiles && ok; i += units) {
-      const Tile t = locate<CG, BN>(p, off, i);
-      if (t.kb == 0 && p.accumulate) continue;
+      const Tile t = locate<CG, BN, SPLIT>(p, off, i, share);
+      if (t.rows == 0 && p.accumulate) continue;
       float acc[kCols];
 #pragma unroll
       for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
@@ -373,13 +392,44 @@ __device__ __forceinline__ void mainloop(const Params& p) {
           for (int j = 0; j < 32; ++j) acc[c * 32 + j] += __uint_as_float(r[j]);
         }
       }
+      if (SPLIT) {
+        // box q of the tile, column j of lane's row: 4 bytes per lane (the ring is free: its steps are summed)
+        const uint32_t mine = smem_u32(smem) + uint32_t(lane * 4);
+        const int q0 = (warp - 4) * (kCols / 32);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+#pragma unroll
+          for (int c = 0; c < kCols / 32; ++c)
+            if ((q0 + c) % p.parts != share) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + uint32_t((q0 + c) * 4096 + j * 128)),
+                             "f"(acc[c * 32 + j])
+                             : "memory");
+            }
+        }
+        cluster_barrier();
+        joined = true;
+        if (ok) {
+#pragma unroll
+          for (int c = 0; c < kCols / 32; ++c)
+            if ((q0 + c) % p.parts == share) {
+              for (int o = 0; o < p.parts; ++o) {
+                if (o == share) continue;
+                const uint32_t from = gemm2::mapa(mine + uint32_t((q0 + c) * 4096), uint32_t(o));
+#pragma unroll
+                for (int j = 0; j < 32; ++j) acc[c * 32 + j] += load_cluster(from + uint32_t(j * 128));
+              }
+            }
+        }
+      }
       if (!ok) break;
       const int row0 = t.m0 + int(rank) * 128 + quarter * 32;
       if (row0 >= p.M) continue;
 #pragma unroll
       for (int c = 0; c < kCols / 32; ++c) {
         const int col = t.n0 + half * kCols + c * 32;
-        if (col < p.N) {
+        if (col < p.N && (!SPLIT || ((warp - 4) * (kCols / 32) + c) % p.parts == share)) {
           // the bulk store that last read the buffer is done with it
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
@@ -399,9 +449,17 @@ __device__ __forceinline__ void mainloop(const Params& p) {
         }
       }
     }
+    if (SPLIT) {
+      if (!joined) cluster_barrier();
+      cluster_barrier();  // no CTA leaves while its sums are read
+    }
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
+  if (SPLIT && warp < 4) {  // the epilogue's two barriers
+    cluster_barrier();
+    cluster_barrier();
+  }
   tc_fence_before();
   __syncthreads();
   if (CG == 2) {

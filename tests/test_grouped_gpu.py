@@ -250,6 +250,36 @@ def test_long_sums_of_few_tiles(cuda, terms, counts, tile):
     _status_ok()
 
 
+@pytest.mark.parametrize("tile", [0, 128])
+@pytest.mark.parametrize("counts", [[1027], [5000, 3, 0, 1], [0, 0, 3500], [9, 4000], [1100] * 5, [64, 8128]])
+@pytest.mark.parametrize("N,K", [(8, 8), (72, 264), (520, 136)])
+def test_weight_gradient_of_few_tiles(cuda, N, K, counts, tile):
+    """Tiles whose rows several blocks share, groups shorter than the shares too."""
+    import torch
+    from tempname_dcu_b200.ops import grouped
+    torch.manual_seed(N + len(counts))
+    off = _offsets(counts, cuda, start=2)
+    spans = list(zip(off.tolist(), off.tolist()[1:]))
+    dy, x = _bf(sum(counts) + 5, N + 8, device=cuda)[:, :N], _bf(sum(counts) + 5, K + 8, device=cuda)[:, 8:]
+    for t in (dy, x):
+        t[:2] = float("nan")
+        t[-3:] = float("inf")
+    exact = torch.stack([dy[a:c].double().t() @ x[a:c].double() for a, c in spans])
+    size = torch.stack([dy[a:c].double().abs().t() @ x[a:c].double().abs() for a, c in spans])
+    base = torch.randn(len(counts), N, K, device=cuda)
+    acc = base.clone()
+    grouped.weight_grad(dy, x, off, acc, accumulate=True, tile=tile)
+    assert _within(acc, exact + base.double(), size + base.double().abs(), max(counts), 2.0 ** -24)
+    fresh = torch.full_like(base, float("nan"))
+    grouped.weight_grad(dy, x, off, fresh, accumulate=False, tile=tile)
+    assert _within(fresh, exact, size, max(counts), 2.0 ** -24)
+    assert torch.equal(fresh, grouped.weight_grad(dy, x, off, tile=tile))
+    for g, n in enumerate(counts):
+        if n == 0:
+            assert torch.equal(acc[g], base[g]) and (fresh[g] == 0).all()
+    _status_ok()
+
+
 @pytest.mark.parametrize("counts", [[5000, 3, 0, 1], [0, 0], [9, 4000], [130] * 40])
 @pytest.mark.parametrize("N", [8, 72, 1000, 4096])
 def test_bias_gradient_of_long_groups(cuda, counts, N):
