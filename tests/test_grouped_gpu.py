@@ -280,6 +280,40 @@ def test_weight_gradient_of_few_tiles(cuda, N, K, counts, tile):
     _status_ok()
 
 
+def test_shared_sums_captured_on_two_streams(cuda):
+    """Calls whose sums several blocks share, first made inside a capture; two graphs at once."""
+    import torch
+    from tempname_dcu_b200.ops import grouped
+    torch.manual_seed(8)
+    off = _offsets([40, 0, 1500, 20], cuda)
+    x, w = _bf(1560, 2056, device=cuda), _bf(4, 40, 2056, device=cuda, scale=0.1)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs, outs = [], []
+    for s in streams:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            y = grouped.linear(x, w, off)
+            outs.append((y, grouped.weight_grad(y, x, off), grouped.matmul_nt(y, w, off)))
+        graphs.append(g)
+    x.copy_(_bf(1560, 2056, device=cuda))
+    off.copy_(_offsets([0, 1000, 60, 500], cuda))
+    torch.cuda.synchronize()
+    for s, g in zip(streams, graphs):
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                g.replay()
+    torch.cuda.synchronize()
+    y = grouped.linear(x, w, off)
+    for got in outs:
+        for have, want in zip(got, (y, grouped.weight_grad(y, x, off), grouped.matmul_nt(y, w, off))):
+            assert torch.equal(have, want)
+    spans = list(zip(off.tolist(), off.tolist()[1:]))
+    exact = torch.cat([x[a:c].double() @ w[g].double().t() for g, (a, c) in enumerate(spans)])
+    size = torch.cat([x[a:c].double().abs() @ w[g].double().abs().t() for g, (a, c) in enumerate(spans)])
+    assert _within(y, exact, size, 2056)
+    _status_ok()
+
+
 @pytest.mark.parametrize("counts", [[5000, 3, 0, 1], [0, 0], [9, 4000], [130] * 40])
 @pytest.mark.parametrize("N", [8, 72, 1000, 4096])
 def test_bias_gradient_of_long_groups(cuda, counts, N):
