@@ -161,13 +161,18 @@ static bool fills(int64_t tiles, int64_t slots) { return 2 * tiles >= slots; }
 // idle, with 64 rows each 13.1 / 14.3 / 14.8, 160: 13.8 / 15.4 / 17.0.  Tiles of
 // 128 rows whose long sums CTAs share fill the SMs as well: 2 groups of 500 rows,
 // 520 x 8192, 40 / 25; 300 rows of 1024 x 2048 in 2 groups, 11.0 / 10.6.
+// Where CTAs cannot share them, SM pairs win long sums even when they fill less:
+// 1024 x 2048 x 8192, 32 pairs, 54 / 43 with 128 / 512, with 2048 summed values
+// 17.4 / 16.6, with 1024 10.7 / 12.1; 24 pairs 54 / 43.
 static int pick_rows_tile(int64_t rows, int64_t groups, int N, int steps) {
   const int64_t used = rows < groups ? rows : groups;
   const int64_t average = used > 0 ? (rows + used - 1) / used : 0;
   const int sms = tdb_host::sm_count();
-  if (average >= 128 && N >= 256 && fills(used * ((average + 255) / 256) * ((N + 255) / 256), sms / 2)) return 512;
+  const int64_t pairs = used * ((average + 255) / 256) * ((N + 255) / 256);
+  const int64_t tiles = used * ((average + 127) / 128) * ((N + 127) / 128);
+  if (average >= 128 && N >= 256 && (fills(pairs, sms / 2) || (steps >= 32 && tiles * 2 > sms))) return 512;
   const int shares = steps >= 32 ? (steps >= 128 ? 8 : steps / 16) : 1;
-  if (average > 32 && fills(used * ((average + 127) / 128) * ((N + 127) / 128) * shares, sms)) return 128;
+  if (average > 32 && fills(tiles * shares, sms)) return 128;
   return 32;
 }
 
