@@ -1,0 +1,54 @@
+"""What the experts' entry points promise beside their results: outputs of a
+refused call stay as they were, limits of GELU and its slope, cost of routing
+in proportion to the tokens, results under a grid limit."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("call", ["linear", "few", "gelu", "data", "weight", "weight_acc", "bias", "bias_acc"])
+@pytest.mark.parametrize("values", [[0, 40, 65], [0, 50, 20], [-1, 10, 64], [0, 64, 80], [70, 70, 70]])
+def test_bad_offsets_leave_the_outputs(cuda, values, call):
+    import torch
+    from tempname_dcu_b200.ops import grouped, native
+    rows = 16 if call == "few" else 64
+    bf = lambda *s: torch.randn(*s, device=cuda).to(torch.bfloat16)
+    x, w = bf(rows, 64), bf(2, 64, 64)
+    off = torch.tensor(values, dtype=torch.int32, device=cuda)
+    native.clear_status()
+    if call in ("linear", "few", "gelu", "data"):
+        outs = [torch.full((rows, 64), 7.0, device=cuda, dtype=torch.bfloat16) for _ in range(2)]
+        if call == "data":
+            grouped.matmul_nt(x, w, off, out=outs[0])
+        elif call == "gelu":
+            grouped.linear_gelu(x, w, off, out=outs[0], pre_out=outs[1])
+        else:
+            grouped.linear(x, w, off, out=outs[0], tile=16 if call == "few" else 0)
+    else:
+        shape = (2, 64, 64) if call.startswith("weight") else (2, 64)
+        outs = [torch.full(shape, 7.0, device=cuda)]
+        grad = grouped.weight_grad if call.startswith("weight") else grouped.bias_grad
+        grad(x, *([x] if call.startswith("weight") else []), off, outs[0], accumulate=call.endswith("acc"))
+    with pytest.raises(native.NativeError):
+        native.raise_on_status()
+    assert all((t == 7).all() for t in outs)
+
+
+@pytest.mark.parametrize("groups,width", [(2, 4096), (700, 64), (1024, 8)])
+def test_one_bad_offset_among_many_groups(cuda, groups, width):
+    """Also where each group has its own blocks, and where the fault lies in the last of many entries."""
+    import torch
+    from tempname_dcu_b200.ops import grouped, native
+    dy = torch.randn(2048, width, device=cuda).to(torch.bfloat16)
+    good = torch.arange(groups + 1, dtype=torch.int32, device=cuda)
+    for at, value in ((groups, 2049), (groups, 0), (0, -1), (groups // 2, 2048)):
+        off = good.clone()
+        off[at] = value
+        for accumulate in (False, True):
+            native.clear_status()
+            out = torch.full((groups, width), 7.0, device=cuda)
+            grouped.bias_grad(dy, off, out, accumulate=accumulate)
+            with pytest.raises(native.NativeError):
+                native.raise_on_status()
+            assert (out == 7).all()
+    native.clear_status()
