@@ -13,8 +13,8 @@
 // result does not depend on the order of execution.
 //
 // Routing is bound by the instructions of the selection, not by memory: 16384
-// tokens, 128 experts, top 8 take 16.3 us (two launches), up to 128 tokens one
-// launch of 4.5 us, the gradient 3.5 us.
+// tokens, 128 experts, top 8 take 16.3 us (two launches), 2^20 tokens 656 us
+// (three), up to 128 tokens one launch of 4.5 us, the gradient 3.5 us.
 //
 // Exchange.  dispatch copies token rows to their k grouped rows, combine forms
 // the weighted sum of a token's k rows; each is the other's gradient.  All four
@@ -274,7 +274,60 @@ __global__ void __launch_bounds__(kRouteThreads) choose_kernel(const T* __restri
   rank_choices(s_ids, 0, tokens * k, E, start, wh, order, slots);
 }
 
-// Slots of one block's choices from every block's counts.
+// Running sums of the counts along the blocks, in place: hist[b][e] becomes the
+// choices of expert e in the blocks up to b.  A block takes 8 experts (a row's
+// 32 bytes) with 128 threads each; a thread reads its share of the rows twice,
+// first for the shares' sums.
+constexpr int kScanExperts = 8;
+constexpr int kScanShares = kRouteThreads / kScanExperts;
+
+__global__ void __launch_bounds__(kRouteThreads) scan_kernel(int* hist, int blocks, int E) {
+  __shared__ int sums[kScanExperts][kScanShares];
+  const int col = threadIdx.x % kScanExperts, share = threadIdx.x / kScanExperts;
+  const int e = blockIdx.x * kScanExperts + col;
+  const int per = (blocks + kScanShares - 1) / kScanShares;
+  const int lo = min(share * per, blocks), hi = e < E ? min(lo + per, blocks) : lo;
+  int* column = hist + e;
+  int sum = 0;
+#pragma unroll 8
+  for (int b = lo; b < hi; ++b) sum += column[int64_t(b) * E];
+  sums[col][share] = sum;
+  __syncthreads();
+  if (threadIdx.x < kScanExperts * 32) {  // a warp per expert, four shares per lane
+    const int lane = threadIdx.x & 31;
+    int* row = sums[threadIdx.x >> 5] + lane * 4;
+    const int n[4] = {row[0], row[1], row[2], row[3]};
+    const int all = n[0] + n[1] + n[2] + n[3];
+    int run = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    run -= all;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      row[i] = run;
+      run += n[i];
+    }
+  }
+  __syncthreads();
+  int run = sums[col][share];
+  for (int b0 = lo; b0 < hi; b0 += 8) {
+    int n[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n[i] = b0 + i < hi ? column[int64_t(b0 + i) * E] : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      run += n[i];
+      if (b0 + i < hi) column[int64_t(b0 + i) * E] = run;
+    }
+  }
+}
+
+// Slots of one block's choices.  hist holds every block's counts, which each
+// block adds up for itself, or (SCANNED) their running sums.
+template <bool SCANNED>
 __global__ void __launch_bounds__(kRouteThreads) group_kernel(const int* __restrict__ ids, const int* __restrict__ hist,
                                                               int blocks, int tokens, int E, int k,
                                                               int* __restrict__ offsets, int* __restrict__ order,
@@ -287,30 +340,37 @@ __global__ void __launch_bounds__(kRouteThreads) group_kernel(const int* __restr
   __shared__ int s_ids[kTokensPerBlock * kMaxTopK];
   const int t0 = blockIdx.x * kTokensPerBlock, t1 = min(t0 + kTokensPerBlock, tokens);
   for (int i = threadIdx.x; i < (t1 - t0) * k; i += kRouteThreads) s_ids[i] = ids[int64_t(t0) * k + i];
-  for (int e = threadIdx.x; e < E; e += kRouteThreads) total[e] = before[e] = 0;
-  __syncthreads();
-  // A thread sums the counts of one expert over every `groups`-th block, eight
-  // loads at a time (each is an L2 round trip).
-  const int wide = (E + 31) / 32 * 32;
-  const int groups = kRouteThreads / wide;
-  const int part = threadIdx.x / wide, e = threadIdx.x % wide;
-  if (part < groups && e < E) {
-    int all = 0, mine = 0;
-    for (int b0 = part; b0 < blocks; b0 += 8 * groups) {
-      int n[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int b = b0 + i * groups;
-        n[i] = b < blocks ? __ldg(hist + int64_t(b) * E + e) : 0;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        all += n[i];
-        mine += b0 + i * groups < int(blockIdx.x) ? n[i] : 0;
-      }
+  if (SCANNED) {
+    for (int e = threadIdx.x; e < E; e += kRouteThreads) {
+      total[e] = __ldg(hist + int64_t(blocks - 1) * E + e);
+      before[e] = blockIdx.x ? __ldg(hist + int64_t(blockIdx.x - 1) * E + e) : 0;
     }
-    atomicAdd(&total[e], all);
-    atomicAdd(&before[e], mine);
+  } else {
+    for (int e = threadIdx.x; e < E; e += kRouteThreads) total[e] = before[e] = 0;
+    __syncthreads();
+    // A thread sums the counts of one expert over every `groups`-th block, eight
+    // loads at a time (each is an L2 round trip).
+    const int wide = (E + 31) / 32 * 32;
+    const int groups = kRouteThreads / wide;
+    const int part = threadIdx.x / wide, e = threadIdx.x % wide;
+    if (part < groups && e < E) {
+      int all = 0, mine = 0;
+      for (int b0 = part; b0 < blocks; b0 += 8 * groups) {
+        int n[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int b = b0 + i * groups;
+          n[i] = b < blocks ? __ldg(hist + int64_t(b) * E + e) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          all += n[i];
+          mine += b0 + i * groups < int(blockIdx.x) ? n[i] : 0;
+        }
+      }
+      atomicAdd(&total[e], all);
+      atomicAdd(&before[e], mine);
+    }
   }
   __syncthreads();
   if (threadIdx.x < 32) scan_experts(total, start, E);
@@ -626,6 +686,14 @@ static bool bad_rows(const void* p, int64_t ld, int H) {
   return !p || reinterpret_cast<uintptr_t>(p) % 16 || ld % 8 || ld < H;
 }
 
+// Whether the blocks' counts are summed once, by a launch of its own, instead of
+// by every block of group_kernel, whose reads grow with the square of the
+// tokens.  Microseconds of the whole call, by every block / once: 128 experts,
+// top 8, 16384 tokens 16.4 / 16.9, 24576 28.0 / 26.5, 65536 65 / 49, 2^20 4697 /
+// 656; 8 experts, top 2, 32768 15.8 / 16.2, 65536 31 / 28; 512 experts, top 8,
+// 4096 38.8 / 39.3, 16384 42.6 / 39.9.
+static bool scan_counts(int blocks, int E) { return blocks > 256 || int64_t(blocks) * E > 16384; }
+
 template <typename T>
 static int route(const T* logits, int64_t ld, int tokens, int E, int k, int normalize, int* ids, float* weights,
                  int* offsets, int* order, int* slots, int* hist, cudaStream_t s) {
@@ -642,9 +710,15 @@ static int route(const T* logits, int64_t ld, int tokens, int E, int k, int norm
 #undef TDB_CHOOSE
   tdb_host::launched(1);
   if (blocks > 1) {
-    group_kernel<<<blocks, kRouteThreads, size_t(3 * E + 1 + kRankWarps * E) * 4, s>>>(ids, hist, blocks, tokens, E, k,
-                                                                                      offsets, order, slots);
-    tdb_host::launched(1);
+    const size_t tables = size_t(3 * E + 1 + kRankWarps * E) * 4;
+    if (scan_counts(blocks, E)) {
+      scan_kernel<<<(E + kScanExperts - 1) / kScanExperts, kRouteThreads, 0, s>>>(hist, blocks, E);
+      group_kernel<true><<<blocks, kRouteThreads, tables, s>>>(ids, hist, blocks, tokens, E, k, offsets, order, slots);
+      tdb_host::launched(2);
+    } else {
+      group_kernel<false><<<blocks, kRouteThreads, tables, s>>>(ids, hist, blocks, tokens, E, k, offsets, order, slots);
+      tdb_host::launched(1);
+    }
   }
   return int(cudaGetLastError());
 }

@@ -52,3 +52,45 @@ def test_one_bad_offset_among_many_groups(cuda, groups, width):
                 native.raise_on_status()
             assert (out == 7).all()
     native.clear_status()
+
+
+def _route_time(tokens, experts, top_k):
+    """Shortest of five calls, in milliseconds."""
+    import torch
+    from tempname_dcu_b200.ops import moe
+    z = torch.randn(tokens, experts, device="cuda")
+    moe.route(z, top_k)
+    best = float("inf")
+    for _ in range(5):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        moe.route(z, top_k)
+        end.record()
+        torch.cuda.synchronize()
+        best = min(best, start.elapsed_time(end))
+    return best
+
+
+def test_routing_time_grows_with_the_tokens(cuda):
+    """Eight times the tokens take eight times the time; 24 leaves room for a
+    busy machine, and a cost of their square (64) fails."""
+    assert _route_time(2 ** 20, 128, 2) < 24 * _route_time(2 ** 17, 128, 2)
+
+
+@pytest.mark.parametrize("tokens,experts,top_k", [(16384, 128, 2), (16385, 7, 3), (20001, 512, 1), (65535, 60, 4),
+                                                  (65536 * 3 + 1, 8, 2), (2 ** 20 + 77, 33, 1)])
+def test_many_tokens_against_a_sort(cuda, tokens, experts, top_k):
+    import torch
+    from tempname_dcu_b200.ops import moe
+    torch.manual_seed(tokens)
+    z = torch.randn(tokens, experts, device=cuda)
+    z[: tokens // 3, 0] += 8  # a long stretch of tokens that choose one expert
+    for _ in range(2):
+        r = moe.route(z, top_k)
+        ids = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :top_k]
+        assert torch.equal(r.ids.long(), ids)
+        order = torch.sort(ids.reshape(-1), stable=True).indices
+        assert torch.equal(r.order.long(), order)
+        assert torch.equal(r.slots.long()[order], torch.arange(order.numel(), device=cuda))
+        counts = torch.bincount(ids.reshape(-1), minlength=experts)
+        assert r.offsets[0] == 0 and torch.equal(r.offsets[1:].long(), counts.cumsum(0))
