@@ -32,6 +32,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kRouteThreads = 1024;    // routing: 32 warps
 constexpr int kTokensPerBlock = 128;   // four tokens per warp; up to 128 tokens are routed by one launch
+constexpr int kMaxTokens = 0x7fffffff - 1024;  // tokens of the block after the last one stay 32-bit
 constexpr int kRankWarps = 8;          // warps that rank a block's choices
 
 // Monotone map float -> uint32 (larger float, larger key); both zeros map to
@@ -188,18 +189,19 @@ __device__ __forceinline__ void scan_experts(const int* total, int* start, int E
   if (lane == 31) start[E] = inc;
 }
 
-// Stable ranks of the block's choices [c0, c1): base[e] is the first slot of
-// the block's choices of expert e.  Warp w < kRankWarps owns a contiguous
+// Stable ranks of the block's `count` choices from c0 on: base[e] is the first
+// slot of the block's choices of expert e.  Warp w < kRankWarps owns a contiguous
 // share, so ranks follow the choice index.  wh: [kRankWarps][E] shared ints.
-// ids: the block's choices in shared memory, ids[c - c0].
-__device__ __forceinline__ void rank_choices(const int* ids, int c0, int c1, int E, const int* base, int* wh,
+// ids: the block's choices in shared memory.  Indices count from c0, so that none
+// leaves 32 bits where the last choices are near 2^31.
+__device__ __forceinline__ void rank_choices(const int* ids, int c0, int count, int E, const int* base, int* wh,
                                              int* __restrict__ order, int* __restrict__ slots) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int share = ((c1 - c0 + kRankWarps - 1) / kRankWarps + 31) / 32 * 32;
-  const int lo = warp < kRankWarps ? min(c0 + warp * share, c1) : c1, hi = min(lo + share, c1);
+  const int share = ((count + kRankWarps - 1) / kRankWarps + 31) / 32 * 32;
+  const int lo = warp < kRankWarps ? min(warp * share, count) : count, hi = min(lo + share, count);
   for (int i = threadIdx.x; i < kRankWarps * E; i += kRouteThreads) wh[i] = 0;
   __syncthreads();
-  for (int c = lo + lane; c < hi; c += 32) atomicAdd(&wh[warp * E + ids[c - c0]], 1);
+  for (int c = lo + lane; c < hi; c += 32) atomicAdd(&wh[warp * E + ids[c]], 1);
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kRouteThreads) {
     int run = base[e];
@@ -214,15 +216,15 @@ __device__ __forceinline__ void rank_choices(const int* ids, int c0, int c1, int
   for (int c = lo; c < hi; c += 32) {
     const int mine = c + lane;
     const bool on = mine < hi;
-    const int id = on ? ids[mine - c0] : -1;
+    const int id = on ? ids[mine] : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, id);
     int first = 0;
     if (on) first = wh[warp * E + id];
     __syncwarp();
     if (on) {
       const int slot = first + __popc(same & ((1u << lane) - 1u));
-      slots[mine] = slot;
-      order[slot] = mine;
+      slots[c0 + mine] = slot;
+      order[slot] = c0 + mine;
       if ((same >> lane) == 1u) wh[warp * E + id] = slot + 1;  // the last of its group
     }
     __syncwarp();
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(kRouteThreads) group_kernel(const int* __restr
     for (int i = threadIdx.x; i <= E; i += kRouteThreads) offsets[i] = start[i];
   for (int i = threadIdx.x; i < E; i += kRouteThreads) before[i] += start[i];
   __syncthreads();
-  rank_choices(s_ids, t0 * k, t1 * k, E, before, wh, order, slots);
+  rank_choices(s_ids, t0 * k, (t1 - t0) * k, E, before, wh, order, slots);
 }
 
 __device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
@@ -741,10 +743,10 @@ static int route_bwd(const T* logits, int64_t ld, int tokens, int E, int k, int 
 
 static int check_route(const char* what, int64_t ld, int tokens, int E, int k) {
   if (tokens < 0 || E < 1 || E > kMaxExperts || k < 1 || k > kMaxTopK || k > E || ld < E ||
-      int64_t(tokens) * k >= (int64_t(1) << 31))
+      int64_t(tokens) * k >= (int64_t(1) << 31) || tokens > kMaxTokens)
     return tdb_host::fail(int(cudaErrorInvalidValue),
-                          "%s: 1..%d experts, 1..%d choices per token (at most the experts), tokens * choices < 2^31", what,
-                          kMaxExperts, kMaxTopK);
+                          "%s: 1..%d experts, 1..%d choices per token (at most the experts), tokens * choices < 2^31, at "
+                          "most %d tokens", what, kMaxExperts, kMaxTopK, kMaxTokens);
   return 0;
 }
 

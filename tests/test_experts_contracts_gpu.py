@@ -94,3 +94,24 @@ def test_many_tokens_against_a_sort(cuda, tokens, experts, top_k):
         assert torch.equal(r.slots.long()[order], torch.arange(order.numel(), device=cuda))
         counts = torch.bincount(ids.reshape(-1), minlength=experts)
         assert r.offsets[0] == 0 and torch.equal(r.offsets[1:].long(), counts.cumsum(0))
+
+
+def test_choices_up_to_2_to_the_31(cuda):
+    """The most tokens that the router takes, with the most choices: the last
+    choice has the index 2^31 - 17.  Equal logits: every token chooses all
+    experts in order, so the row of choice (t, j) is j * tokens + t."""
+    import torch
+    from tempname_dcu_b200.ops import moe, native
+    T, k = 2 ** 27 - 1, 16
+    r = moe.route(torch.zeros(T, k, device=cuda, dtype=torch.bfloat16), k)
+    assert torch.equal(r.offsets.long(), torch.arange(k + 1, device=cuda) * T)
+    expert = torch.arange(k, device=cuda)
+    for t0 in (0, T // 2, T - 4000):
+        rows = slice(t0, t0 + 4000)
+        t = torch.arange(t0, min(t0 + 4000, T), device=cuda)
+        assert torch.equal(r.ids[rows].long(), expert.expand(t.numel(), k))
+        assert (r.weights[rows] == 1 / 16).all()
+        slots = expert * T + t[:, None]
+        assert torch.equal(r.slots.view(T, k)[rows].long(), slots)
+        assert torch.equal(r.order[slots.reshape(-1)].long(), (t[:, None] * k + expert).reshape(-1))
+    native.raise_on_status()
