@@ -343,33 +343,42 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4
 }
 
 // GELU and its derivative with the normal distribution function from Abramowitz
-// and Stegun's approximation 7.1.26 of erfc (|error| < 1.5e-7, an order below
-// half a bf16 step of values near 1): with z = |x| / sqrt 2, t = 1 / (1 + 0.3275911 z),
+// and Stegun's approximation 7.1.26 of erfc (|error| < 1.5e-7): with z = |x| /
+// sqrt 2, t = 1 / (1 + 0.3275911 z),
 //   erfc(z) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-z^2),
-// whose exponential is the density's too.  upper_tail is half of it, the
-// probability above |x|; then gelu(x) = max(x, 0) - |x| upper_tail(x), some 14
-// instructions.  At the power limit the epilogue's instructions are paid for in
-// the tensor cores' clock: 4096 rows through 16384 x 4096 with GELU 463 -> 452 us
-// against the form with a division, a selection and separate factors.
-__device__ __forceinline__ float upper_tail(float x, float z, float& e) {
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-0.72134752f * x * x));  // exp(-x^2 / 2)
+// whose exponential is the density's too.  Half of it is the probability above
+// |x|, so gelu(x) = max(x, 0) - |x| tail and gelu'(x) = 1 - v (x >= 0) or v (x <
+// 0) with v = tail - |x| density; nothing cancels where the results are small.
+// What is left is the formula's own error: below 1.5e-7 / 2 (times |x| for gelu)
+// anywhere, 5e-4 of gelu(x) at -4, 2.5e-3 at -5.5 (half a bf16 step is 2e-3 to
+// 4e-3), 3 % at -12, where gelu is 1e-32; an |x|^2 th part of that in gelu'(x).
+// Some 14 instructions each.  At the power limit the epilogue's instructions are
+// paid for in the tensor cores' clock: 4096 rows through 16384 x 4096 with GELU
+// 463 -> 452 us against the form with a division, a selection and separate factors.
+// |x| is cut at 1e30, since an infinity times its tail of 0 would be NaN; a NaN
+// stays one through the exponential.
+__device__ __forceinline__ float gelu_density(float x) {  // exp(-x^2 / 2)
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-0.72134752f * x * x));
+  return e;
+}
+__device__ __forceinline__ float gelu_tail(float z) {  // the probability above z over gelu_density(z)
   float t;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f * 0.70710678f, z, 1.f)));
   float q = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
   q = fmaf(t, q, 0.5f * 1.421413741f);
   q = fmaf(t, q, 0.5f * -0.284496736f);
   q = fmaf(t, q, 0.5f * 0.254829592f);
-  return t * q * e;
+  return t * q;
 }
 __device__ __forceinline__ float gelu(float x) {
-  float e;
-  const float z = fminf(fabsf(x), 1e30f);  // an infinity times its tail of 0 would be NaN (a NaN stays one through e)
-  return fmaf(-z, upper_tail(x, z, e), fmaxf(x, 0.f));
+  const float z = fminf(fabsf(x), 1e30f);
+  return fmaf(-z, gelu_tail(z) * gelu_density(x), fmaxf(x, 0.f));
 }
 __device__ __forceinline__ float gelu_slope(float x) {
-  float e;
-  const float cdf = 0.5f + copysignf(0.5f - upper_tail(x, fabsf(x), e), x);
-  return fmaf(0.3989422804f * x, e, cdf);
+  const float z = fminf(fabsf(x), 1e30f);
+  const float v = fmaf(-0.3989422804f, z, gelu_tail(z)) * gelu_density(x);
+  return x >= 0.f ? 1.f - v : v;
 }
 
 // One epilogue warp: 32 output columns (TMEM lanes) of a tile, 32 rows at a

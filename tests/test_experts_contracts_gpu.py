@@ -115,3 +115,27 @@ def test_choices_up_to_2_to_the_31(cuda):
         assert torch.equal(r.slots.view(T, k)[rows].long(), slots)
         assert torch.equal(r.order[slots.reshape(-1)].long(), (t[:, None] * k + expert).reshape(-1))
     native.raise_on_status()
+
+
+@pytest.mark.parametrize("tile", [32, 128, 512])
+def test_gelu_slope_at_its_limits(cuda, tile):
+    """The gradient is the slope itself where the product is 1.  Its formula is
+    off by less than 7.5e-8, fp32 adds 2^-24 near 1; below -4 the error is relative:
+    the tail's (3 % at -12) divided by x^2, far below 2^-10."""
+    import torch
+    from tempname_dcu_b200.ops import grouped
+    inf, nan = float("inf"), float("nan")
+    special = [inf, -inf, nan, 0.0, -0.0, 1e20, -1e20, 3e38, -3e38, 1e-30, -1e-30, 14.0, -14.0, 40.0, -40.0, 1.0]
+    pre = torch.cat([torch.tensor(special), torch.linspace(-12, 12, 2048 - 16)]).to(cuda, torch.bfloat16).view(32, 64)
+    dy, w = torch.zeros(32, 8, device=cuda, dtype=torch.bfloat16), torch.ones(1, 8, 64, device=cuda, dtype=torch.bfloat16)
+    dy[:, 3] = 1
+    off = torch.tensor([0, 32], dtype=torch.int32, device=cuda)
+    got = grouped.matmul_nt(dy, w, off, gelu_pre=pre, tile=tile).double().view(-1)
+    assert got[:2].tolist() == [1.0, 0.0] and got[2].isnan() and got[3:5].tolist() == [0.5, 0.5]
+    assert got[5:9].tolist() == [1.0, 0.0, 1.0, 0.0] and got[9:12].tolist() == [0.5, 0.5, 1.0]
+    x = pre.double().view(-1)[11:]
+    exact = 0.5 * torch.erfc(-x / 2 ** 0.5) + x * torch.exp(-x * x / 2) / (2 * torch.pi) ** 0.5
+    err = (got[11:] - exact).abs()
+    assert (err <= exact.abs() * 2.0 ** -8 + 1.5e-7).all()
+    low = (x <= -4) & (x >= -12)
+    assert low.sum() > 600 and (err[low] <= exact[low].abs() * (2.0 ** -8 + 2.0 ** -10)).all()
