@@ -28,6 +28,7 @@ using grouped::kMaxGroups;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;  // 256-value pieces of a row in flight per warp
+constexpr int kMaxK = 65535 * kBatch * 256;  // 2^26 - 1024: a grid has at most 65535 blocks along K
 
 // Block exponent from the bits of the largest |bf16|: the smallest e with
 // a <= 6 * 2^e = 1.5 * 2^(e + 2), at least -127 (also for 0 and subnormals).
@@ -255,11 +256,11 @@ static dim3 grid_for(int64_t rows, int64_t K, bool offsets) {
 }
 
 static int check(const char* what, int64_t matrices, int64_t rows, int64_t K, int groups, const void* offsets) {
-  if (matrices < 1 || rows < 0 || K < 32 || K % 32 || K >= (int64_t(1) << 26) || rows >= (int64_t(1) << 31) ||
+  if (matrices < 1 || rows < 0 || K < 32 || K % 32 || K > kMaxK || rows >= (int64_t(1) << 31) ||
       matrices >= (int64_t(1) << 31) || matrices * rows >= (int64_t(1) << 31) ||
       (offsets && (groups < 1 || groups > kMaxGroups || matrices != 1)))
-    return tdb_host::fail(int(cudaErrorInvalidValue), "%s: K must be a multiple of 32 below 2^26; 1..%d groups of one matrix's rows",
-                          what, kMaxGroups);
+    return tdb_host::fail(int(cudaErrorInvalidValue), "%s: K must be a multiple of 32, at most %d; 1..%d groups of one matrix's rows",
+                          what, kMaxK, kMaxGroups);
   return 0;
 }
 
@@ -328,8 +329,9 @@ TDB_API int tdb_mx4_gemm(const void* qx, const void* sfx, const void* qw, const 
                          void* C, int64_t ldc, int rows, int N, int K, const void* bias, int tile, void* stream) {
   using namespace tdb::grouped;
   if (groups < 1 || groups > kMaxGroups || (!offsets && groups != 1) || rows < 0 || N <= 0 || N % 8 || K < 32 ||
-      K % 32 || K >= (1 << 26) || rows > kMaxExtent || N > kMaxExtent)
-    return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 product: 1..%d groups, N a multiple of 8, K of 32", kMaxGroups);
+      K % 32 || K > mx4::kMaxK || rows > kMaxExtent || N > kMaxExtent)
+    return tdb_host::fail(int(cudaErrorInvalidValue), "mx4 product: 1..%d groups, N a multiple of 8, K of 32 and at most %d",
+                          kMaxGroups, mx4::kMaxK);
   if (rows == 0) return 0;
   if (!qx || !sfx || !qw || !sfw || !C || ldc % 8 || ldc < N ||
       (reinterpret_cast<uintptr_t>(qx) | reinterpret_cast<uintptr_t>(sfx) | reinterpret_cast<uintptr_t>(qw) |

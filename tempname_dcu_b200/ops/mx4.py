@@ -9,7 +9,8 @@ block with an infinity or NaN decodes as NaN.  Two values share a byte (even K
 index low); scales are stored in 512-byte atoms as the tensor cores read them
 and are opaque to callers (``dequantize`` is the way back).
 
-Rows may be any number, K a multiple of 32, N of the products a multiple of 8.
+Rows may be any number, K a multiple of 32 up to 2^26 - 1024, N of the products
+a multiple of 8.
 ``offsets`` (int32 [groups + 1], on the device) are those of ``ops.grouped``:
 an operand quantized with offsets goes into ``grouped_linear`` with the same
 offsets.  Weights are quantized once, [N, K] or [groups, N, K].
@@ -37,6 +38,7 @@ native.register("tdb_mx4_gemm", [V, V, V, V, V, I, V, I64, I, I, I, V, I, V])
 
 E2M1_MAX = 6.0
 MAX_GROUPS = 1024
+MAX_K = 2 ** 26 - 1024
 
 
 def _groups(offsets, device):
@@ -69,8 +71,8 @@ def _operand(q, sf, groups, device, what):
     shape = q.shape
     matrices = shape[0] if len(shape) == 3 else 1
     rows, K = shape[-2], 2 * shape[-1]
-    if not (K > 0 and K % 32 == 0 and K < 2 ** 26 and rows < 2 ** 31):
-        raise ValueError(f"{what}: K must be a positive multiple of 32 below 2^26, and rows fewer than 2^31")
+    if not (0 < K <= MAX_K and K % 32 == 0 and rows < 2 ** 31):
+        raise ValueError(f"{what}: K must be a positive multiple of 32 up to {MAX_K}, and rows fewer than 2^31")
     if not (sf.dtype is torch.uint8 and sf.is_contiguous() and sf.get_device() == device and
             sf.numel() >= scale_bytes(rows, K, groups, matrices)):
         raise ValueError(f"the scales of {what} must be the uint8 buffer that quantize wrote for these rows (and "
@@ -89,8 +91,8 @@ def quantize(x, offsets=None, q=None, sf=None):
         raise ValueError("x must be [rows, K] or [matrices, rows, K] on a CUDA device")
     shape, stride = x.shape, x.stride()
     rows, K = shape[-2:]
-    if not (K > 0 and K % 32 == 0 and stride[-1] == 1):
-        raise ValueError("K must be a positive multiple of 32, the last dimension contiguous")
+    if not (0 < K <= MAX_K and K % 32 == 0 and stride[-1] == 1):
+        raise ValueError(f"K must be a positive multiple of 32 up to {MAX_K}, the last dimension contiguous")
     index = x.get_device()
     groups = _groups(offsets, index)
     matrices, ld = 1, stride[0] if rows > 1 else K

@@ -139,3 +139,22 @@ def test_gelu_slope_at_its_limits(cuda, tile):
     assert (err <= exact.abs() * 2.0 ** -8 + 1.5e-7).all()
     low = (x <= -4) & (x >= -12)
     assert low.sum() > 600 and (err[low] <= exact[low].abs() * (2.0 ** -8 + 2.0 ** -10)).all()
+
+
+def test_longest_4_bit_rows(cuda):
+    """The largest K: one row as an operand of a product of two rows' worth of ones."""
+    import torch
+    from tempname_dcu_b200.ops import mx4, native
+    K = mx4.MAX_K
+    x = torch.zeros(1, K, device=cuda, dtype=torch.bfloat16)
+    x[0, -1], x[0, 0], x[0, K // 2] = 3, 1, -0.5
+    q, sf = mx4.quantize(x)
+    assert torch.equal(mx4.dequantize(q, sf), x)
+    w = torch.zeros(8, K, device=cuda, dtype=torch.bfloat16)
+    w[:, -1] = torch.arange(8, device=cuda) % 4
+    w[:, 0] = 2
+    y = mx4.linear(q, sf, *mx4.quantize(w))
+    assert y.tolist() == [[2.0 + 3 * (n % 4) for n in range(8)]]
+    with pytest.raises(ValueError):
+        mx4.quantize(torch.empty(1, K + 32, device=cuda, dtype=torch.bfloat16))
+    native.raise_on_status()
