@@ -37,22 +37,29 @@ static int launch_rows_tile(int tile, const RowsParams& p, cudaStream_t s) {
   return launch_rows<1, 32, OP, MODE, false>(p, s);
 }
 
+// Bytes of the weights in use up to which the streaming kernel takes few rows: it
+// starts sooner, the tiles read faster.
+constexpr int64_t kFewBytes = 80 << 20;
+
 // Tile of a call.  Forward with few rows: the streaming kernel (16) while the
-// 128-column tiles of the groups that can have rows would leave SMs idle (two
-// experts of 4096 x 16384 and one token: 52 us against 80; 16384 x 4096, 256
-// tiles: 53 against 47).  Weight gradient: SM pairs (512) when the sums are long
-// enough to hide their larger tiles' output (8 groups of 4096 x 4096 with 256
-// rows each 126 us with 128, 137 with 512; 384: 168 and 140; 1024: 374 and 249)
-// and the tiles fill half of the pairs (8 of 512 x 512 with 1024 rows each: 11.5
-// and 14.0).
+// 128-column tiles of the groups that can have rows would leave SMs idle, also
+// where CTAs share their sums, and the weights are at most kFewBytes.
+// Microseconds with 16 / 32: one expert of 1024 x 1024 3.6 / 8.2, of 4096 x 4096
+// (34 MB) 10.4 / 14.2, two (67 MB) 17.3 / 18.2; two of 2048 x 8192 (67 MB) 17.1 /
+// 19.3, three (101 MB) 24.6 / 23.1; eight of 1024 x 8192 (134 MB) 31.0 / 27.3; two
+// of 4096 x 16384 (268 MB) 54 / 49; of 16384 x 4096, 256 tiles, 52 / 46.  Weight
+// gradient: SM pairs (512) when the sums are long enough to hide their larger
+// tiles' output (8 groups of 4096 x 4096 with 256 rows each 126 us with 128, 137
+// with 512; 384: 168 and 140; 1024: 374 and 249) and the tiles fill half of the
+// pairs (8 of 512 x 512 with 1024 rows each: 11.5 and 14.0).
 static int pick_tile(int op, int64_t rows, int groups, int M, int N) {
   if (op == kWeightGrad) {
     const int64_t tiles = int64_t(groups) * ((M + 255) / 256) * ((N + 255) / 256);
     return M >= 256 && N >= 256 && rows >= int64_t(groups) * 320 && fills(tiles, tdb_host::sm_count() / 2) ? 512 : 128;
   }
   if (op == kForward && rows <= kFewRows) {
-    const int64_t tiles = (rows < groups ? rows : groups) * ((N + 127) / 128);
-    if (tiles * 5 < int64_t(tdb_host::sm_count()) * 4) return 16;
+    const int64_t used = rows < groups ? rows : groups, tiles = used * ((N + 127) / 128);
+    if (tiles * 5 < int64_t(tdb_host::sm_count()) * 4 && used * N * M <= kFewBytes / 2) return 16;
   }
   return pick_rows_tile(rows, groups, N, (M + gemm::BK - 1) / gemm::BK);
 }

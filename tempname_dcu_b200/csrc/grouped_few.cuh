@@ -14,8 +14,9 @@
 // copies the pieces that it will use itself into its own slots of a ring in
 // shared memory (cp.async, up to 12 turns ahead, across units), so two blocks
 // keep some 190 KB of an SM's loads in flight and wait for no other thread.
-// One token through two experts of 4096 x 16384: 52 us (5.1 TB/s), of 1024 x
-// 1024: 3.6 us (the tcgen05 tiles: 80 and 8.1 us).
+// One token through two experts of 4096 x 4096: 17.3 us (3.9 TB/s), through one of
+// 1024 x 1024 3.6 us (the tcgen05 tiles, sums shared: 18.2 and 8.2 us); of larger
+// weights the tiles read faster (see pick_tile in grouped.cu).
 #pragma once
 #include "grouped_rows.cuh"
 
