@@ -72,7 +72,8 @@ struct SplitState {
 
 // Launches `kern` with a cluster of CTAs on each tile, its p.parts set: as many
 // as keep kSumSteps steps each while all tiles' clusters are resident.  Returns
-// -1 if the tiles fill the SMs or the sums are too short.  Measured, bf16,
+// -1 if the tiles fill the SMs, the sums are too short or the caller has only a
+// share of the SMs (clusters beyond it would not be resident).  Measured, bf16,
 // microseconds with 1 / 2 / 4 / 8 CTAs: 4 tiles of 32 rows, 8192 summed values,
 // 38.8 / 23.8 / 14.9 / 11.6; 66 tiles, 4096 values, 21.4 / 15.0 / 13.0 / 24.0
 // (not all resident); 45 tiles of 128 rows, 8192 values, 51 / 31 / 39 / 48, with

@@ -15,7 +15,8 @@ Operands are bf16 with 16-byte aligned rows (N, K and row strides multiples of
 8), sums fp32, outputs bf16 (gradients of parameters fp32).  Offsets that
 decrease or leave the rows are found on the device: the call computes nothing
 and ``native.raise_on_status`` raises.  Calls run on the current stream of the
-tensors' device and are deterministic.  ``tile`` asks for a tile shape (0: by
+tensors' device and are deterministic: equal calls give equal bits (a different
+``tile`` or ``native.grid_limit`` may add in another order).  ``tile`` asks for a tile shape (0: by
 the sizes; see ``pick_tile`` in csrc/grouped.cu), for measurements.
 """
 from __future__ import annotations

@@ -170,7 +170,9 @@ class grid_limit:
     GEMMs, fused collectives) launched inside, from this thread, use at most
     ``n`` CTAs (0: no cap), so that two of them on different streams share the
     SMs instead of queueing.  Launch geometry is fixed when a CUDA graph is
-    captured, so the cap also holds on replay."""
+    captured, so the cap also holds on replay.  Grouped and 4-bit products with
+    few tiles and long sums are summed by several CTAs per tile without a cap
+    and by one with it, so their last bits may depend on it."""
 
     def __init__(self, ctas):
         self.ctas = int(ctas)

@@ -158,3 +158,38 @@ def test_longest_4_bit_rows(cuda):
     with pytest.raises(ValueError):
         mx4.quantize(torch.empty(1, K + 32, device=cuda, dtype=torch.bfloat16))
     native.raise_on_status()
+
+
+def test_shared_sums_under_a_grid_limit(cuda):
+    """A limited grid shares no sums: the order of the additions differs from the
+    unlimited call's, so the results agree within their error and, among calls
+    of either kind, bit for bit."""
+    import torch
+    from tempname_dcu_b200.ops import grouped, mx4, native
+    torch.manual_seed(7)
+    K, rows = 4104, 1500
+    off = torch.tensor([0, 40, 40, 1480, rows], dtype=torch.int32, device=cuda)
+    spans = [(0, 40), (40, 40), (40, 1480), (1480, rows)]
+    x = torch.randn(rows, K, device=cuda).to(torch.bfloat16)
+    w = (torch.randn(4, 40, K, device=cuda) * 0.1).to(torch.bfloat16)
+    x4, w4 = torch.randn(40, 4096, device=cuda).to(torch.bfloat16), torch.randn(64, 4096, device=cuda).to(torch.bfloat16)
+    q4 = (*mx4.quantize(x4), *mx4.quantize(w4))
+
+    def calls():
+        y = grouped.linear(x, w, off)
+        return y, grouped.weight_grad(y, x, off), grouped.bias_grad(y, off), mx4.linear(*q4)
+    free, again = calls(), calls()
+    with native.grid_limit(20):
+        limited, repeated = calls(), calls()
+    assert all(torch.equal(a, b) for a, b in zip(free, again))
+    assert all(torch.equal(a, b) for a, b in zip(limited, repeated))
+    v4 = [mx4.dequantize(*q4[i:i + 2]).double() for i in (0, 2)]
+    for y, dw, db, y4 in (free, limited):
+        for g, (a, b) in enumerate(spans):
+            exact, size = x[a:b].double() @ w[g].double().t(), x[a:b].double().abs() @ w[g].double().abs().t()
+            assert ((y[a:b].double() - exact).abs() <= exact.abs() * 2.0 ** -8 + size * K * 2.0 ** -22).all()
+            exact = y[a:b].double().t() @ x[a:b].double()
+            assert (dw[g].double() - exact).norm() <= 2.0 ** -20 * exact.norm()  # see test_experts_exact_gpu.py
+        exact, size = v4[0] @ v4[1].t(), v4[0].abs() @ v4[1].abs().t()
+        assert ((y4.double() - exact).abs() <= exact.abs() * 2.0 ** -8 + size * 4096 * 2.0 ** -22).all()
+    native.raise_on_status()
