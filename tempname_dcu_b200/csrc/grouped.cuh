@@ -23,9 +23,14 @@
 // so the MMAs do not wait; chains of 256 rows cost 7 % more time.
 //
 // Bounds: short sums the fp32 output (8 groups of 128 rows, 4096 x 4096: 108 us,
-// 5 TB/s), long ones the tensor cores and the output's share of the same path
-// to memory (7 groups of 1170 rows: 287 us from a cool start, 316 us back to
-// back at the power limit, 0.87 PFLOP/s).
+// 5 TB/s), long ones the rate of the steps.  7 groups, 4096 x 4096, from a cool
+// start / back to back at the power limit (1.43 to 1.57 GHz at 990 W), us: 512
+// rows each 134 / 154, 1024 228 / 253, 2048 399 / 449, 4096 760 / 862, 8192 1498 /
+// 1706.  A group's row costs 26 ns (1.3 PFLOP/s cool, 1.14 at the limit), the
+// output 25 to 55 us that the sums do not hide, the partial steps of 1170 rows
+// some 18 us (272 / 303 in all).  Library products of the same operands with bf16
+// outputs take 658 / 743 us for 4096 rows (1.46 and 1.30 PFLOP/s); the chains and
+// the 256 x 256 tile's 64 KB of operands per step are what differs here.
 //
 // Few tiles with long sums (SPLIT, CG = 1): a cluster of CTAs computes one tile,
 // each a part of the group's steps.  The tile's 16 boxes of 32 x 32 values go to

@@ -313,6 +313,8 @@ class GPT:
         grouped.bias_grad(dz, off, self.Gr(p + "fc1_bias"), accumulate=acc)
         grouped.weight_grad(dz, xs, off, self.Gr(p + "fc1_weight"), accumulate=acc)
         dxs = grouped.matmul_nt(dz, self.P(p + "fc1_weight"), off)
+        # rounded to bf16 (half a step, 2^-9) for the two products that take it, like every gradient between
+        # layers; the logits themselves are fp32 because their order decides the routing
         dlogits = moe.route_bwd(logits, r, dweights,
                                 out=torch.empty(logits.shape, dtype=torch.bfloat16, device=logits.device))
         G.weight_grad(dlogits, ln2, self.Gr(p + "router_weight"), accumulate=acc)
